@@ -42,7 +42,7 @@
 extern "C" {
 #endif
 
-#define TRL_ABI_VERSION 8
+#define TRL_ABI_VERSION 9
 
 enum { TRL_F32 = 0, TRL_F64 = 1 };
 
@@ -483,6 +483,77 @@ int trl_vtrace_bwd_cpu(int val_dtype, int coef_dtype, const void *grad_advantage
 /* {N, sum, sumsq} of x (host double[3]) / (x - mean) / max(std, eps) from such statistics, as trl_moments / trl_normalize */
 int trl_moments_cpu(int dtype, const void *x, int64_t n, double *stats);
 int trl_normalize_cpu(int dtype, const void *x, int64_t n, const double *stats, double eps, void *out);
+
+/*
+ * Policies over tokens (ABI 9).  V-trace reads log_pi and log_mu; for a policy that picks tokens these are log-probabilities of
+ * the stored tokens under the distribution that was sampled from: the network's logits after penalties for repeated tokens, a
+ * bias, a temperature and a mask.  No counterpart in the reference's value path (its MaskedCategorical, torchrl/modules/
+ * distributions/discrete.py, masks the logits in ATen).  Device pointers, stream and errors as above.
+ *
+ * Rows (b, t): sequence b of B has T rows (T == 1: one decoding step).  For row r = b * T + t, token j, all in 32 bits:
+ *   c_j = how often j stands in tokens[b][0 .. lengths[r]),  n_j = how often in tokens[b][prompt[b] .. lengths[r])
+ *   z1 = c_j > 0 ? (z > 0 ? z / rep : z * rep) : z;   z2 = z1 - freq * n_j - (n_j > 0 ? pres : 0);   z3 = (z2 + bias_j) / temp
+ *   z' = mask_j ? z3 : -inf        (what stands in a masked place is never read: NaN and infinities there do no harm)
+ * Ids outside [0, V) in `tokens` are no tokens; lengths are clamped to [0, L].
+ */
+enum { TRL_BF16 = 2, TRL_F16 = 3 }; /* element types of these entry points, besides TRL_F32 */
+enum { TRL_MASK_NONE = 0, TRL_MASK_BOOL = 1, TRL_MASK_BITS = 2 }; /* a byte (0 / 1) a token; bit j % 32 of 32-bit word j / 32 */
+
+typedef struct trl_token_args {
+    int32_t dtype;                            /* of logits, out, grad_out: TRL_F32, TRL_BF16, TRL_F16 */
+    int32_t mask_kind;                        /* TRL_MASK_* */
+    int32_t bias_kind;                        /* 0: no bias, else 1 + its TRL_* type */
+    int32_t tokens_wide, lengths_wide, prompt_wide, action_wide; /* 1: 64-bit integers, 0: 32-bit */
+    float rep, pres, freq, temp;              /* scalars, where the arrays below are NULL */
+    int64_t B, T, V, L;
+    const void *logits;                       /* element (b, t, j) at b * logits_sb + t * logits_st + j */
+    int64_t logits_sb, logits_st;
+    const void *tokens;                       /* (B, L) with row stride tokens_sb, or NULL: no penalties */
+    int64_t tokens_sb;
+    const void *lengths;                      /* (B, T) dense, or NULL: L */
+    const void *prompt;                       /* (B,) dense, or NULL: 0 */
+    const float *rep_t, *pres_t, *freq_t, *temp_t; /* (B,) each, or NULL */
+    const void *bias;                         /* strides in BYTES; 0: shared */
+    int64_t bias_sb, bias_st;
+    const void *mask;                         /* strides in BYTES; 0: shared */
+    int64_t mask_sb, mask_st;
+    void *out;                                /* processed logits / gradient: strides in elements */
+    int64_t out_sb, out_st;
+    const void *grad_out;                     /* trl_process_logits_bwd: (B, T, V) dense */
+    const void *action;                       /* (B, T) dense; negative: a padded row */
+    float *log_prob, *entropy;                /* (B, T); entropy may be NULL */
+    float *stats;                             /* (B, T, 2): {max z' * log2(e), log2 of the sum}; written by the forward call, read by the backward */
+    const float *g_log_prob, *g_entropy;      /* (B, T) incoming gradients, either may be NULL (= zeros) */
+} trl_token_args;
+
+/* out = z' (one rounding to dtype); out may be the logits themselves (same strides), and must not overlap them otherwise.
+ * bwd: out = d_logits = grad_out * dz'/dz, 0 in masked places; reads the logits only where rep != 1 (their sign). */
+int trl_process_logits_fwd(void *stream, const trl_token_args *args);
+int trl_process_logits_bwd(void *stream, const trl_token_args *args);
+/* log_prob = log p[action], entropy = -sum p log p of p = softmax(z'), fused with the processing: one read of the logits.
+ * A negative action marks padding: 0, 0, no gradient, the row is not read.  A row with nothing allowed: -inf, 0, no gradient.  An
+ * action of V or more: NaN.  bwd (out = d_logits; needs stats and, with g_entropy, entropy from the forward call):
+ *   (g_lp ([j = action] - p_j) - g_H p_j (log p_j + H)) dz'/dz.
+ * workspace: trl_token_workspace_bytes(), 16-byte aligned, free again when the call's launches have run. */
+size_t trl_token_workspace_bytes(int64_t B, int64_t T, int64_t V);
+int trl_token_log_prob_fwd(void *stream, const trl_token_args *args, void *workspace, size_t workspace_bytes);
+int trl_token_log_prob_bwd(void *stream, const trl_token_args *args);
+
+/*
+ * Activations kept for the backward pass in 8 bits (ABI 9).  x is (N, D) with row stride x_stride (elements).  Blocks of 32
+ * features share a power of two: step = 2^(floor(log2 max|x|) - 6), not under 2^-126; code = x / step to nearest even, at most 127 in
+ * magnitude, so a value is off by half a step (within the last step below the clamp: by less than one).  `codes` is (N, Dp) with
+ * Dp = D rounded up to 32 (the rest zeros), `exponents` (N, Dp / 32): step = 2^(exponent - 127).  A block with a NaN or an infinity
+ * gets exponent 255 and stands for NaN.  Every value is exact in bfloat16 and in x's own type.
+ */
+int trl_act_quantize(void *stream, int dtype, const void *x, int64_t x_stride, int64_t N, int64_t D, int8_t *codes, uint8_t *exponents);
+int trl_act_dequantize(void *stream, int dtype, const int8_t *codes, const uint8_t *exponents, int64_t N, int64_t D, void *out);
+/* The weight gradient of a linear layer whose input was kept that way: dw (O, D) = dy (N, O)^T x^, and db (O) = column sums of dy
+ * (or NULL).  dy has row stride dy_stride (elements) and type dtype, as dw and db.  Sums in 32 bits, in a fixed order.
+ * workspace: trl_act_weight_grad_workspace_bytes(), 16-byte aligned, free again when the call's launches have run. */
+size_t trl_act_weight_grad_workspace_bytes(int dtype, int64_t N, int64_t O, int64_t D);
+int trl_act_weight_grad(void *stream, int dtype, const void *dy, int64_t dy_stride, const int8_t *codes, const uint8_t *exponents,
+                        int64_t N, int64_t O, int64_t D, void *dw, void *db, void *workspace, size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,382 @@
+"""GPU: process_logits and token_log_prob against plain 64-bit forms (tests/token_oracle.py), at the sizes and masks where they can go wrong."""
+import math
+
+import pytest
+import torch
+
+import token_oracle as O
+from torchrl_amd.objectives.value import CheckpointedLinear, RolloutData, TokenActor, VTrace, functional as F, process_logits, token_log_prob
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+KINDS = ["plain", "penalties", "bits", "bool", "all"]
+
+
+def make(kind, dtype, B, T, V, L=0, seed=0, monotonic=True, bias_dtype=torch.float32):
+    """CPU inputs of one call; T == 0: one decoding step.  Masked places hold NaN and infinities."""
+    g = torch.Generator().manual_seed(seed)
+    rows = max(T, 1)
+    z = (torch.randn(B, rows, V, generator=g) * 3).to(dtype)
+    c = {"z": z, "T": T, "kwargs": {}, "oracle": {}}
+    kw, o = c["kwargs"], c["oracle"]
+    if kind in ("penalties", "all") and L:
+        tokens = torch.randint(-2, V + 2, (B, L), generator=g)
+        common = torch.randint(0, V, (3,), generator=g)
+        tokens = torch.where(torch.rand(B, L, generator=g) < 0.4, common[torch.randint(0, 3, (B, L), generator=g)], tokens)
+        lengths = torch.randint(-1, L + 2, (B, rows), generator=g)
+        if monotonic:
+            lengths = lengths.sort(1).values
+        lengths[0, 0] = 0
+        prompt = torch.randint(0, L + 1, (B,), generator=g)
+        o.update(tokens=tokens, lengths=lengths, prompt=prompt, rep=1.3, pres=0.25, freq=0.125)
+        kw.update(tokens=tokens, lengths=lengths if T else lengths[:, 0], prompt_lengths=prompt, repetition_penalty=1.3, presence_penalty=0.25,
+                  frequency_penalty=0.125)
+    if kind == "all":
+        bias = torch.randn(B, 1, V, generator=g).to(bias_dtype)
+        o.update(bias=bias, temp=0.7)
+        kw.update(bias=bias if T else bias[:, 0], temperature=0.7)
+    if kind in ("bits", "bool", "all"):
+        mask = torch.rand(B, rows, V, generator=g) < torch.rand(B, rows, 1, generator=g)
+        mask[-1, -1] = False  # a row that allows nothing
+        if rows > 2:
+            mask[0, 1] = True
+        junk = torch.tensor([math.nan, math.inf, -math.inf])[torch.randint(0, 3, z.shape, generator=g)].to(dtype)
+        c["z"] = torch.where(mask, z, junk)
+        o["mask"] = mask
+        m = O.bool_to_bits(mask) if kind == "bits" else mask
+        kw["mask"] = m if T else m[:, 0]
+    c["action"] = torch.randint(0, V, (B, rows), generator=g)
+    if "mask" in o:  # mostly allowed ones
+        pick = torch.where(o["mask"], torch.rand(B, rows, V, generator=g), -1.0).argmax(-1)
+        c["action"] = torch.where(torch.rand(B, rows, generator=g) < 0.8, pick, c["action"])
+    c["g"] = (torch.randn(B, rows, generator=g), torch.randn(B, rows, generator=g) * 0.3)
+    c["g_out"] = torch.randn(B, rows, V, generator=g).to(dtype)
+    return c
+
+
+def gpu(c, x):
+    x = x.cuda()
+    return x if c["T"] else x[:, 0]
+
+
+def kwargs(c):
+    return {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in c["kwargs"].items()}
+
+
+def same(a, b):
+    """The same bits, NaN (of an unknown id) being equal to itself."""
+    return torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(a.nan_to_num(), b.nan_to_num())
+
+
+def check(c):
+    z, kw = gpu(c, c["z"]), kwargs(c)
+    dtype = z.dtype
+    want = O.token_policy(c["z"], action=c["action"], g_lp=c["g"][0], g_H=c["g"][1], g_out=c["g_out"], **c["oracle"])
+    out = process_logits(z, **kw)
+    assert out.dtype == dtype and out.shape == z.shape and F.last_kernel() == "process_logits"
+    O.assert_close(out, want.out, want.out_tol, "process_logits")
+    leaf = z.clone().requires_grad_()
+    (d,) = torch.autograd.grad(process_logits(leaf, **kw), leaf, gpu(c, c["g_out"]))
+    O.assert_close(d, want.d_process, want.d_process_tol, "process_logits gradient")
+    action = gpu(c, c["action"])
+    lp, H = token_log_prob(z, action, entropy=True, **kw)
+    assert lp.dtype == H.dtype == torch.float32 and lp.shape == action.shape
+    O.assert_close(lp, want.log_prob, want.log_prob_tol, "log_prob")
+    O.assert_close(H, want.entropy, want.entropy_tol, "entropy")
+    leaf = z.clone().requires_grad_()
+    both = token_log_prob(leaf, action, entropy=True, **kw)
+    assert same(both[0].detach(), lp) and same(both[1].detach(), H)
+    (d,) = torch.autograd.grad(both, leaf, tuple(gpu(c, g) for g in c["g"]))
+    assert d.dtype == dtype
+    O.assert_close(d, want.d_logits, want.d_logits_tol, "log_prob gradient")
+
+
+@pytest.mark.parametrize("V", [1, 2, 7, 8, 9, 31, 32, 33, 511, 512, 513, 2047, 2048, 2049, 16383, 16385, 40001])
+@pytest.mark.parametrize("kind", KINDS)
+def test_vocabulary_sizes(V, kind):
+    check(make(kind, torch.bfloat16, 2, 3, V, L=9, seed=V))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("B,T,V,L", [(1, 0, 3001, 1), (5, 0, 4096, 300), (3, 4, 2500, 70), (1, 1, 517, 1), (2, 9, 130, 200)])
+def test_types_and_forms(dtype, kind, B, T, V, L):
+    check(make(kind, dtype, B, T, V, L, seed=B * 7 + T))
+
+
+@pytest.mark.parametrize("monotonic", [True, False])
+@pytest.mark.parametrize("kind", ["penalties", "all"])
+def test_runs_of_rows_of_one_block(kind, monotonic):
+    """Many rows of few tokens: a block walks through runs of rows and carries the counts (histories that grow, and any order)."""
+    check(make(kind, torch.float32, 60, 150, 41, L=170, seed=4, monotonic=monotonic))
+
+
+def test_grown_by_one_token_a_row():
+    c = make("all", torch.bfloat16, 40, 200, 50, L=230, seed=9)
+    start = torch.arange(40) % 31
+    c["oracle"]["lengths"] = c["kwargs"]["lengths"] = start[:, None] + torch.arange(200)
+    c["oracle"]["prompt"] = c["kwargs"]["prompt_lengths"] = start
+    check(c)
+
+
+@pytest.mark.parametrize("bias_dtype", DTYPES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_bias_types(dtype, bias_dtype):
+    check(make("all", dtype, 2, 3, 1003, L=20, seed=5, bias_dtype=bias_dtype))
+
+
+def test_int32_inputs_and_parameters_a_sequence():
+    c = make("all", torch.float32, 6, 5, 700, L=50, seed=6)
+    g = torch.Generator().manual_seed(1)
+    par = {k: torch.rand(6, generator=g) + 0.5 for k in ("rep", "pres", "freq", "temp")}
+    c["oracle"].update(par)
+    c["kwargs"].update(repetition_penalty=par["rep"], presence_penalty=par["pres"], frequency_penalty=par["freq"], temperature=par["temp"])
+    for k in ("tokens", "lengths", "prompt_lengths"):
+        c["kwargs"][k] = c["kwargs"][k].to(torch.int32)
+    c["action"] = c["action"].to(torch.int32)
+    want = O.token_policy(c["z"], action=c["action"].long(), **c["oracle"])
+    out = process_logits(gpu(c, c["z"]), **kwargs(c))
+    O.assert_close(out, want.out, want.out_tol, "process_logits")
+    lp = token_log_prob(gpu(c, c["z"]), gpu(c, c["action"]), **kwargs(c))
+    O.assert_close(lp, want.log_prob, want.log_prob_tol, "log_prob")
+
+
+@pytest.mark.parametrize("form", ["padded vocabulary", "time first", "expanded", "offset", "strided vocabulary", "two batch dims"])
+def test_layouts(form):
+    c = make("all", torch.bfloat16, 4, 6, 1037, L=12, seed=8)
+    want = O.token_policy(c["z"], action=c["action"], g_lp=c["g"][0], g_H=c["g"][1], **c["oracle"])
+    z, kw, action, g = c["z"].cuda(), kwargs(c), c["action"].cuda(), tuple(x.cuda() for x in c["g"])
+    if form == "padded vocabulary":
+        wide = torch.full((4, 6, 1040 + 11), math.nan, dtype=z.dtype, device="cuda")
+        wide[..., :1037] = z
+        z = wide[..., :1037]
+    elif form == "time first":
+        z = z.transpose(0, 1).contiguous().transpose(0, 1)
+        kw["mask"] = kw["mask"].transpose(0, 1).contiguous().transpose(0, 1)
+    elif form == "expanded":
+        c["z"] = c["z"][:1].expand(4, 6, 1037).nan_to_num(0.5, 0.5, 0.5)
+        want = O.token_policy(c["z"], action=c["action"], g_lp=c["g"][0], g_H=c["g"][1], **c["oracle"])
+        z = c["z"][:1].cuda().expand(4, 6, 1037)
+    elif form == "offset":
+        z = torch.cat([torch.zeros(3, dtype=z.dtype, device="cuda"), z.flatten()])[3:].view(4, 6, 1037)
+    elif form == "strided vocabulary":
+        z = torch.stack([z, z], -1)[..., 0]
+    else:
+        z, action, g = z.view(2, 2, 6, 1037), action.view(2, 2, 6), tuple(x.view(2, 2, 6) for x in g)
+        kw = {k: v.unflatten(0, (2, 2)) if isinstance(v, torch.Tensor) else v for k, v in kw.items()}
+    out = process_logits(z, **kw)
+    assert out.shape == z.shape
+    O.assert_close(out, want.out, want.out_tol, "process_logits")
+    leaf = z.detach().requires_grad_()
+    lp, H = token_log_prob(leaf, action, entropy=True, **kw)
+    O.assert_close(lp, want.log_prob, want.log_prob_tol, "log_prob")
+    (d,) = torch.autograd.grad((lp, H), leaf, g)
+    O.assert_close(d, want.d_logits, want.d_logits_tol, "gradient")
+
+
+@pytest.mark.parametrize("which", ["log_prob", "entropy"])
+def test_one_of_the_two_gradients(which):
+    c = make("all", torch.float32, 3, 4, 900, L=12, seed=3)
+    leaf = c["z"].cuda().requires_grad_()
+    out = token_log_prob(leaf, c["action"].cuda(), entropy=True, **kwargs(c))
+    i = 0 if which == "log_prob" else 1
+    (d,) = torch.autograd.grad(out[i], leaf, c["g"][i].cuda())
+    want = O.token_policy(c["z"], action=c["action"], **{"g_lp" if i == 0 else "g_H": c["g"][i]}, **c["oracle"])
+    O.assert_close(d, want.d_logits, want.d_logits_tol, "gradient")
+
+
+def test_gradient_against_differences():
+    """<gradient, v> against central differences, in 64 bits, of the oracle's own forward form.  The differences' error: third derivatives of a
+    log-softmax along |v| <= 1 are at most 2, so h^2 / 3 a row and 2^-52 / h of rounding; then the gradient's own bound."""
+    c = make("penalties", torch.float32, 3, 4, 200, L=12, seed=13)
+    leaf = c["z"].cuda().requires_grad_()
+    out = token_log_prob(leaf, c["action"].cuda(), entropy=True, **kwargs(c))
+    (d,) = torch.autograd.grad(out, leaf, tuple(g.cuda() for g in c["g"]))
+    v = torch.rand(c["z"].shape, dtype=torch.float64, generator=torch.Generator().manual_seed(2)) * 2 - 1
+    v = v * (c["z"].abs() > 1e-3)  # the repetition penalty has a kink at 0
+    h = 1e-5
+
+    def loss(z):
+        r = O.token_policy(z, action=c["action"], **c["oracle"])
+        return float((r.log_prob * c["g"][0].double()).sum() + (r.entropy * c["g"][1].double()).sum())
+
+    want = O.token_policy(c["z"], action=c["action"], g_lp=c["g"][0], g_H=c["g"][1], **c["oracle"])
+    diff = (loss(c["z"].double() + h * v) - loss(c["z"].double() - h * v)) / (2 * h)
+    got = float((d.cpu().double() * v).sum())
+    tol = float(want.d_logits_tol.sum() + O.U * want.d_logits.abs().sum()) + 12 * 40 * h * h + 1e-9
+    assert abs(got - diff) <= tol, (got, diff, tol)
+
+
+def test_padding_and_unknown_actions():
+    c = make("bits", torch.bfloat16, 3, 5, 600, seed=14)
+    c["action"][0, 2:] = -1
+    c["action"][1, 1] = -100
+    c["action"][1, 3] = 600
+    c["action"][2, 0] = 2 ** 40
+    c["z"][0, 3] = math.nan  # a padded row is not looked at
+    check(c)
+
+
+def test_extreme_values():
+    """Infinities and lowest values in allowed places."""
+    z = torch.randn(6, 1, 300, generator=torch.Generator().manual_seed(3))
+    low = torch.finfo(torch.float32).min
+    z[0, 0, 5:] = -math.inf
+    z[1, 0] = -math.inf
+    z[2, 0] = low
+    z[3, 0, ::2] = low
+    z[4, 0] *= 1e4
+    z[5, 0, 7] = 1e30
+    action = torch.tensor([[2], [0], [4], [1], [9], [7]])
+    g = (torch.ones(6, 1), torch.full((6, 1), 0.5))
+    want = O.token_policy(z, action=action, g_lp=g[0], g_H=g[1])
+    leaf = z[:, 0].cuda().requires_grad_()
+    lp, H = token_log_prob(leaf, action[:, 0].cuda(), entropy=True)
+    O.assert_close(lp, want.log_prob, want.log_prob_tol, "log_prob")
+    O.assert_close(H, want.entropy, want.entropy_tol, "entropy")
+    (d,) = torch.autograd.grad((lp, H), leaf, tuple(x[:, 0].cuda() for x in g))
+    O.assert_close(d, want.d_logits, want.d_logits_tol, "gradient")
+    # maxima of any size, here and there in the vocabulary: the joined partials lie on both sides of every threshold
+    g = torch.Generator().manual_seed(5)
+    far = torch.randn(64, 1, 9000, generator=g)
+    far += (torch.randn(64, 1, 1, generator=g).sign() * torch.exp2(torch.linspace(0, 126, 64))[:, None, None])
+    far[::2, 0, 3000:] += torch.exp2(torch.linspace(0, 60, 32))[:, None]
+    far[1::4, 0, :5000] = -3e6
+    action = far.argmax(-1)
+    want = O.token_policy(far, action=action)
+    lp, H = token_log_prob(far[:, 0].cuda(), action[:, 0].cuda(), entropy=True)
+    O.assert_close(lp, want.log_prob, 2e-5, "log_prob")  # of the very values: nothing rounds before the differences z - max
+    # the sums' share of the oracle's bound, with ln 9000 + 1 < 11 (the logits' share would be vast, and is none: they are exact)
+    O.assert_close(H, want.entropy, O.U * 160 * (want.entropy + 11) + 2e-5, "entropy")
+    # a bias of the lowest value in place of a mask: no NaN, and the rest as if it were masked
+    bias = torch.zeros(300)
+    bias[10:] = torch.finfo(torch.bfloat16).min
+    lp = token_log_prob(z[4:5, 0].bfloat16().cuda() / 1e4, torch.tensor([3]).cuda(), bias=bias.bfloat16().cuda(), temperature=0.5)
+    want = O.token_policy((z[4:5].bfloat16() / 1e4), action=torch.tensor([[3]]), bias=bias, temp=0.5)
+    O.assert_close(lp, want.log_prob, O.token_policy((z[4:5, :, :10].bfloat16() / 1e4), action=torch.tensor([[3]]), temp=0.5).log_prob_tol, "lowest bias")
+    assert torch.isnan(token_log_prob(torch.tensor([[0.0, math.nan, 1.0]]).cuda(), torch.tensor([0]).cuda())).all()
+    assert torch.isnan(token_log_prob(torch.tensor([[0.0, math.inf, 1.0]]).cuda(), torch.tensor([0]).cuda())).all()
+
+
+def test_out_and_in_place():
+    c = make("all", torch.bfloat16, 5, 0, 1201, L=30, seed=15)
+    kw = kwargs(c)
+    z = gpu(c, c["z"])
+    want = process_logits(z, **kw)
+    wide = torch.full((5, 1300), 7.0, dtype=z.dtype, device="cuda")
+    got = process_logits(z, out=wide[:, :1201], **kw)
+    assert got.data_ptr() == wide.data_ptr() and torch.equal(wide[:, :1201], want) and (wide[:, 1201:] == 7.0).all()  # the rest is left as it was
+    mine = z.clone()
+    assert process_logits(mine, out=mine, **kw) is mine and torch.equal(mine, want)
+
+
+def test_in_place_write_before_backward_is_noticed():
+    c = make("all", torch.float32, 2, 3, 100, L=9, seed=16)
+    leaf, kw = c["z"].cuda().requires_grad_(), kwargs(c)
+    lp = token_log_prob(leaf, c["action"].cuda(), **kw)
+    kw["mask"].fill_(True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        lp.sum().backward()
+
+
+def test_empty_batches():
+    z = torch.zeros(0, 4, 33, device="cuda", requires_grad=True)
+    lp, H = token_log_prob(z, torch.zeros(0, 4, dtype=torch.long, device="cuda"), entropy=True)
+    assert lp.shape == H.shape == (0, 4)
+    (lp.sum() + H.sum()).backward()
+    assert z.grad.shape == z.shape
+    assert process_logits(torch.zeros(3, 0, 5, device="cuda")).shape == (3, 0, 5)
+    tokens = torch.zeros(2, 0, dtype=torch.long, device="cuda")
+    z = torch.randn(2, 5, device="cuda")
+    assert torch.equal(process_logits(z, tokens=tokens, repetition_penalty=2.0), z)
+
+
+def test_results_do_not_depend_on_the_call():
+    """The same bits, twice, and beside a call on another stream."""
+    c = make("all", torch.bfloat16, 6, 20, 5000, L=60, seed=17)
+    kw, z, action = kwargs(c), c["z"].cuda(), c["action"].cuda()
+    first = token_log_prob(z, action, entropy=True, **kw)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = token_log_prob(z, action, entropy=True, **kw)
+    here = token_log_prob(z, action, entropy=True, **kw)
+    torch.cuda.current_stream().wait_stream(side)
+    for x in (there, here):
+        assert same(x[0], first[0]) and same(x[1], first[1])
+
+
+def test_captured_and_replayed():
+    c = make("all", torch.bfloat16, 4, 8, 3000, L=40, seed=18)
+    kw, z, action, g = kwargs(c), c["z"].cuda(), c["action"].cuda(), tuple(x.cuda() for x in c["g"])
+
+    def step(leaf):
+        lp, H = token_log_prob(leaf, action, entropy=True, **kw)
+        out = process_logits(leaf.detach(), **kw)
+        return (lp.detach(), H.detach(), out, torch.autograd.grad((lp, H), leaf, g)[0])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(z.clone().requires_grad_())  # warm-up, on leaves that do not live on
+    torch.cuda.current_stream().wait_stream(side)
+    static = z.clone().requires_grad_()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step(static)
+        graphs.append((graph, outs))
+    for k in range(4):
+        with torch.no_grad():
+            static.copy_(torch.roll(z, k, 0) if k < 3 else z)
+        for graph, outs in graphs:
+            graph.replay()
+        eager = step(static.detach().clone().requires_grad_())
+        torch.cuda.synchronize()
+        for _, outs in graphs:
+            for a, b in zip(outs, eager):
+                assert same(a, b)
+
+
+def test_a_token_policy_through_vtrace():
+    """As they are used: a head that keeps its input in 8 bits, the actor on top, V-trace through the actor, and the policy-gradient step."""
+    torch.manual_seed(0)
+    B, T, D, V, P = 3, 7, 48, 320, 4
+    dev = "cuda"
+    head = CheckpointedLinear(D, V, device=dev, dtype=torch.float32)
+    feats = torch.randn(B, T, D, device=dev)
+    tokens = torch.randint(0, V, (B, P + T), device=dev)
+    lengths = (P + torch.arange(T, device=dev)).expand(B, T).contiguous()
+    mask = torch.rand(B, T, V, device=dev) < 0.7
+    action = tokens[:, P:]
+    mask.scatter_(-1, action.unsqueeze(-1), True)
+    data = RolloutData({"features": feats, "tokens": tokens, "lengths": lengths, "prompt_lengths": torch.full((B,), P, device=dev), "mask": mask,
+                        "action": action, "state_value": torch.randn(B, T, 1, device=dev), "sample_log_prob": torch.randn(B, T, 1, device=dev) - 5,
+                        ("next", "state_value"): torch.randn(B, T, 1, device=dev), ("next", "reward"): torch.randn(B, T, 1, device=dev),
+                        ("next", "done"): torch.zeros(B, T, 1, dtype=torch.bool, device=dev),
+                        ("next", "terminated"): torch.zeros(B, T, 1, dtype=torch.bool, device=dev)}, batch_size=[B, T])
+    actor = TokenActor(lambda d: head(d.get("features")), tokens_key="tokens", lengths_key="lengths", prompt_lengths_key="prompt_lengths",
+                       mask_key="mask", temperature=0.9, repetition_penalty=1.2, presence_penalty=0.1, frequency_penalty=0.05)
+    vtrace = VTrace(gamma=0.99, actor_network=actor, value_network=None)
+    vtrace(data)
+    logits = head(feats).detach()
+    want = O.token_policy(logits.cpu(), tokens=tokens.cpu(), lengths=lengths.cpu(), prompt=torch.full((B,), P), rep=1.2, pres=0.1, freq=0.05,
+                          mask=mask.cpu(), temp=0.9, action=action.cpu())
+    lp = actor(data)
+    O.assert_close(lp, want.log_prob, want.log_prob_tol, "actor")
+    adv, _ = F.vtrace_advantage_estimate(0.99, lp.detach().unsqueeze(-1), data.get("sample_log_prob"), data.get("state_value"),
+                                         data.get(("next", "state_value")), data.get(("next", "reward")), data.get(("next", "done")),
+                                         data.get(("next", "terminated")))
+    assert torch.equal(data.get("advantage"), adv)
+    lp, H = actor.evaluate(data)
+    loss = -(lp * adv.squeeze(-1)).mean() - 0.01 * H.mean()
+    loss.backward()
+    n = B * T
+    back = O.token_policy(logits.cpu(), tokens=tokens.cpu(), lengths=lengths.cpu(), prompt=torch.full((B,), P), rep=1.2, pres=0.1, freq=0.05,
+                          mask=mask.cpu(), temp=0.9, action=action.cpu(), g_lp=-adv.squeeze(-1).cpu() / n, g_H=torch.full((B, T), -0.01 / n))
+    kept = O.kept(feats.reshape(n, D).cpu())[2]
+    dz, dz_tol = back.d_logits.reshape(n, V), back.d_logits_tol.reshape(n, V) + 2 * O.U * back.d_logits.reshape(n, V).abs()
+    # n products in 32 bits: n roundings of sums that stay below the sum of magnitudes, two more for -adv / n
+    O.assert_close(head.weight.grad, dz.T @ kept, dz_tol.T @ kept.abs() + (n + 3) * O.U * (dz.abs().T @ kept.abs()), "weight gradient")
+    O.assert_close(head.bias.grad, dz.sum(0), dz_tol.sum(0) + (n + 3) * O.U * dz.abs().sum(0), "bias gradient")

@@ -19,7 +19,7 @@ import warnings
 _LIB_NAME = "libtrl_value.so"
 # TRL_VALUE_LIB: development switch (kernel variants built beside the product library); unset in normal use
 _LIB_PATH = os.environ.get("TRL_VALUE_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", _LIB_NAME)
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 EXTENSION_WARNING = (
     f"Failed to load the torchrl_amd HIP library ({_LIB_PATH}). The value estimators "
@@ -37,6 +37,22 @@ _lib = None
 _load_error = None
 
 _vp, _i64, _dbl, _int, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_double, ctypes.c_int, ctypes.c_size_t
+
+
+class TokenArgs(ctypes.Structure):
+    """trl_token_args of include/trl_value.h."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "mask_kind", "bias_kind", "tokens_wide", "lengths_wide", "prompt_wide", "action_wide")]
+    _fields_ += [(n, ctypes.c_float) for n in ("rep", "pres", "freq", "temp")]
+    _fields_ += [(n, _i64) for n in ("B", "T", "V", "L")]
+    _fields_ += [("logits", _vp), ("logits_sb", _i64), ("logits_st", _i64), ("tokens", _vp), ("tokens_sb", _i64), ("lengths", _vp),
+                 ("prompt", _vp), ("rep_t", _vp), ("pres_t", _vp), ("freq_t", _vp), ("temp_t", _vp), ("bias", _vp), ("bias_sb", _i64),
+                 ("bias_st", _i64), ("mask", _vp), ("mask_sb", _i64), ("mask_st", _i64), ("out", _vp), ("out_sb", _i64), ("out_st", _i64),
+                 ("grad_out", _vp), ("action", _vp), ("log_prob", _vp), ("entropy", _vp), ("stats", _vp), ("g_log_prob", _vp),
+                 ("g_entropy", _vp)]
+
+
+_tok = ctypes.POINTER(TokenArgs)
 
 # symbol -> (restype, argtypes); must list every entry point of include/trl_value.h
 _PROTOTYPES = {
@@ -86,6 +102,17 @@ _PROTOTYPES = {
     "trl_gae_normalize_xchg_fwd": (_int, [_vp, _int, _int, _vp, _vp, _vp, _vp, _vp, _int, _vp, _vp, _dbl, _dbl, _dbl,
                                           _i64, _i64, _i64, _vp, _vp, _dbl, _vp, _vp, _sz, _vp, _int]),
     "trl_xchg_destroy": (_int, [_vp, _vp]),
+    # policies over tokens
+    "trl_process_logits_fwd": (_int, [_vp, _tok]),
+    "trl_process_logits_bwd": (_int, [_vp, _tok]),
+    "trl_token_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "trl_token_log_prob_fwd": (_int, [_vp, _tok, _vp, _sz]),
+    "trl_token_log_prob_bwd": (_int, [_vp, _tok]),
+    # activations kept in 8 bits
+    "trl_act_quantize": (_int, [_vp, _int, _vp, _i64, _i64, _i64, _vp, _vp]),
+    "trl_act_dequantize": (_int, [_vp, _int, _vp, _vp, _i64, _i64, _vp]),
+    "trl_act_weight_grad_workspace_bytes": (_sz, [_int, _i64, _i64, _i64]),
+    "trl_act_weight_grad": (_int, [_vp, _int, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _sz]),
     # host entry points (tensors in host memory)
     "trl_cpu_threads": (_int, []),
     "trl_set_cpu_threads": (_int, [_int]),

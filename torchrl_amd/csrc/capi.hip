@@ -7,7 +7,9 @@
 
 #include <mutex>
 
+#include "act_common.h"
 #include "common.h"
+#include "token_common.h"
 
 namespace {
 
@@ -796,6 +798,136 @@ int trl_moments(void *stream, int dtype, const void *x, int64_t n, double *stats
     launch_reduce_partials((hipStream_t)stream, partials, np, (double)n, stats);
     if (int rc = check_launch("trl_moments(reduce)")) return rc;
     g_kernel = "moments";
+    return TRL_OK;
+}
+
+// ---- policies over tokens ------------------------------------------------------------------------------------------------
+static bool low_dtype_ok(int d) { return d == TRL_F32 || d == TRL_BF16 || d == TRL_F16; }
+
+// what every token entry point checks; *empty: no rows, nothing to do
+static int check_token_args(const char *fn, const trl_token_args *a, bool *empty) {
+    if (!a) return fail(TRL_ERR_INVALID_ARGUMENT, "%s: null arguments", fn);
+    if (!low_dtype_ok(a->dtype)) return fail(TRL_ERR_INVALID_ARGUMENT, "%s: bad dtype", fn);
+    if (a->B < 0 || a->T < 0 || a->V <= 0 || a->V > 0x7fffffffLL || a->L < 0)
+        return fail(TRL_ERR_INVALID_ARGUMENT, "%s: bad sizes (B %lld, T %lld, V %lld, L %lld)", fn, (long long)a->B, (long long)a->T, (long long)a->V,
+                    (long long)a->L);
+    if ((long double)a->B * (long double)a->T * (long double)a->V > 4.0e18L) return fail(TRL_ERR_INVALID_ARGUMENT, "%s: B*T*V too large", fn);
+    *empty = a->B == 0 || a->T == 0;
+    if (*empty) return TRL_OK;
+    if (a->mask_kind < TRL_MASK_NONE || a->mask_kind > TRL_MASK_BITS || (a->mask_kind != TRL_MASK_NONE && !a->mask))
+        return fail(TRL_ERR_INVALID_ARGUMENT, "%s: bad mask", fn);
+    if (a->bias_kind != 0 && (!low_dtype_ok(a->bias_kind - 1) || !a->bias)) return fail(TRL_ERR_INVALID_ARGUMENT, "%s: bad bias", fn);
+    if (!(a->rep_t || a->rep > 0.0f) || !(a->temp_t || a->temp > 0.0f))
+        return fail(TRL_ERR_INVALID_ARGUMENT, "%s: rep and temp must be positive", fn);
+    return TRL_OK;
+}
+
+int trl_process_logits_fwd(void *stream, const trl_token_args *args) {
+    bool empty = false;
+    if (int rc = check_token_args("trl_process_logits_fwd", args, &empty)) return rc;
+    if (empty) return TRL_OK;
+    if (!args->logits || !args->out) return fail(TRL_ERR_INVALID_ARGUMENT, "trl_process_logits_fwd: null pointer");
+    TokenArgs a{*args, nullptr, nullptr, 0, 0, 0, 0};
+    if (launch_process_logits((hipStream_t)stream, a)) return fail(TRL_ERR_UNSUPPORTED, "trl_process_logits_fwd: too many rows for one launch");
+    if (int rc = check_launch("trl_process_logits_fwd")) return rc;
+    g_kernel = "process_logits";
+    return TRL_OK;
+}
+
+int trl_process_logits_bwd(void *stream, const trl_token_args *args) {
+    bool empty = false;
+    if (int rc = check_token_args("trl_process_logits_bwd", args, &empty)) return rc;
+    if (empty) return TRL_OK;
+    const bool needs_z = args->tokens && (args->rep_t || args->rep != 1.0f);
+    if (!args->grad_out || !args->out || (needs_z && !args->logits)) return fail(TRL_ERR_INVALID_ARGUMENT, "trl_process_logits_bwd: null pointer");
+    TokenArgs a{*args, nullptr, nullptr, 0, 0, 0, 0};
+    if (launch_process_logits_bwd((hipStream_t)stream, a)) return fail(TRL_ERR_UNSUPPORTED, "trl_process_logits_bwd: too many rows for one launch");
+    if (int rc = check_launch("trl_process_logits_bwd")) return rc;
+    g_kernel = "process_logits_bwd";
+    return TRL_OK;
+}
+
+size_t trl_token_workspace_bytes(int64_t B, int64_t T, int64_t V) {
+    if (B <= 0 || T <= 0 || V <= 0) return 0;
+    return (size_t)B * (size_t)T * ((size_t)token_subs(V) * 16 + 4);
+}
+
+int trl_token_log_prob_fwd(void *stream, const trl_token_args *args, void *workspace, size_t workspace_bytes) {
+    bool empty = false;
+    if (int rc = check_token_args("trl_token_log_prob_fwd", args, &empty)) return rc;
+    if (empty) return TRL_OK;
+    if (!args->logits || !args->action || !args->log_prob) return fail(TRL_ERR_INVALID_ARGUMENT, "trl_token_log_prob_fwd: null pointer");
+    const size_t need = trl_token_workspace_bytes(args->B, args->T, args->V);
+    if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))
+        return fail(TRL_ERR_WORKSPACE, "trl_token_log_prob_fwd: workspace is %zu bytes, need %zu (16-byte aligned)", workspace_bytes, need);
+    float *partials = (float *)workspace;
+    TokenArgs a{*args, partials, partials + (size_t)args->B * (size_t)args->T * (size_t)token_subs(args->V) * 4, 0, 0, 0, 0};
+    if (launch_token_log_prob((hipStream_t)stream, a)) return fail(TRL_ERR_UNSUPPORTED, "trl_token_log_prob_fwd: too many rows for one launch");
+    if (int rc = check_launch("trl_token_log_prob_fwd")) return rc;
+    g_kernel = "token_log_prob";
+    return TRL_OK;
+}
+
+int trl_token_log_prob_bwd(void *stream, const trl_token_args *args) {
+    bool empty = false;
+    if (int rc = check_token_args("trl_token_log_prob_bwd", args, &empty)) return rc;
+    if (empty) return TRL_OK;
+    if (!args->logits || !args->action || !args->stats || !args->out || (args->g_entropy && !args->entropy) ||
+        (!args->g_entropy && !args->g_log_prob))
+        return fail(TRL_ERR_INVALID_ARGUMENT, "trl_token_log_prob_bwd: null pointer");
+    TokenArgs a{*args, nullptr, nullptr, 0, 0, 0, 0};
+    if (launch_token_log_prob_bwd((hipStream_t)stream, a)) return fail(TRL_ERR_UNSUPPORTED, "trl_token_log_prob_bwd: too many rows for one launch");
+    if (int rc = check_launch("trl_token_log_prob_bwd")) return rc;
+    g_kernel = "token_log_prob_bwd";
+    return TRL_OK;
+}
+
+// ---- activations kept in 8 bits ------------------------------------------------------------------------------------------
+static int check_act_dims(const char *fn, int dtype, int64_t N, int64_t D) {
+    if (!low_dtype_ok(dtype)) return fail(TRL_ERR_INVALID_ARGUMENT, "%s: bad dtype", fn);
+    if (N < 0 || D <= 0 || N > 0x7fffffffLL || D > 0x7fffffe0LL) return fail(TRL_ERR_INVALID_ARGUMENT, "%s: bad sizes (N %lld, D %lld)", fn, (long long)N, (long long)D);
+    if ((D + kActBlock - 1) / kActBlock * N > 0x7fffffffLL * 64) return fail(TRL_ERR_UNSUPPORTED, "%s: too large for one launch", fn);
+    return TRL_OK;
+}
+
+int trl_act_quantize(void *stream, int dtype, const void *x, int64_t x_stride, int64_t N, int64_t D, int8_t *codes, uint8_t *exponents) {
+    if (int rc = check_act_dims("trl_act_quantize", dtype, N, D)) return rc;
+    if (N == 0) return TRL_OK;
+    if (!x || !codes || !exponents || ((uintptr_t)codes & 15)) return fail(TRL_ERR_INVALID_ARGUMENT, "trl_act_quantize: null pointer, or codes not 16-byte aligned");
+    launch_act_quantize((hipStream_t)stream, dtype, x, x_stride, N, D, codes, exponents);
+    if (int rc = check_launch("trl_act_quantize")) return rc;
+    g_kernel = "act_quantize";
+    return TRL_OK;
+}
+
+int trl_act_dequantize(void *stream, int dtype, const int8_t *codes, const uint8_t *exponents, int64_t N, int64_t D, void *out) {
+    if (int rc = check_act_dims("trl_act_dequantize", dtype, N, D)) return rc;
+    if (N == 0) return TRL_OK;
+    if (!out || !codes || !exponents || ((uintptr_t)codes & 15)) return fail(TRL_ERR_INVALID_ARGUMENT, "trl_act_dequantize: null pointer, or codes not 16-byte aligned");
+    launch_act_dequantize((hipStream_t)stream, dtype, codes, exponents, N, D, out);
+    if (int rc = check_launch("trl_act_dequantize")) return rc;
+    g_kernel = "act_dequantize";
+    return TRL_OK;
+}
+
+size_t trl_act_weight_grad_workspace_bytes(int dtype, int64_t N, int64_t O, int64_t D) {
+    if (!low_dtype_ok(dtype) || N <= 0 || O <= 0 || D <= 0) return 0;
+    return act_weight_grad_workspace(dtype, N, O, D);
+}
+
+int trl_act_weight_grad(void *stream, int dtype, const void *dy, int64_t dy_stride, const int8_t *codes, const uint8_t *exponents,
+                        int64_t N, int64_t O, int64_t D, void *dw, void *db, void *workspace, size_t workspace_bytes) {
+    if (int rc = check_act_dims("trl_act_weight_grad", dtype, N, D)) return rc;
+    if (O <= 0 || O > 0x7fffffffLL || !dw) return fail(TRL_ERR_INVALID_ARGUMENT, "trl_act_weight_grad: O <= 0 or null pointer");
+    if (N > 0 && (!dy || !codes || !exponents || ((uintptr_t)codes & 15)))
+        return fail(TRL_ERR_INVALID_ARGUMENT, "trl_act_weight_grad: null pointer, or codes not 16-byte aligned");
+    const size_t need = trl_act_weight_grad_workspace_bytes(dtype, N, O, D);
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
+        return fail(TRL_ERR_WORKSPACE, "trl_act_weight_grad: workspace is %zu bytes, need %zu (16-byte aligned)", workspace_bytes, need);
+    if (launch_act_weight_grad((hipStream_t)stream, dtype, dy, dy_stride, codes, exponents, N, O, D, dw, db, workspace))
+        return fail(TRL_ERR_UNSUPPORTED, "trl_act_weight_grad: too large for one launch");
+    if (int rc = check_launch("trl_act_weight_grad")) return rc;
+    g_kernel = "act_weight_grad";
     return TRL_OK;
 }
 

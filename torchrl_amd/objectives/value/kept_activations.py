@@ -1,0 +1,161 @@
+"""Activations kept for the backward pass in 8 bits.
+
+A critic's or actor's linear layers keep their inputs until the backward pass; over a rollout of many steps those activations, not the
+weights, fill the memory.  :func:`quantize_activation` keeps them at one byte an element and one more every 32 (half of bfloat16's, a
+quarter of float32's); :func:`checkpointed_linear` / :class:`CheckpointedLinear` is the layer whose weight gradient is computed from them
+directly, in matrix instructions that read the bytes: the wide activations never come back to memory.  The output and the gradient of the input
+are those of an ordinary linear layer; only the weight gradient sees the rounding (half a step of 2^-6 of the block's largest
+magnitude, less than one at the very top).  The format and the kernels are behind ``trl_act_*`` of include/trl_value.h.
+
+The reference has no counterpart.
+"""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+from torch import nn, Tensor
+from torch.autograd.function import once_differentiable
+
+from torchrl_amd import _extension
+from torchrl_amd.objectives.value import functional as F
+
+__all__ = ["QuantizedActivation", "quantize_activation", "checkpointed_linear", "CheckpointedLinear"]
+
+BLOCK = 32  # features that share a step
+_DT = {torch.float32: 0, torch.bfloat16: 2, torch.float16: 3}
+
+
+def _check(x: Tensor, name: str):
+    if not isinstance(x, Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if x.dtype not in _DT:
+        raise NotImplementedError(f"torchrl_amd 8-bit activations support float32, bfloat16 and float16, got {x.dtype}")
+
+
+def _check_device(x: Tensor):
+    if x.device.type != "cuda":
+        raise RuntimeError(f"torchrl_amd 8-bit activations run on MI355X (HIP, device type 'cuda') tensors only; got a tensor on {x.device}.")
+
+
+def _rows(x: Tensor) -> Tensor:
+    """``x`` as (N, D) with last stride 1."""
+    x = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+
+
+def _call(name, device, *args):
+    lib = _extension.get_lib()
+    with F._on(device):
+        rc = getattr(lib, name)(F._stream(device), *args)
+    if rc:
+        _extension.check(rc, lib)
+
+
+@dataclass
+class QuantizedActivation:
+    """``codes`` (int8, last dim filled up to whole blocks) and ``exponents`` (uint8, one a block: a step is ``2 ** (exponent - 127)``) of a
+    tensor of ``shape`` and ``dtype``."""
+
+    codes: Tensor
+    exponents: Tensor
+    shape: torch.Size
+    dtype: torch.dtype
+
+    def dequantize(self, dtype: Optional[torch.dtype] = None) -> Tensor:
+        """The values that the bytes stand for (exact in the tensor's own dtype and in bfloat16)."""
+        dtype = self.dtype if dtype is None else dtype
+        if dtype not in _DT:
+            raise NotImplementedError(f"torchrl_amd 8-bit activations support float32, bfloat16 and float16, got {dtype}")
+        out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
+        if out.numel():
+            D = self.shape[-1]
+            _call("trl_act_dequantize", out.device, _DT[dtype], self.codes.data_ptr(), self.exponents.data_ptr(), out.numel() // D, D, out.data_ptr())
+        return out
+
+
+def quantize_activation(x: Tensor) -> QuantizedActivation:
+    """Keeps ``x`` ``[*B, D]`` (float32, bfloat16 or float16) in 8 bits: blocks of 32 features share a power of two, 2^-6 of the one at or below
+    the block's largest magnitude; codes are rounded to nearest even and held to 127.  Blocks with a NaN or an infinity stand for NaN."""
+    _check(x, "x")
+    if x.ndim < 1 or x.shape[-1] == 0:
+        raise RuntimeError(f"quantize_activation needs a feature dim, got shape {tuple(x.shape)}")
+    _check_device(x)
+    lead, D = x.shape[:-1], x.shape[-1]
+    blocks = (D + BLOCK - 1) // BLOCK
+    codes = torch.empty(*lead, blocks * BLOCK, dtype=torch.int8, device=x.device)
+    exponents = torch.empty(*lead, blocks, dtype=torch.uint8, device=x.device)
+    if x.numel():
+        rows = _rows(x.detach())
+        _call("trl_act_quantize", x.device, _DT[x.dtype], rows.data_ptr(), rows.stride(0), rows.shape[0], D, codes.data_ptr(), exponents.data_ptr())
+    return QuantizedActivation(codes, exponents, x.shape, x.dtype)
+
+
+def _weight_grad(dy: Tensor, codes: Tensor, exponents: Tensor, D: int, want_db: bool):
+    """(dy^T x^, column sums of dy or None) of (N, O) gradients and a kept (N, D) activation."""
+    dy = dy if dy.stride(1) == 1 or dy.shape[1] == 1 else dy.contiguous()
+    N, O = dy.shape
+    dt = _DT[dy.dtype]
+    dw = torch.empty(O, D, dtype=dy.dtype, device=dy.device)
+    db = torch.empty(O, dtype=dy.dtype, device=dy.device) if want_db else None
+    need = _extension.get_lib().trl_act_weight_grad_workspace_bytes(dt, N, O, D)
+    ws = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
+    _call("trl_act_weight_grad", dy.device, dt, dy.data_ptr(), dy.stride(0), codes.data_ptr(), exponents.data_ptr(), N, O, D, dw.data_ptr(),
+          None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), need)
+    return dw, db
+
+
+class _CheckpointedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        kept = quantize_activation(x) if ctx.needs_input_grad[1] else None
+        ctx.save_for_backward(None if kept is None else kept.codes, None if kept is None else kept.exponents,
+                              weight if ctx.needs_input_grad[0] else None)
+        ctx.features = x.shape[-1]
+        return torch.nn.functional.linear(x, weight, bias)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        codes, exponents, weight = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad
+        dx = dw = db = None
+        dy = grad.reshape(math.prod(grad.shape[:-1]), grad.shape[-1])
+        if need_x:
+            dx = (dy @ weight).view(*grad.shape[:-1], ctx.features)
+        if need_w:
+            dw, db = _weight_grad(dy, codes, exponents, ctx.features, need_b)
+        elif need_b:
+            db = dy.sum(0)
+        return dx, dw, db
+
+
+def checkpointed_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None) -> Tensor:
+    """``torch.nn.functional.linear(x, weight, bias)`` that keeps ``x`` in 8 bits for the weight gradient (see the module's docstring).
+
+    ``x`` ``[*B, D]``, ``weight`` ``[O, D]`` and ``bias`` ``[O]`` share one dtype (float32, bfloat16 or float16) and device; under autocast they
+    are cast to its dtype.  Without a gradient to ``weight`` nothing is kept."""
+    for t, name in ((x, "x"), (weight, "weight"), (bias, "bias")):
+        if t is not None or name != "bias":
+            _check(t, name)
+    if torch.is_autocast_enabled("cuda"):
+        dt = torch.get_autocast_dtype("cuda")
+        x, weight, bias = x.to(dt), weight.to(dt), None if bias is None else bias.to(dt)
+    if weight.ndim != 2 or x.ndim < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise RuntimeError(f"checkpointed_linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise RuntimeError(f"checkpointed_linear: bias must have shape {(weight.shape[0],)}, got {tuple(bias.shape)}")
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+            raise RuntimeError(f"checkpointed_linear: {name} is {t.dtype} on {t.device}, x is {x.dtype} on {x.device}")
+    _check_device(x)
+    return _CheckpointedLinear.apply(x, weight, bias)
+
+
+class CheckpointedLinear(nn.Linear):
+    """``torch.nn.Linear`` on :func:`checkpointed_linear`: value and policy heads, and the hidden layers of actors and critics."""
+
+    def forward(self, x: Tensor) -> Tensor:
+        return checkpointed_linear(x, self.weight, self.bias)
