@@ -67,43 +67,256 @@ __global__ __launch_bounds__(256) void act_dequantize_kernel(const int8_t *codes
     store8(out + row * D + col, left >= kVec ? kVec : (int)left, v);
 }
 
-// dw = dy^T x^, one 64 x 64 tile a block, 4 x 4 values a thread.
-template <typename T>
-__global__ __launch_bounds__(256) void act_weight_grad_kernel(const T *dy, i64 dy_stride, const int8_t *codes, const u8 *exponents, i64 N, i64 O,
-                                                              i64 D, i64 Dp, i64 tiles_d, T *dw, T *db) {
-    constexpr int BM = 64, BN = 64, BK = 16;
-    __shared__ float sa[BK][BM], sb[BK][BN];
-    const i64 o0 = (blockIdx.x / tiles_d) * BM, d0 = (blockIdx.x % tiles_d) * BN;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    float acc[4][4] = {}, bias[4] = {};
-    for (i64 n0 = 0; n0 < N; n0 += BK) {
-        for (int i = threadIdx.x; i < BK * BM; i += 256) {
-            const i64 n = n0 + i / BM, o = o0 + i % BM;
-            sa[i / BM][i % BM] = n < N && o < O ? (float)dy[n * dy_stride + o] : 0.0f;
+// ---- dw = dy^T x^ ------------------------------------------------------------------------------------------------------------------
+// A (N, O) and a (N, D) matrix, both with the summed dimension outermost, on 32 x 32 x 16 bf16 matrix instructions.
+//   exact   A code times its step has 7 bits, so x^ is exact in bf16.  dy is split into bf16 terms that add up to it exactly: one for
+//           bf16, two for fp16 (8 + 3 bits), three for fp32 (8 + 8 + 8).  Every product is then exact in the 32-bit accumulators, and
+//           the result is off by the sum's own roundings and one to the output type.
+//   tiles   The codes go from registers through the conversion into LDS, rows of tokens as in memory; ds_read_tr16 turns 4 x 16 pieces so
+//           that a lane gets four consecutive tokens of its own column.  Rows are filled up by 16 elements, so that the four rows of a
+//           piece lie in different banks.  Two LDS buffers; the next tile's loads are in flight while one is multiplied.
+//   splits  Few output tiles (value heads) split the tokens; the parts are 32 bits and are added in order by a second launch.
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+
+template <typename T> constexpr int kTerms = sizeof(T) == 4 ? 3 : 1;
+template <> constexpr int kTerms<_Float16> = 2;
+
+__device__ __forceinline__ u32 high_halves(u32 lo, u32 hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
+
+// the bf16 terms of 8 values: term j of element i in w[j]
+template <int NT>
+__device__ __forceinline__ void split8(const float *v, u32x4 *w) {
+    float r[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) r[i] = v[i];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        u32 top[kVec];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+            u32 bits = __builtin_bit_cast(u32, r[i]);
+            if (j == 0 && (bits & 0x7fffffffu) > 0x7f800000u) bits |= 0x00400000u;  // a NaN keeps being one without its low half
+            top[i] = bits & 0xffff0000u;
+            // what is left, exactly; nothing of an infinity or a NaN
+            r[i] = (bits & 0x7f800000u) == 0x7f800000u ? 0.0f : r[i] - __builtin_bit_cast(float, top[i]);
         }
-        for (int i = threadIdx.x; i < BK * BN; i += 256) {
-            const i64 n = n0 + i / BN, d = d0 + i % BN;
-            sb[i / BN][i % BN] = n < N && d < Dp ? (float)codes[n * Dp + d] * step_of(exponents[(n * Dp + d) / kActBlock]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[j][i] = high_halves(top[2 * i], top[2 * i + 1]);
+    }
+}
+
+struct WeightGradArgs {
+    const void *dy;
+    i64 dy_stride;
+    const int8_t *codes;
+    const u8 *exponents;
+    i64 N, O, D, Dp;
+    int tiles_d, tiles;  // output tiles
+    i64 part;            // tokens of a split, a multiple of the tile's
+    void *dw, *db;       // one split: the outputs
+    float *parts;        // more: (splits, O, D) and, behind them, (splits, O)
+    int splits;
+};
+
+template <typename T, int BM, int BN, int BK, int WM, int WN>
+__global__ __launch_bounds__(WM *WN *kWave) void act_weight_grad_kernel(WeightGradArgs a) {
+    constexpr int NT = kTerms<T>, NTHR = WM * WN * kWave;
+    constexpr int SA = BM + 16, SB = BN + 16;              // LDS row strides
+    constexpr int MI = BM / WM / 32, NI = BN / WN / 32;    // a wave's 32 x 32 pieces
+    constexpr int VA = BK * BM / kVec / NTHR, VB = BK * BN / 16 / NTHR;
+    static_assert(VA * kVec * NTHR == BK * BM && VB * 16 * NTHR == BK * BN && NTHR % (BM / kVec) == 0 && NTHR % (BN / 16) == 0, "whole vectors");
+    constexpr int kBuf = BK * (NT * SA + SB);              // elements of a buffer
+    extern __shared__ __align__(16) short lds[];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), wm = wave / WN, wn = wave % WN;
+
+    // consecutive blocks go to the 8 XCDs in turn: give each a run of neighbouring tiles, which share their panels in its L2
+    int tile = blockIdx.x % a.tiles;
+    const int split = blockIdx.x / a.tiles;
+    if (a.tiles % 8 == 0) tile = (tile % 8) * (a.tiles / 8) + tile / 8;
+    const i64 o0 = (i64)(tile / a.tiles_d) * BM, d0 = (i64)(tile % a.tiles_d) * BN;
+    const i64 n0 = split * a.part, n1 = n0 + a.part < a.N ? n0 + a.part : a.N;
+    const bool want_db = a.db && d0 == 0;
+
+    const int a_col = tid % (BM / kVec) * kVec, a_row = tid / (BM / kVec), b_col = tid % (BN / 16) * 16, b_row = tid / (BN / 16);
+    const i64 a_left = a.O - (o0 + a_col);
+    const int a_n = a_left >= kVec ? kVec : a_left < 0 ? 0 : (int)a_left;
+    const bool b_in = d0 + b_col < a.Dp;
+    Raw8<T> ra[VA];
+    u32x4 rb[VB];
+    int re[VB];
+    auto load = [&](i64 n) {
+#pragma unroll
+        for (int q = 0; q < VA; ++q) {
+            const i64 row = n + a_row + q * (NTHR / (BM / kVec));
+            ra[q] = Raw8<T>{};
+            if (row < n1 && a_n > 0) load8((const T *)a.dy + row * a.dy_stride + o0 + a_col, a_n, ra[q]);
         }
-        __syncthreads();
 #pragma unroll
-        for (int k = 0; k < BK; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                bias[i] += sa[k][ty * 4 + i];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][ty * 4 + i], sb[k][tx * 4 + j], acc[i][j]);
+        for (int q = 0; q < VB; ++q) {
+            const i64 row = n + b_row + q * (NTHR / (BN / 16));
+            rb[q] = u32x4{0, 0, 0, 0};
+            re[q] = 127;
+            if (row < n1 && b_in) {
+                rb[q] = *(const u32x4 *)(a.codes + row * a.Dp + d0 + b_col);
+                re[q] = a.exponents[(row * a.Dp + d0 + b_col) / kActBlock];
             }
+        }
+    };
+    float col_sum[kVec] = {};
+    auto store = [&](short *buf) {
+#pragma unroll
+        for (int q = 0; q < VA; ++q) {
+            u32x4 w[NT];
+            float v[kVec];
+            if (NT > 1 || want_db) unpack8(ra[q], v);
+            if (want_db) {
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) col_sum[i] += v[i];
+            }
+            if constexpr (NT > 1) split8<NT>(v, w);
+            else w[0] = ra[q].a;
+            short *to = buf + (a_row + q * (NTHR / (BM / kVec))) * (NT * SA) + a_col;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) *(u32x4 *)(to + j * SA) = w[j];
+        }
+#pragma unroll
+        for (int q = 0; q < VB; ++q) {
+            const float step = step_of(re[q]);
+            u32x4 w[2];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const u32 c = rb[q][i / 2];
+                const float lo = (float)(int8_t)(c >> (16 * (i & 1))) * step, hi = (float)(int8_t)(c >> (16 * (i & 1) + 8)) * step;
+                w[i / 4][i % 4] = high_halves(__builtin_bit_cast(u32, lo), __builtin_bit_cast(u32, hi));
+            }
+            short *to = buf + BK * NT * SA + (b_row + q * (NTHR / (BN / 16))) * SB + b_col;
+            *(u32x4 *)to = w[0];
+            *(u32x4 *)(to + 8) = w[1];
+        }
+    };
+
+    v16f acc[MI][NI] = {};
+    // a lane's place in a 16 (tokens) x 32 (columns) piece: see ds_read_tr16 above
+    const int fk = (lane / 32) * 8 + (lane % 16) / 4, fc = ((lane / 16) % 2) * 16 + (lane % 4) * 4;
+    auto fragment = [&](const short *row0, int stride) {
+        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(row0 + fk * stride + fc));
+        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(row0 + (fk + 4) * stride + fc));
+        return __builtin_bit_cast(v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    if (n0 < n1) {
+        load(n0);
+        store(lds);
+    }
+    __syncthreads();
+    int cur = 0;
+    for (i64 n = n0; n < n1; n += BK, cur ^= 1) {
+        const bool more = n + BK < n1;
+        if (more) load(n + BK);
+        const short *la = lds + cur * kBuf, *lb = la + BK * NT * SA;
+#pragma unroll
+        for (int k = 0; k < BK; k += 16) {
+            v8bf fb[NI];
+#pragma unroll
+            for (int j = 0; j < NI; ++j) fb[j] = fragment(lb + k * SB + (wn * NI + j) * 32, SB);
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const v8bf fa = fragment(la + k * (NT * SA) + t * SA + (wm * MI + i) * 32, NT * SA);
+#pragma unroll
+                    for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa, fb[j], acc[i][j], 0, 0, 0);
+                }
+        }
+        if (more) store(lds + (cur ^ 1) * kBuf);
         __syncthreads();
     }
+
+    // element (row, column) of a piece: row 8 (r / 4) + 4 (lane / 32) + r % 4, column lane % 32
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const i64 o = o0 + ty * 4 + i;
-        if (o >= O) continue;
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (d0 + tx * 4 + j < D) dw[o * D + d0 + tx * 4 + j] = (T)acc[i][j];
-        if (db && d0 == 0 && tx == 0) db[o] = (T)bias[i];
+        for (int j = 0; j < NI; ++j) {
+            const i64 d = d0 + (wn * NI + j) * 32 + lane % 32;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const i64 o = o0 + (wm * MI + i) * 32 + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
+                if (o < a.O && d < a.D) {
+                    if (a.splits == 1) ((T *)a.dw)[o * a.D + d] = (T)acc[i][j][r];
+                    else a.parts[((i64)split * a.O + o) * a.D + d] = acc[i][j][r];
+                }
+            }
+        }
+    if (want_db) {  // the block's threads of a column group, added in order (the loop's last barrier has freed the buffers)
+        float *sums = (float *)lds;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) sums[a_row * BM + a_col + i] = col_sum[i];
+        __syncthreads();
+        for (int c = tid; c < BM; c += NTHR) {
+            float s = 0.0f;
+            for (int r = 0; r < NTHR / (BM / kVec); ++r) s += sums[r * BM + c];
+            if (o0 + c < a.O) {
+                if (a.splits == 1) ((T *)a.db)[o0 + c] = (T)s;
+                else a.parts[(i64)a.splits * a.O * a.D + (i64)split * a.O + o0 + c] = s;
+            }
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void act_join_kernel(const float *parts, int splits, i64 n_w, i64 n_b, T *dw, T *db) {
+    const i64 i = (i64)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n_w + n_b) return;
+    const bool w = i < n_w;
+    const i64 n = w ? n_w : n_b, at = w ? i : i - n_w;
+    const float *p = parts + (w ? 0 : splits * n_w) + at;
+    float s = 0.0f;
+    for (int k = 0; k < splits; ++k) s += p[k * n];
+    (w ? dw : db)[at] = (T)s;
+}
+
+// Tile and splits by the sizes: 32 rows for layers with few outputs, whose codes are all the traffic; 256 x 256 where that fills the
+// chip; else 128 x 128.  Tokens are split until there are about two blocks a compute unit, in parts of at least 256 tokens.
+struct WeightGradPlan { int bm, bn, bk; i64 tiles_d, tiles, part; int splits; };
+WeightGradPlan weight_grad_plan(int dtype, i64 N, i64 O, i64 D) {
+    WeightGradPlan p{};
+    auto tiles = [&](int bm, int bn) { return ((O + bm - 1) / bm) * ((D + bn - 1) / bn); };
+    p.bk = dtype == TRL_BF16 ? 64 : 32;
+    if (O <= 32) { p.bm = 32; p.bn = 128; p.bk = 64; }
+    else if (dtype != TRL_F32 && tiles(256, 256) >= 192) { p.bm = 256; p.bn = 256; }
+    else { p.bm = 128; p.bn = 128; }
+    p.tiles_d = (D + p.bn - 1) / p.bn;
+    p.tiles = tiles(p.bm, p.bn);
+    const i64 want = p.bm == 256 ? 1 : (512 + p.tiles - 1) / p.tiles, most = N / 256 > 0 ? N / 256 : 1;
+    i64 splits = want < most ? want : most;
+    p.part = ((N + splits - 1) / splits + p.bk - 1) / p.bk * p.bk;
+    if (p.part == 0) p.part = p.bk;
+    p.splits = (int)(N ? (N + p.part - 1) / p.part : 1);
+    return p;
+}
+
+template <typename T, int BM, int BN, int BK, int WM, int WN>
+void launch_weight_grad(hipStream_t s, const WeightGradArgs &a) {
+    constexpr size_t bytes = 2 * sizeof(short) * BK * (kTerms<T> * (BM + 16) + BN + 16);
+    static_assert(bytes <= 160 * 1024 && bytes >= sizeof(float) * kVec * WM * WN * kWave, "LDS: two buffers, and the column sums after them");
+    static const hipError_t raised = hipFuncSetAttribute((const void *)act_weight_grad_kernel<T, BM, BN, BK, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    (void)raised;
+    hipLaunchKernelGGL((act_weight_grad_kernel<T, BM, BN, BK, WM, WN>), dim3((unsigned)(a.tiles * a.splits)), dim3(WM * WN * kWave), bytes, s, a);
+}
+template <typename T>
+void launch_weight_grad_t(hipStream_t s, const WeightGradArgs &a, const WeightGradPlan &p) {
+    if (p.bm == 32) launch_weight_grad<T, 32, 128, 64, 1, 4>(s, a);
+    else if constexpr (sizeof(T) == 4) launch_weight_grad<T, 128, 128, 32, 2, 2>(s, a);
+    else {
+        constexpr int BK = kTerms<T> == 1 ? 64 : 32;
+        if (p.bm == 256) launch_weight_grad<T, 256, 256, BK, 2, 4>(s, a);
+        else launch_weight_grad<T, 128, 128, BK, 2, 2>(s, a);
+    }
+    if (a.splits > 1) {
+        const i64 n_w = a.O * a.D, n_b = a.db ? a.O : 0;
+        hipLaunchKernelGGL(act_join_kernel<T>, dim3((unsigned)((n_w + n_b + 255) / 256)), dim3(256), 0, s, a.parts, a.splits, n_w, n_b, (T *)a.dw, (T *)a.db);
     }
 }
 
@@ -125,18 +338,19 @@ void launch_act_dequantize(hipStream_t s, int dtype, const int8_t *codes, const 
     else hipLaunchKernelGGL(act_dequantize_kernel<_Float16>, grid, dim3(256), 0, s, codes, exponents, N, D, G, (_Float16 *)out);
 }
 
-size_t act_weight_grad_workspace(int dtype, i64 N, i64 O, i64 D) { return 0; }
+size_t act_weight_grad_workspace(int dtype, i64 N, i64 O, i64 D) {
+    const WeightGradPlan p = weight_grad_plan(dtype, N, O, D);
+    return p.splits > 1 ? (size_t)p.splits * (size_t)O * (size_t)(D + 1) * sizeof(float) : 0;
+}
 
 int launch_act_weight_grad(hipStream_t s, int dtype, const void *dy, i64 dy_stride, const int8_t *codes, const u8 *exponents, i64 N, i64 O,
                            i64 D, void *dw, void *db, void *workspace) {
-    const i64 Dp = (D + kActBlock - 1) / kActBlock * kActBlock, tiles_d = (D + 63) / 64, tiles = tiles_d * ((O + 63) / 64);
-    if (tiles > 0x7fffffffLL) return 2;
-    const dim3 grid((unsigned)tiles);
-    if (dtype == TRL_F32)
-        hipLaunchKernelGGL(act_weight_grad_kernel<float>, grid, dim3(256), 0, s, (const float *)dy, dy_stride, codes, exponents, N, O, D, Dp, tiles_d, (float *)dw, (float *)db);
-    else if (dtype == TRL_BF16)
-        hipLaunchKernelGGL(act_weight_grad_kernel<__bf16>, grid, dim3(256), 0, s, (const __bf16 *)dy, dy_stride, codes, exponents, N, O, D, Dp, tiles_d, (__bf16 *)dw, (__bf16 *)db);
-    else
-        hipLaunchKernelGGL(act_weight_grad_kernel<_Float16>, grid, dim3(256), 0, s, (const _Float16 *)dy, dy_stride, codes, exponents, N, O, D, Dp, tiles_d, (_Float16 *)dw, (_Float16 *)db);
+    const WeightGradPlan p = weight_grad_plan(dtype, N, O, D);
+    if (p.tiles * p.splits > 0x7fffffffLL || (O * (D + 1) + 255) / 256 > 0x7fffffffLL) return 2;
+    const WeightGradArgs a{dy, dy_stride, codes, exponents, N, O, D, (D + kActBlock - 1) / kActBlock * kActBlock, (int)p.tiles_d, (int)p.tiles, p.part, dw, db,
+                           (float *)workspace, p.splits};
+    if (dtype == TRL_F32) launch_weight_grad_t<float>(s, a, p);
+    else if (dtype == TRL_BF16) launch_weight_grad_t<__bf16>(s, a, p);
+    else launch_weight_grad_t<_Float16>(s, a, p);
     return 0;
 }
