@@ -27,6 +27,8 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f
 constexpr float kFloor = -1.0e4f;            // 2^kFloor is 0: keeps 0 * (-inf) out of the entropy
 constexpr u32 kSeenInPrompt = 0x80000000u;
 
+template <bool B>
+struct Bool { static constexpr bool value = B; };
 enum Mode { kProcess, kProcessBwd, kLogProb, kLogProbBwd };
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
@@ -45,84 +47,90 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-__device__ __forceinline__ void count_token(u32 *counts, i64 tok, i64 lo, i64 n, bool prompt) {
+__device__ __forceinline__ void count_token(u32 *counts, i64 tok, i64 lo, int n, bool prompt) {
     const i64 off = tok - lo;
     if (off < 0 || off >= n) return;  // another slice's token, or no token at all (padding)
-    u32 *c = counts + (off & ~(i64)(kSub - 1)) + count_word((int)(off & (kSub - 1)));
+    u32 *c = counts + ((int)off & ~(kSub - 1)) + count_word((int)off & (kSub - 1));
     if (prompt) atomicOr(c, kSeenInPrompt);
     else atomicAdd(c, 1u);
 }
 
-// ---- one row's share of a lane -------------------------------------------------------------------------------------------------
-__device__ __forceinline__ u32 mask_bits(const TokenArgs &a, const u8 *mask_row, i64 tok, int n) {
+// ---- a lane's share of a row: 8 tokens at `off` of the wave's sub-slice, of which the first n exist (n >= 8: all) -----------------------
+__device__ __forceinline__ u32 mask_bits(int kind, const u8 *mask_lo, int off, int n) {
     if (n <= 0) return 0u;
     const u32 in = n >= kVec ? 0xffu : (1u << n) - 1u;
-    if (a.mask_kind == TRL_MASK_NONE) return in;
-    if (a.mask_kind == TRL_MASK_BITS) return mask_row[tok >> 3] & in;  // tok is a multiple of 8
+    if (kind == TRL_MASK_NONE) return in;
+    if (kind == TRL_MASK_BITS) return mask_lo[off >> 3] & in;
     u32 bits = 0;
     if (n >= kVec) {
         typedef u32 u32x2 __attribute__((ext_vector_type(2)));
         typedef u32x2 u32x2_any __attribute__((aligned(1)));
-        const u32x2 w = *(const u32x2_any *)(mask_row + tok);  // 8 truth values of one byte
+        const u32x2 w = *(const u32x2_any *)(mask_lo + off);  // 8 truth values of one byte
         // byte i's lowest bit to bit 24 + i: no carries, the partial products do not meet
         bits = (((w[0] & 0x01010101u) * 0x01020408u) >> 24 & 0xfu) | (((w[1] & 0x01010101u) * 0x01020408u) >> 20 & 0xf0u);
     } else {
 #pragma unroll
         for (int i = 0; i < kVec; ++i)
-            if (i < n && mask_row[tok + i]) bits |= 1u << i;
+            if (i < n && mask_lo[off + i]) bits |= 1u << i;
     }
     return bits;
 }
 
-struct RowParams { float rep, inv_rep, pres, freq, inv_temp; };
-
-// z (in: the raw logits; out: the processed ones), slope = d processed / d raw.  `bits`: what the mask allows.
-template <bool PEN, bool SLOPE>
-__device__ __forceinline__ void process8(float *z, float *slope, u32 bits, const RowParams &p, const u32 *counts8, const void *bias_row,
-                                         int bias_kind, i64 tok, int n) {
-    if constexpr (SLOPE) {
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) slope[i] = p.inv_temp;
+__device__ __forceinline__ void load_bias8(int kind, const char *bias_row, i64 tok, int n, float *b) {
+    if (kind == kBiasF32) {
+        Raw8<float> r{};
+        load8((const float *)bias_row + tok, n, r);
+        unpack8(r, b);
+    } else if (kind == kBiasBf16) {
+        Raw8<__bf16> r{};
+        load8((const __bf16 *)bias_row + tok, n, r);
+        unpack8(r, b);
+    } else {
+        Raw8<_Float16> r{};
+        load8((const _Float16 *)bias_row + tok, n, r);
+        unpack8(r, b);
     }
-    if constexpr (PEN) {
-        const u32x4 c0 = *(const u32x4 *)counts8, c1 = *(const u32x4 *)(counts8 + kBlk / 2);
-        const u32 any = (c0[0] | c0[1] | c0[2]) | (c0[3] | c1[0] | c1[1]) | (c1[2] | c1[3]);
-        if (__any(any != 0)) {
+}
+
+struct Penalties { float rep, inv_rep, pres, freq; };
+
+// 8 counts of a lane; a wave whose 512 tokens hold none of the history's skips the rest, and so does each of the 8 places
+struct Counts8 {
+    u32 c[kVec];
+    bool any;
+    __device__ __forceinline__ Counts8() : any(false) {}
+    __device__ __forceinline__ explicit Counts8(const u32 *counts8) {
+        const u32x4 lo = *(const u32x4 *)counts8, hi = *(const u32x4 *)(counts8 + kBlk / 2);
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) {
-                const u32 c = i < 4 ? c0[i & 3] : c1[i & 3], k = c & ~kSeenInPrompt;
-                float f = z[i] > 0.0f ? p.inv_rep : p.rep;
-                f = c ? f : 1.0f;
-                const float sub = k ? fmaf((float)k, p.freq, p.pres) : 0.0f;
-                z[i] = fmaf(z[i], f, -sub);
-                if constexpr (SLOPE) slope[i] *= f;
+        for (int i = 0; i < 4; ++i) { c[i] = lo[i]; c[4 + i] = hi[i]; }
+        any = __any(((c[0] | c[1] | c[2]) | (c[3] | c[4] | c[5]) | (c[6] | c[7])) != 0);
+    }
+    __device__ __forceinline__ static float factor(float z, const Penalties &p) { return z > 0.0f ? p.inv_rep : p.rep; }
+    __device__ __forceinline__ void apply(float *z, const Penalties &p) const {
+        if (!any) return;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+            if (c[i]) {
+                const u32 k = c[i] & ~kSeenInPrompt;
+                z[i] = fmaf(z[i], factor(z[i], p), k ? -fmaf((float)k, p.freq, p.pres) : 0.0f);
             }
         }
     }
-    if (bias_kind != kBiasNone) {
-        float b[kVec];
-        if (bias_kind == kBiasF32) {
-            Raw8<float> r;
-            load8((const float *)bias_row + tok, n, r);
-            unpack8(r, b);
-        } else if (bias_kind == kBiasBf16) {
-            Raw8<__bf16> r;
-            load8((const __bf16 *)bias_row + tok, n, r);
-            unpack8(r, b);
-        } else {
-            Raw8<_Float16> r;
-            load8((const _Float16 *)bias_row + tok, n, r);
-            unpack8(r, b);
-        }
+    __device__ __forceinline__ void slope(float *d, const float *raw, const Penalties &p) const {
+        if (!any) return;
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) z[i] += b[i];
+        for (int i = 0; i < kVec; ++i)
+            if (c[i]) d[i] *= factor(raw[i], p);
     }
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-        z[i] *= p.inv_temp;
-        if (!(bits & (1u << i))) z[i] = neg_inf();
-    }
+};
+
+// place i is not allowed: all bits set
+__device__ __forceinline__ u32 barred(u32 bits, int i) { return (u32)__builtin_amdgcn_sbfe((int)~bits, i, 1); }
+__device__ __forceinline__ float where_allowed(u32 bits, int i, float z, u32 other) {
+    const u32 m = barred(bits, i);
+    return __builtin_bit_cast(float, (__builtin_bit_cast(u32, z) & ~m) | (other & m));
 }
+constexpr u32 kNegInfBits = 0xff800000u;
 
 __device__ __forceinline__ float wave_max_f(float x) {
     x = fmaxf(x, dpp_mov<0xB1>(x));
@@ -147,203 +155,285 @@ __device__ __forceinline__ float softmax_shift(float m, bool *steep) {
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-template <typename T, int MODE, bool PEN, int W>
+// What a lane knows of row t0 + lane before the block's rows begin: a row's scalars are then one v_readlane away, not a memory latency.
+struct RowAhead {
+    int want = 0;    // PEN: length of the history
+    int action = 0;  // -1: padding; 0x7fffffff: no token of the vocabulary
+    // backward: d processed = -e (ca + cb d), + g at the action
+    float shift = 0.0f, top = 0.0f, ca = 0.0f, cb = 0.0f, g = 0.0f;
+    int kind = 0;  // kRowZero, kRowSteep
+};
+enum { kRowZero = 1, kRowSteep = 2 };  // no gradient; subtract first
+
+template <typename T, int MODE, bool PEN, bool BIAS, int W>
 __global__ __launch_bounds__(W *kWave) void token_kernel(TokenArgs a) {
-    constexpr bool kBwd = MODE == kProcessBwd || MODE == kLogProbBwd;
     extern __shared__ __align__(16) u32 lds_counts[];  // PEN: W * kSub words
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const i64 blk = blockIdx.x;
-    const i64 slice = blk % a.nslices, rest = blk / a.nslices, chunk = rest % a.nchunks, b = rest / a.nchunks;
-    const i64 t0 = chunk * a.chunk, t1 = t0 + a.chunk < a.T ? t0 + a.chunk : a.T;
-    const i64 slice_lo = slice * (W * kSub), lo = slice_lo + (i64)wave * kSub;
+    const u32 nslices = (u32)a.nslices, nchunks = (u32)a.nchunks, rest = blockIdx.x / nslices, slice = blockIdx.x - rest * nslices;
+    const i64 b = rest / nchunks, t0 = (i64)(rest - (u32)b * nchunks) * a.chunk;
+    const int rows = a.T - t0 < a.chunk ? (int)(a.T - t0) : (int)a.chunk;
+    const i64 slice_lo = (i64)slice * (W * kSub), lo = slice_lo + wave * kSub, r0 = b * a.T + t0;
     u32 *counts = lds_counts + wave * kSub;
 
-    i64 h = 0, prompt = 0;  // history tokens that the counts hold; where the generated ones begin
+    RowAhead mine;
+    if (lane < rows) {
+        if constexpr (PEN) {
+            const i64 n = a.lengths ? load_int(a.lengths, a.lengths_wide, r0 + lane) : a.L;
+            mine.want = n < 0 ? 0 : n > a.L ? (int)a.L : (int)n;
+        }
+        if constexpr (MODE == kLogProb || MODE == kLogProbBwd) {
+            const i64 y = load_int(a.action, a.action_wide, r0 + lane);
+            mine.action = y < 0 ? -1 : y >= a.V ? 0x7fffffff : (int)y;
+        }
+    }
+    int h = 0, prompt = 0;  // history tokens that the counts hold; where the generated ones begin
     if constexpr (PEN) {
-        prompt = a.prompt ? load_int(a.prompt, a.prompt_wide, b) : 0;
+        const i64 p = a.prompt ? load_int(a.prompt, a.prompt_wide, b) : 0;
+        prompt = p < 0 ? 0 : p > a.L ? (int)a.L : (int)p;
         u32x4 *c4 = (u32x4 *)lds_counts;
 #pragma unroll
         for (int i = 0; i < kSub / 4 / kWave; ++i) c4[threadIdx.x + i * (W * kWave)] = u32x4{0, 0, 0, 0};
         __syncthreads();
-        h = a.lengths ? load_int(a.lengths, a.lengths_wide, b * a.T + t0) : a.L;
-        h = h < 0 ? 0 : h > a.L ? a.L : h;
-        for (i64 j = threadIdx.x; j < h; j += W * kWave)
+        h = read_lane(mine.want, 0);
+        for (int j = threadIdx.x; j < h; j += W * kWave)
             count_token(lds_counts, load_int(a.tokens, a.tokens_wide, b * a.tokens_sb + j), slice_lo, W * kSub, j < prompt);
         __syncthreads();
     }
     if (lo >= a.V) return;
 
-    RowParams p;
-    p.rep = a.rep_t ? a.rep_t[b] : a.rep;
-    p.inv_rep = 1.0f / p.rep;
-    p.pres = a.pres_t ? a.pres_t[b] : a.pres;
-    p.freq = a.freq_t ? a.freq_t[b] : a.freq;
-    p.inv_temp = 1.0f / (a.temp_t ? a.temp_t[b] : a.temp);
+    const Penalties pen{a.rep_t ? a.rep_t[b] : a.rep, 1.0f / (a.rep_t ? a.rep_t[b] : a.rep), a.pres_t ? a.pres_t[b] : a.pres, a.freq_t ? a.freq_t[b] : a.freq};
+    const float inv_temp = 1.0f / (a.temp_t ? a.temp_t[b] : a.temp);
     const bool needs_z = MODE != kProcessBwd || (PEN && (a.rep_t || a.rep != 1.0f));
-
-    i64 win_lo = 0;
-    i64 win = -1;
-    bool have_win = false;
-
-    i64 tok[kRowVecs];
-    int nv[kRowVecs];
-#pragma unroll
-    for (int k = 0; k < kRowVecs; ++k) {
-        tok[k] = lo + k * kBlk + lane * kVec;
-        const i64 left = a.V - tok[k];
-        nv[k] = left > kVec ? kVec : left < 0 ? 0 : (int)left;
-    }
-    u32 next_bits[kRowVecs];
-    const u8 *mask_row = a.mask_kind == TRL_MASK_NONE ? nullptr : (const u8 *)a.mask + b * a.mask_sb + t0 * a.mask_st;
-#pragma unroll
-    for (int k = 0; k < kRowVecs; ++k) next_bits[k] = mask_bits(a, mask_row, tok[k], nv[k]);
-
-    for (i64 t = t0; t < t1; ++t) {
-        const i64 r = b * a.T + t;
-        u32 bits[kRowVecs];
-#pragma unroll
-        for (int k = 0; k < kRowVecs; ++k) bits[k] = next_bits[k];
-        if (t + 1 < t1 && a.mask_kind != TRL_MASK_NONE && a.mask_st != 0) {
-            const u8 *row = (const u8 *)a.mask + b * a.mask_sb + (t + 1) * a.mask_st;
-#pragma unroll
-            for (int k = 0; k < kRowVecs; ++k) next_bits[k] = mask_bits(a, row, tok[k], nv[k]);
-        }
-        // -- the row's scalars
-        i64 y = 0;
-        float g_lp = 0.0f, ca = 0.0f, cb = 0.0f, shift = 0.0f, top = 0.0f;
-        bool zero_row = false, steep = false;
-        if constexpr (MODE == kLogProb || MODE == kLogProbBwd) {
-            y = load_int(a.action, a.action_wide, r);
-            if constexpr (MODE == kLogProb) {
-                if (y < 0) continue;  // padding: the joining launch answers for it
+    if constexpr (MODE == kLogProbBwd) {
+        if (lane < rows) {
+            const i64 r = r0 + lane;
+            const float m = a.stats[2 * r], log2s = a.stats[2 * r + 1];
+            if (mine.action < 0 || (m == neg_inf() && log2s == 0.0f)) {  // padding, or nothing allowed (a row of NaN has a NaN in its sum)
+                mine.kind = kRowZero;
             } else {
-                const float m = a.stats[2 * r], log2s = a.stats[2 * r + 1];
-                zero_row = y < 0 || (m == neg_inf() && log2s == 0.0f);  // a row of NaN has a NaN there
-                if (!zero_row) {
-                    const float g_h = a.g_entropy ? a.g_entropy[r] : 0.0f, rs = exp2_hw(-log2s);
-                    g_lp = a.g_log_prob ? a.g_log_prob[r] : 0.0f;
-                    if (y >= a.V) g_lp = __builtin_nanf("");
-                    top = m;
-                    shift = softmax_shift(m, &steep);
-                    ca = rs * (g_lp + g_h * (a.entropy[r] - kLn2 * log2s));
-                    cb = rs * g_h * kLn2;
-                }
+                bool steep;
+                mine.shift = softmax_shift(m, &steep);
+                mine.top = m;
+                const float g_h = a.g_entropy ? a.g_entropy[r] : 0.0f, rs = exp2_hw(-log2s);
+                float g = a.g_log_prob ? a.g_log_prob[r] : 0.0f;
+                if (mine.action == 0x7fffffff) g = __builtin_nanf("");
+                const float entropy = a.g_entropy ? a.entropy[r] : 0.0f;
+                mine.ca = rs * (g + g_h * (entropy - kLn2 * log2s)) * inv_temp;
+                mine.cb = rs * g_h * kLn2 * inv_temp;
+                mine.g = g * inv_temp;
+                mine.kind = steep ? kRowSteep : 0;
             }
         }
-        // -- loads
-        const T *z_row = (const T *)a.logits + b * a.logits_sb + t * a.logits_st;
-        Raw8<T> zr[kRowVecs], gr[kRowVecs];
+    }
+
+    // a window of the history, a token a lane
+    int win_lo = 0, win_end = 0;
+    i64 win = -1;
+    auto grow_history = [&](int want) {
+        if (want < h) {  // not a rollout's order: count anew
+            wave_fence();
+            u32x4 *c4 = (u32x4 *)counts;
+#pragma unroll
+            for (int i = 0; i < kSub / 4 / kWave; ++i) c4[lane + i * kWave] = u32x4{0, 0, 0, 0};
+            h = 0;
+        }
+        wave_fence();
+        while (h < want) {
+            if (h < win_lo || h >= win_end) {
+                win_lo = h;
+                win_end = h + kWave;
+                win = h + lane < (int)a.L ? load_int(a.tokens, a.tokens_wide, b * a.tokens_sb + h + lane) : -1;
+            }
+            const int end = want < win_end ? want : win_end, j = win_lo + lane;
+            if (j >= h && j < end) count_token(counts, win, lo, kSub, j < prompt);
+            h = end;
+        }
+        wave_fence();
+    };
+
+    const i64 left = a.V - lo;
+    const i64 elem0 = lo;
+    const T *z_lo = (const T *)a.logits + b * a.logits_sb + t0 * a.logits_st + elem0;
+    const i64 mask_step = a.mask_kind == TRL_MASK_BITS ? lo >> 3 : lo;
+    const u8 *mask_lo = a.mask_kind == TRL_MASK_NONE ? nullptr : (const u8 *)a.mask + b * a.mask_sb + t0 * a.mask_st + mask_step;
+
+    // FULL: every token of the sub-slice exists
+    auto run_rows = [&](auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        int off[kRowVecs], nv[kRowVecs];
+        u32 next_bits[kRowVecs];
 #pragma unroll
         for (int k = 0; k < kRowVecs; ++k) {
-            zr[k] = Raw8<T>{};
-            if (needs_z && bits[k] && !zero_row) load8(z_row + tok[k], nv[k], zr[k]);
-            if constexpr (MODE == kProcessBwd) {
-                gr[k] = Raw8<T>{};
-                if (bits[k]) load8((const T *)a.grad_out + r * a.V + tok[k], nv[k], gr[k]);
+            off[k] = k * kBlk + lane * kVec;
+            nv[k] = FULL || left - off[k] > kVec ? kVec : left < off[k] ? 0 : (int)(left - off[k]);
+            next_bits[k] = mask_bits(a.mask_kind, mask_lo, off[k], nv[k]);
+        }
+        float bias[BIAS ? kRowVecs : 1][kVec];
+        if constexpr (BIAS) {
+            if (a.bias_st == 0) {  // one bias for all rows of the block: kept in registers
+                const char *row = (const char *)a.bias + b * a.bias_sb;
+#pragma unroll
+                for (int k = 0; k < kRowVecs; ++k) load_bias8(a.bias_kind, row, elem0 + off[k], nv[k], bias[k]);
             }
         }
-        // -- the history grows to this row's
-        if constexpr (PEN) {
-            i64 want = a.lengths ? load_int(a.lengths, a.lengths_wide, r) : a.L;
-            want = want < 0 ? 0 : want > a.L ? a.L : want;
-            if (want != h) {
-                if (want < h) {  // not a rollout's order: count anew
-                    wave_fence();
-                    u32x4 *c4 = (u32x4 *)counts;
-#pragma unroll
-                    for (int i = 0; i < kSub / 4 / kWave; ++i) c4[lane + i * kWave] = u32x4{0, 0, 0, 0};
-                    h = 0;
-                }
-                wave_fence();
-                while (h < want) {
-                    if (!have_win || h < win_lo || h >= win_lo + kWave) {
-                        win_lo = h;
-                        have_win = true;
-                        const i64 j = h + lane;
-                        win = j < a.L ? load_int(a.tokens, a.tokens_wide, b * a.tokens_sb + j) : -1;
-                    }
-                    const i64 end = want < win_lo + kWave ? want : win_lo + kWave, j = win_lo + lane;
-                    if (j >= h && j < end) count_token(counts, win, lo, kSub, j < prompt);
-                    h = end;
-                }
-                wave_fence();
-            }
-        }
-        const void *bias_row = nullptr;
-        if (a.bias_kind != kBiasNone) bias_row = (const char *)a.bias + (b * a.bias_sb + t * a.bias_st);
-
-        if constexpr (MODE == kLogProb) {
-            float z[kRowVecs][kVec];
-            float m = neg_inf();
+        for (int i_row = 0; i_row < rows; ++i_row) {
+            const i64 t = t0 + i_row, r = r0 + i_row;
+            u32 bits[kRowVecs];
+            bool live[kRowVecs];  // of the wave
 #pragma unroll
             for (int k = 0; k < kRowVecs; ++k) {
-                unpack8(zr[k], z[k]);
-                process8<PEN, false>(z[k], nullptr, bits[k], p, counts + k * kBlk + lane * 4, bias_row, a.bias_kind, tok[k], nv[k]);
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) m = fmaxf(m, z[k][i]);
+                bits[k] = next_bits[k];
+                live[k] = __any(bits[k] != 0);
             }
-            m = wave_max_f(m);
-            if (y >= lo && y < lo + kSub && y < a.V) {
+            if (a.mask_st != 0 && i_row + 1 < rows) {
+                mask_lo += a.mask_st;
+#pragma unroll
+                for (int k = 0; k < kRowVecs; ++k) next_bits[k] = mask_bits(a.mask_kind, mask_lo, off[k], nv[k]);
+            }
+            const T *z_row = z_lo + i_row * a.logits_st;
+            T *out_row = (T *)a.out + b * a.out_sb + t * a.out_st + elem0;
+            const int y = MODE == kLogProb || MODE == kLogProbBwd ? read_lane(mine.action, i_row) : 0;
+            const int kind = MODE == kLogProbBwd ? read_lane(mine.kind, i_row) : 0;
+            if (MODE == kLogProb && y < 0) continue;  // padding: the joining launch answers for it
+            if (MODE == kLogProbBwd && (kind & kRowZero)) {
+                const float zero[kVec] = {};
 #pragma unroll
                 for (int k = 0; k < kRowVecs; ++k)
-#pragma unroll
-                    for (int i = 0; i < kVec; ++i)
-                        if (tok[k] + i == y) a.z_action[r] = z[k][i];
+                    if (FULL || nv[k] > 0) store8(out_row + off[k], nv[k], zero);
+                continue;
             }
-            bool steep;
-            const float shift = softmax_shift(m, &steep);
-            if (steep) {
-#pragma unroll
-                for (int k = 0; k < kRowVecs; ++k)
-#pragma unroll
-                    for (int i = 0; i < kVec; ++i) z[k][i] -= m;
-            }
-            float s = 0.0f, u = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kRowVecs; ++k)
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    const float d = fmaf(z[k][i], kLog2e, -shift), e = exp2_hw(d);
-                    s += e;
-                    u = fmaf(e, fmaxf(d, kFloor), u);
-                }
-            s = wave_sum_f(s);
-            u = wave_sum_f(u);
-            if (lane == 0) ((float4 *)a.partials)[r * a.nsubs + lo / kSub] = make_float4(m, s, u, 0.0f);
-        } else {
+            // -- loads; a lane with nothing allowed makes none
+            Raw8<T> zr[kRowVecs], gr[MODE == kProcessBwd ? kRowVecs : 1];
 #pragma unroll
             for (int k = 0; k < kRowVecs; ++k) {
-                float z[kVec], slope[kVec];
-                unpack8(zr[k], z);
-                process8<PEN, kBwd>(z, slope, bits[k], p, counts + k * kBlk + lane * 4, MODE == kProcessBwd ? nullptr : bias_row,
-                                    MODE == kProcessBwd ? (int)kBiasNone : a.bias_kind, tok[k], bits[k] ? nv[k] : 0);
+                zr[k] = Raw8<T>{};
+                if (needs_z && bits[k]) load8(z_row + off[k], nv[k], zr[k]);
                 if constexpr (MODE == kProcessBwd) {
-                    unpack8(gr[k], z);
-#pragma unroll
-                    for (int i = 0; i < kVec; ++i) z[i] = bits[k] & (1u << i) ? z[i] * slope[i] : 0.0f;
+                    gr[k] = Raw8<T>{};
+                    if (bits[k]) load8((const T *)a.grad_out + r * a.V + elem0 + off[k], nv[k], gr[k]);
                 }
-                if constexpr (MODE == kLogProbBwd) {
+            }
+            if constexpr (PEN) {
+                const int want = read_lane(mine.want, i_row);
+                if (want != h) grow_history(want);
+            }
+            if constexpr (BIAS) {
+                if (a.bias_st != 0) {
+                    const char *row = (const char *)a.bias + b * a.bias_sb + t * a.bias_st;
+#pragma unroll
+                    for (int k = 0; k < kRowVecs; ++k) load_bias8(a.bias_kind, row, elem0 + off[k], nv[k], bias[k]);
+                }
+            }
+            auto processed = [&](int k, float *z, const Counts8 &c) {
+                if constexpr (PEN) c.apply(z, pen);
+                if constexpr (BIAS) {
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) z[i] += bias[k][i];
+                }
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) z[i] *= inv_temp;
+                if (!FULL || !__all(bits[k] == 0xffu)) {
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) z[i] = where_allowed(bits[k], i, z[i], kNegInfBits);
+                }
+            };
+            const u32 *counts8 = counts + lane * 4;
+
+            if constexpr (MODE == kLogProb) {
+                float z[kRowVecs][kVec];
+                float m = neg_inf();
+#pragma unroll
+                for (int k = 0; k < kRowVecs; ++k) {
+                    if (!live[k]) continue;
+                    unpack8(zr[k], z[k]);
+                    processed(k, z[k], PEN ? Counts8(counts8 + k * kBlk) : Counts8());
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) m = fmaxf(m, z[k][i]);
+                }
+                m = wave_max_f(m);
+                if (y >= lo && y < lo + kSub) {
+                    const int at = (int)(y - lo);
+#pragma unroll
+                    for (int k = 0; k < kRowVecs; ++k)
+#pragma unroll
+                        for (int i = 0; i < kVec; ++i)
+                            if (off[k] + i == at) a.z_action[r] = live[k] ? z[k][i] : neg_inf();
+                }
+                bool steep;
+                const float shift = softmax_shift(m, &steep);
+                float s = 0.0f, u = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kRowVecs; ++k) {
+                    if (!live[k]) continue;
                     if (steep) {
 #pragma unroll
-                        for (int i = 0; i < kVec; ++i) z[i] -= top;
+                        for (int i = 0; i < kVec; ++i) z[k][i] -= m;
                     }
 #pragma unroll
                     for (int i = 0; i < kVec; ++i) {
-                        const float d = fmaf(z[i], kLog2e, -shift), e = exp2_hw(d);
-                        z[i] = -e * fmaf(cb, fmaxf(d, kFloor), ca);
+                        const float d = fmaf(z[k][i], kLog2e, -shift), e = exp2_hw(d);
+                        s += e;
+                        u = fmaf(e, fmaxf(d, kFloor), u);
                     }
-                    if (y >= lo && y < lo + kSub) {
-#pragma unroll
-                        for (int i = 0; i < kVec; ++i)
-                            if (tok[k] + i == y) z[i] += g_lp;
-                    }
-#pragma unroll
-                    for (int i = 0; i < kVec; ++i) z[i] = (bits[k] & (1u << i)) && !zero_row ? z[i] * slope[i] : 0.0f;
                 }
-                if (nv[k] > 0) store8((T *)a.out + b * a.out_sb + t * a.out_st + tok[k], nv[k], z);
+                s = wave_sum_f(s);
+                u = wave_sum_f(u);
+                if (lane == 0) ((float4 *)a.partials)[r * a.nsubs + lo / kSub] = make_float4(m, s, u, 0.0f);
+            } else {
+                const float shift = read_lane(mine.shift, i_row), top = read_lane(mine.top, i_row), ca = read_lane(mine.ca, i_row),
+                            cb = read_lane(mine.cb, i_row), g = read_lane(mine.g, i_row);
+#pragma unroll
+                for (int k = 0; k < kRowVecs; ++k) {
+                    float z[kVec];
+                    if (!live[k]) {
+#pragma unroll
+                        for (int i = 0; i < kVec; ++i) z[i] = MODE == kProcess ? neg_inf() : 0.0f;
+                    } else {
+                        const Counts8 c = PEN ? Counts8(counts8 + k * kBlk) : Counts8();
+                        float raw[kVec];
+                        unpack8(zr[k], raw);
+                        if constexpr (MODE == kProcessBwd) {
+                            unpack8(gr[k], z);
+#pragma unroll
+                            for (int i = 0; i < kVec; ++i) z[i] *= inv_temp;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < kVec; ++i) z[i] = raw[i];
+                            processed(k, z, c);
+                        }
+                        if constexpr (MODE == kLogProbBwd) {
+                            if (kind & kRowSteep) {
+#pragma unroll
+                                for (int i = 0; i < kVec; ++i) z[i] -= top;
+                            }
+#pragma unroll
+                            for (int i = 0; i < kVec; ++i) {
+                                const float d = fmaf(z[i], kLog2e, -shift), e = exp2_hw(d);
+                                z[i] = -e * fmaf(cb, fmaxf(d, kFloor), ca);
+                            }
+                            const i64 at = y - lo - k * kBlk;
+                            if (at >= 0 && at < kBlk) {  // one vector of one wave
+#pragma unroll
+                                for (int i = 0; i < kVec; ++i)
+                                    if (lane * kVec + i == (int)at) z[i] += g;
+                            }
+                        }
+                        if constexpr (PEN && MODE != kProcess) c.slope(z, raw, pen);
+                        // masked places have e = 0; an action among them, and coefficients that are no numbers, need the zero itself
+                        if (MODE == kProcessBwd || MODE == kLogProbBwd) {
+                            if (!__all(bits[k] == 0xffu)) {
+#pragma unroll
+                                for (int i = 0; i < kVec; ++i) z[i] = where_allowed(bits[k], i, z[i], 0u);
+                            }
+                        }
+                    }
+                    if (FULL || nv[k] > 0) store8(out_row + off[k], nv[k], z);
+                }
             }
         }
-    }
+    };
+    if (left >= kSub) run_rows(Bool<true>());
+    else run_rows(Bool<false>());
 }
 
 // Joins a row's partials: one wave a row.
@@ -394,24 +484,27 @@ __global__ __launch_bounds__(256) void token_join_kernel(TokenArgs a) {
     }
 }
 
-template <typename T, int MODE, bool PEN, int W>
+template <typename T, int MODE, bool PEN, bool BIAS, int W>
 int launch_w(hipStream_t s, TokenArgs &a) {
     const i64 span = (i64)W * kSub;
     a.nslices = (a.V + span - 1) / span;
     a.nsubs = token_subs(a.V);
     const i64 units = a.nslices * a.B * a.T;
-    a.chunk = units / 2048;  // enough blocks for every compute unit, then as long a run of rows as that leaves
-    a.chunk = a.chunk < 1 ? 1 : a.chunk > 64 ? 64 : a.chunk;
+    a.chunk = units / 2048;  // enough blocks for every compute unit, then as long a run of rows as that leaves (a lane holds a row's scalars)
+    a.chunk = a.chunk < 1 ? 1 : a.chunk > kWave ? kWave : a.chunk;
     if (a.chunk > a.T) a.chunk = a.T;
     a.nchunks = (a.T + a.chunk - 1) / a.chunk;
     const i64 grid = a.nslices * a.nchunks * a.B;
     if (grid > 0x7fffffffLL) return 2;
-    hipLaunchKernelGGL((token_kernel<T, MODE, PEN, W>), dim3((unsigned)grid), dim3(W * kWave), PEN ? W * kSub * sizeof(u32) : 0, s, a);
+    hipLaunchKernelGGL((token_kernel<T, MODE, PEN, BIAS, W>), dim3((unsigned)grid), dim3(W * kWave), PEN ? W * kSub * sizeof(u32) : 0, s, a);
     return 0;
 }
 template <typename T, int MODE>
 int launch_mode(hipStream_t s, TokenArgs &a) {
-    return a.tokens ? launch_w<T, MODE, true, 8>(s, a) : launch_w<T, MODE, false, 4>(s, a);
+    if constexpr (MODE != kProcessBwd) {
+        if (a.bias_kind != kBiasNone) return a.tokens ? launch_w<T, MODE, true, true, 8>(s, a) : launch_w<T, MODE, false, true, 4>(s, a);
+    }
+    return a.tokens ? launch_w<T, MODE, true, false, 8>(s, a) : launch_w<T, MODE, false, false, 4>(s, a);
 }
 template <int MODE>
 int launch_dtype(hipStream_t s, TokenArgs &a) {
