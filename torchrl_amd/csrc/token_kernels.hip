@@ -166,7 +166,7 @@ struct RowAhead {
 enum { kRowZero = 1, kRowSteep = 2 };  // no gradient; subtract first
 
 template <typename T, int MODE, bool PEN, bool BIAS, int W>
-__global__ __launch_bounds__(W *kWave) void token_kernel(TokenArgs a) {
+__global__ __launch_bounds__(W *kWave, 4) void token_kernel(TokenArgs a) {
     extern __shared__ __align__(16) u32 lds_counts[];  // PEN: W * kSub words
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const u32 nslices = (u32)a.nslices, nchunks = (u32)a.nchunks, rest = blockIdx.x / nslices, slice = blockIdx.x - rest * nslices;
