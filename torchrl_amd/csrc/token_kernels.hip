@@ -11,10 +11,10 @@
 //            64-token window of the history in registers).  Integer counts: the order of the atomics cannot change a result.
 //   masks    A lane's 8 mask bits of the NEXT row are fetched a row ahead, so lanes with nothing allowed skip their logits without
 //            a dependent load; masked logits are never read, whatever they hold.
-//   softmax  In base 2 with one fma an element: d = z * log2(e) - M, e = 2^d, all relative to M = max * log2(e) as rounded, so that
-//            M's rounding cancels between the numerator and the sum.  That rounding has to stay small in the exponent, so rows whose
-//            maximum is 2^20 or more in magnitude (rows of the type's lowest value among them) subtract first: d = (z - max) * log2(e).
-//            Everything is held in 32 bits.
+//   softmax  In base 2 with one fma an element: d = z * c - M, e = 2^d, c = log2(e) / temperature (z before the division), all
+//            relative to M = max * c as rounded, so that M's rounding cancels between the numerator and the sum.  It has to stay small
+//            in the exponent for that, so rows with a maximum of 2^20 or more in magnitude (rows of the type's lowest value among
+//            them) subtract first: d = (z - max) * c.  Everything is held in 32 bits.
 #include "token_common.h"
 #include "vec8.h"
 
@@ -26,6 +26,7 @@ constexpr int kSub = kBlk * kRowVecs;        // 2048 tokens of a wave
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr float kFloor = -1.0e4f;            // 2^kFloor is 0: keeps 0 * (-inf) out of the entropy
 constexpr u32 kSeenInPrompt = 0x80000000u;
+typedef unsigned long long u64;
 
 template <bool B>
 struct Bool { static constexpr bool value = B; };
@@ -92,46 +93,68 @@ __device__ __forceinline__ void load_bias8(int kind, const char *bias_row, i64 t
     }
 }
 
-struct Penalties { float rep, inv_rep, pres, freq; };
+struct Penalties { float rep, inv_rep, pres, freq; bool subtracts; };
 
-// 8 counts of a lane; a wave whose 512 tokens hold none of the history's skips the rest, and so does each of the 8 places
+// keeps a rarely taken scalar branch one (8 selects in its place cost more than the row's softmax)
+__device__ __forceinline__ void stay_branch(float &x) { asm volatile("" : "+v"(x)); }
+
+// 8 counts of a lane.  `places`, the same in all lanes: bit i where any lane's count i is not 0 -- a wave looks at those alone.
 struct Counts8 {
-    u32 c[kVec];
-    bool any;
-    __device__ __forceinline__ Counts8() : any(false) {}
-    __device__ __forceinline__ explicit Counts8(const u32 *counts8) {
+    u32 c[kVec], places;
+    __device__ __forceinline__ Counts8() : places(0) {}
+    __device__ __forceinline__ Counts8(const u32 *counts8, u32 p) : places(p) {
+        if (!places) return;
         const u32x4 lo = *(const u32x4 *)counts8, hi = *(const u32x4 *)(counts8 + kBlk / 2);
 #pragma unroll
         for (int i = 0; i < 4; ++i) { c[i] = lo[i]; c[4 + i] = hi[i]; }
-        any = __any(((c[0] | c[1] | c[2]) | (c[3] | c[4] | c[5]) | (c[6] | c[7])) != 0);
     }
-    __device__ __forceinline__ static float factor(float z, const Penalties &p) { return z > 0.0f ? p.inv_rep : p.rep; }
+    __device__ __forceinline__ static float factor(float z, u32 c, const Penalties &p) {
+        const float f = z > 0.0f ? p.inv_rep : p.rep;
+        return c ? f : 1.0f;
+    }
     __device__ __forceinline__ void apply(float *z, const Penalties &p) const {
-        if (!any) return;
+        if (!places) return;
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
-            if (c[i]) {
-                const u32 k = c[i] & ~kSeenInPrompt;
-                z[i] = fmaf(z[i], factor(z[i], p), k ? -fmaf((float)k, p.freq, p.pres) : 0.0f);
+            if (places & (1u << i)) {
+                z[i] *= factor(z[i], c[i], p);
+                stay_branch(z[i]);
+                if (p.subtracts) {
+                    const u32 k = c[i] & ~kSeenInPrompt;
+                    z[i] -= k ? fmaf((float)k, p.freq, p.pres) : 0.0f;
+                }
             }
         }
     }
     __device__ __forceinline__ void slope(float *d, const float *raw, const Penalties &p) const {
-        if (!any) return;
+        if (!places) return;
 #pragma unroll
         for (int i = 0; i < kVec; ++i)
-            if (c[i]) d[i] *= factor(raw[i], p);
+            if (places & (1u << i)) {
+                d[i] *= factor(raw[i], c[i], p);
+                stay_branch(d[i]);
+            }
     }
 };
 
-// place i is not allowed: all bits set
-__device__ __forceinline__ u32 barred(u32 bits, int i) { return (u32)__builtin_amdgcn_sbfe((int)~bits, i, 1); }
+// z where bit i allows it, else `other`: two instructions a place
 __device__ __forceinline__ float where_allowed(u32 bits, int i, float z, u32 other) {
-    const u32 m = barred(bits, i);
-    return __builtin_bit_cast(float, (__builtin_bit_cast(u32, z) & ~m) | (other & m));
+    const int m = __builtin_amdgcn_sbfe((int)bits, i, 1);  // all bits set where it is allowed
+    float r;
+    asm("v_bfi_b32 %0, %1, %2, %3" : "=v"(r) : "v"(m), "v"(z), "v"(other));
+    return r;
 }
 constexpr u32 kNegInfBits = 0xff800000u;
+// What stands for -inf in masked places of the log-probability's forward pass: 0 * d stays finite there without a clamp.  Waves whose
+// maximum comes near it, and waves whose weighted sum is NaN (infinities in allowed places), start over with -inf and a clamp.
+constexpr float kFarBelow = -1e30f;
 
+// (the builtin would first pass values of unknown origin through a multiplication by one)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 __device__ __forceinline__ float wave_max_f(float x) {
     x = fmaxf(x, dpp_mov<0xB1>(x));
     x = fmaxf(x, dpp_mov<0x4E>(x));
@@ -147,30 +170,43 @@ __device__ __forceinline__ float wave_sum_f(float x) {
     return (read_lane(x, 0) + read_lane(x, 16)) + (read_lane(x, 32) + read_lane(x, 48));
 }
 
-// the shift of d = z * log2(e) - shift for a row's (or a wave's) largest value m; *steep: d = (z - m) * log2(e), see the head of the file
-__device__ __forceinline__ float softmax_shift(float m, bool *steep) {
-    *steep = fabsf(m) >= 0x1p20f && !__builtin_isinf(m);
-    return m == neg_inf() || *steep ? 0.0f : m * kLog2e;
+// the shift of d = z * c - shift for a row's (or a wave's) largest value m; *steep: d = (z - m) * c, see the head of the file
+__device__ __forceinline__ float softmax_shift(float m, float c, bool *steep) {
+    const float m2 = m * c;
+    *steep = fabsf(m2) >= 0x1p20f && !__builtin_isinf(m);
+    return m == neg_inf() || *steep ? 0.0f : m2;
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A kernel argument as a scalar of its own.  Arguments are fetched 16 words at a time, and one that has to leave the scalar registers
+// would take its 15 neighbours with it, to vector lanes and back in every row.
+__device__ __forceinline__ int scalar(int v) {
+    v = __builtin_amdgcn_readfirstlane(v);
+    asm volatile("" : "+s"(v));
+    return v;
+}
+__device__ __forceinline__ i64 scalar(i64 v) { return (i64)((u64)(u32)scalar((int)v) | (u64)(u32)scalar((int)(v >> 32)) << 32); }
+__device__ __forceinline__ i64 scalar(int64_t v) { return scalar((i64)v); }
+template <typename P>
+__device__ __forceinline__ P *scalar(P *p) { return (P *)scalar((i64)p); }
 
 // What a lane knows of row t0 + lane before the block's rows begin: a row's scalars are then one v_readlane away, not a memory latency.
 struct RowAhead {
     int want = 0;    // PEN: length of the history
     int action = 0;  // -1: padding; 0x7fffffff: no token of the vocabulary
-    // backward: d processed = -e (ca + cb d), + g at the action
+    // backward: d raw = -e (ca + cb d), + g at the action
     float shift = 0.0f, top = 0.0f, ca = 0.0f, cb = 0.0f, g = 0.0f;
     int kind = 0;  // kRowZero, kRowSteep
 };
 enum { kRowZero = 1, kRowSteep = 2 };  // no gradient; subtract first
 
 template <typename T, int MODE, bool PEN, bool BIAS, int W>
-__global__ __launch_bounds__(W *kWave, 4) void token_kernel(TokenArgs a) {
+__global__ __launch_bounds__(W *kWave, PEN && BIAS ? 3 : 4) void token_kernel(TokenArgs a) {
     extern __shared__ __align__(16) u32 lds_counts[];  // PEN: W * kSub words
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const u32 nslices = (u32)a.nslices, nchunks = (u32)a.nchunks, rest = blockIdx.x / nslices, slice = blockIdx.x - rest * nslices;
-    const i64 b = rest / nchunks, t0 = (i64)(rest - (u32)b * nchunks) * a.chunk;
+    const u32 nslices = (u32)a.nslices, nchunks = (u32)a.nchunks, rest = scalar((int)(blockIdx.x / nslices)), slice = blockIdx.x - rest * nslices;
+    const i64 b = scalar((int)(rest / nchunks)), t0 = (i64)(rest - (u32)b * nchunks) * a.chunk;
     const int rows = a.T - t0 < a.chunk ? (int)(a.T - t0) : (int)a.chunk;
     const i64 slice_lo = (i64)slice * (W * kSub), lo = slice_lo + wave * kSub, r0 = b * a.T + t0;
     u32 *counts = lds_counts + wave * kSub;
@@ -201,8 +237,11 @@ __global__ __launch_bounds__(W *kWave, 4) void token_kernel(TokenArgs a) {
     }
     if (lo >= a.V) return;
 
-    const Penalties pen{a.rep_t ? a.rep_t[b] : a.rep, 1.0f / (a.rep_t ? a.rep_t[b] : a.rep), a.pres_t ? a.pres_t[b] : a.pres, a.freq_t ? a.freq_t[b] : a.freq};
+    Penalties pen{a.rep_t ? a.rep_t[b] : a.rep, 0.0f, a.pres_t ? a.pres_t[b] : a.pres, a.freq_t ? a.freq_t[b] : a.freq, false};
+    pen.inv_rep = 1.0f / pen.rep;
+    pen.subtracts = pen.pres != 0.0f || pen.freq != 0.0f;
     const float inv_temp = 1.0f / (a.temp_t ? a.temp_t[b] : a.temp);
+    const float scale = kLog2e * inv_temp;
     const bool needs_z = MODE != kProcessBwd || (PEN && (a.rep_t || a.rep != 1.0f));
     if constexpr (MODE == kLogProbBwd) {
         if (lane < rows) {
@@ -212,7 +251,7 @@ __global__ __launch_bounds__(W *kWave, 4) void token_kernel(TokenArgs a) {
                 mine.kind = kRowZero;
             } else {
                 bool steep;
-                mine.shift = softmax_shift(m, &steep);
+                mine.shift = softmax_shift(m, scale, &steep);
                 mine.top = m;
                 const float g_h = a.g_entropy ? a.g_entropy[r] : 0.0f, rs = exp2_hw(-log2s);
                 float g = a.g_log_prob ? a.g_log_prob[r] : 0.0f;
@@ -226,36 +265,68 @@ __global__ __launch_bounds__(W *kWave, 4) void token_kernel(TokenArgs a) {
         }
     }
 
-    // a window of the history, a token a lane
-    int win_lo = 0, win_end = 0;
-    i64 win = -1;
+    // bit k * 8 + i: some token of place i of the wave's vector k was seen
+    u32 seen_places = 0;
+    if constexpr (PEN) {
+#pragma unroll
+        for (int k = 0; k < kRowVecs; ++k) {
+            const Counts8 c(counts + k * kBlk + lane * 4, 1);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) seen_places |= __any(c.c[i] != 0) ? 1u << (k * kVec + i) : 0u;
+        }
+    }
+    // a window of the history, a token a lane, as its place in the sub-slice (negative: elsewhere), and which of them are here at all
+    const char *tokens = PEN ? scalar((const char *)a.tokens + b * a.tokens_sb * (a.tokens_wide ? 8 : 4)) : nullptr;
+    const int tokens_wide = PEN ? scalar(a.tokens_wide) : 0, n_tokens = PEN ? scalar((int)a.L) : 0;
+    int win_lo = 0, win_end = 0, win = -1;
+    unsigned long long win_hits = 0;
     auto grow_history = [&](int want) {
         if (want < h) {  // not a rollout's order: count anew
             wave_fence();
             u32x4 *c4 = (u32x4 *)counts;
 #pragma unroll
             for (int i = 0; i < kSub / 4 / kWave; ++i) c4[lane + i * kWave] = u32x4{0, 0, 0, 0};
+            wave_fence();
             h = 0;
+            seen_places = 0;
         }
-        wave_fence();
         while (h < want) {
             if (h < win_lo || h >= win_end) {
                 win_lo = h;
                 win_end = h + kWave;
-                win = h + lane < (int)a.L ? load_int(a.tokens, a.tokens_wide, b * a.tokens_sb + h + lane) : -1;
+                const i64 at = h + lane < n_tokens ? load_int(tokens, tokens_wide, h + lane) - lo : -1;
+                win = at >= 0 && at < kSub ? (int)at : -1;
+                win_hits = __ballot(win >= 0);
             }
-            const int end = want < win_end ? want : win_end, j = win_lo + lane;
-            if (j >= h && j < end) count_token(counts, win, lo, kSub, j < prompt);
+            const int end = want < win_end ? want : win_end;
+            unsigned long long todo = win_hits >> (h - win_lo);
+            if (end - h < kWave) todo &= (1ull << (end - h)) - 1;
+            if (todo) {
+                wave_fence();
+                for (; todo; todo &= todo - 1) {
+                    const int j = h + __builtin_ctzll(todo), at = read_lane(win, j - win_lo);
+                    if (lane == 0) count_token(counts, at, 0, kSub, j < prompt);
+                    seen_places |= 1u << (at / kBlk * kVec + at % kVec);
+                }
+                wave_fence();
+            }
             h = end;
         }
-        wave_fence();
     };
 
     const i64 left = a.V - lo;
-    const i64 elem0 = lo;
-    const T *z_lo = (const T *)a.logits + b * a.logits_sb + t0 * a.logits_st + elem0;
-    const i64 mask_step = a.mask_kind == TRL_MASK_BITS ? lo >> 3 : lo;
-    const u8 *mask_lo = a.mask_kind == TRL_MASK_NONE ? nullptr : (const u8 *)a.mask + b * a.mask_sb + t0 * a.mask_st + mask_step;
+    const int mask_kind = scalar(a.mask_kind);
+    const i64 logits_st = scalar(a.logits_st), out_st = scalar(a.out_st), mask_st = scalar(a.mask_st), nsubs = scalar(a.nsubs);
+    // of the next row
+    const T *z_next = scalar((const T *)a.logits + b * a.logits_sb + t0 * a.logits_st + lo);
+    const T *g_next = scalar((const T *)a.grad_out + r0 * a.V + lo);
+    T *out_next = scalar((T *)a.out + b * a.out_sb + t0 * a.out_st + lo);
+    const u8 *mask_next = scalar((const u8 *)a.mask + b * a.mask_sb + t0 * a.mask_st + (mask_kind == TRL_MASK_BITS ? lo >> 3 : lo));
+    const int bias_kind = scalar(a.bias_kind);
+    const i64 bias_st = scalar(a.bias_st), vocabulary = scalar(a.V);
+    const char *bias_next = scalar((const char *)a.bias + b * a.bias_sb + t0 * a.bias_st);
+    float4 *part_next = scalar((float4 *)a.partials + r0 * a.nsubs + lo / kSub);
+    float *z_action = scalar(a.z_action + r0);
 
     // FULL: every token of the sub-slice exists
     auto run_rows = [&](auto full) {
@@ -266,18 +337,16 @@ __global__ __launch_bounds__(W *kWave, 4) void token_kernel(TokenArgs a) {
         for (int k = 0; k < kRowVecs; ++k) {
             off[k] = k * kBlk + lane * kVec;
             nv[k] = FULL || left - off[k] > kVec ? kVec : left < off[k] ? 0 : (int)(left - off[k]);
-            next_bits[k] = mask_bits(a.mask_kind, mask_lo, off[k], nv[k]);
+            next_bits[k] = mask_bits(mask_kind, mask_next, off[k], nv[k]);
         }
         float bias[BIAS ? kRowVecs : 1][kVec];
         if constexpr (BIAS) {
-            if (a.bias_st == 0) {  // one bias for all rows of the block: kept in registers
-                const char *row = (const char *)a.bias + b * a.bias_sb;
+            if (bias_st == 0) {  // one bias for all rows of the block: kept in registers
 #pragma unroll
-                for (int k = 0; k < kRowVecs; ++k) load_bias8(a.bias_kind, row, elem0 + off[k], nv[k], bias[k]);
+                for (int k = 0; k < kRowVecs; ++k) load_bias8(bias_kind, bias_next, lo + off[k], nv[k], bias[k]);
             }
         }
         for (int i_row = 0; i_row < rows; ++i_row) {
-            const i64 t = t0 + i_row, r = r0 + i_row;
             u32 bits[kRowVecs];
             bool live[kRowVecs];  // of the wave
 #pragma unroll
@@ -285,13 +354,20 @@ __global__ __launch_bounds__(W *kWave, 4) void token_kernel(TokenArgs a) {
                 bits[k] = next_bits[k];
                 live[k] = __any(bits[k] != 0);
             }
-            if (a.mask_st != 0 && i_row + 1 < rows) {
-                mask_lo += a.mask_st;
+            if (mask_st != 0 && i_row + 1 < rows) {
+                mask_next += mask_st;
 #pragma unroll
-                for (int k = 0; k < kRowVecs; ++k) next_bits[k] = mask_bits(a.mask_kind, mask_lo, off[k], nv[k]);
+                for (int k = 0; k < kRowVecs; ++k) next_bits[k] = mask_bits(mask_kind, mask_next, off[k], nv[k]);
             }
-            const T *z_row = z_lo + i_row * a.logits_st;
-            T *out_row = (T *)a.out + b * a.out_sb + t * a.out_st + elem0;
+            const T *z_row = z_next, *g_row = g_next;
+            T *out_row = out_next;
+            const char *bias_row = bias_next;
+            float4 *part = part_next;
+            z_next += logits_st;
+            out_next += out_st;
+            bias_next += bias_st;
+            part_next += nsubs;
+            if constexpr (MODE == kProcessBwd) g_next += vocabulary;
             const int y = MODE == kLogProb || MODE == kLogProbBwd ? read_lane(mine.action, i_row) : 0;
             const int kind = MODE == kLogProbBwd ? read_lane(mine.kind, i_row) : 0;
             if (MODE == kLogProb && y < 0) continue;  // padding: the joining launch answers for it
@@ -310,7 +386,7 @@ __global__ __launch_bounds__(W *kWave, 4) void token_kernel(TokenArgs a) {
                 if (needs_z && bits[k]) load8(z_row + off[k], nv[k], zr[k]);
                 if constexpr (MODE == kProcessBwd) {
                     gr[k] = Raw8<T>{};
-                    if (bits[k]) load8((const T *)a.grad_out + r * a.V + elem0 + off[k], nv[k], gr[k]);
+                    if (bits[k]) load8(g_row + off[k], nv[k], gr[k]);
                 }
             }
             if constexpr (PEN) {
@@ -318,23 +394,25 @@ __global__ __launch_bounds__(W *kWave, 4) void token_kernel(TokenArgs a) {
                 if (want != h) grow_history(want);
             }
             if constexpr (BIAS) {
-                if (a.bias_st != 0) {
-                    const char *row = (const char *)a.bias + b * a.bias_sb + t * a.bias_st;
+                if (bias_st != 0) {
 #pragma unroll
-                    for (int k = 0; k < kRowVecs; ++k) load_bias8(a.bias_kind, row, elem0 + off[k], nv[k], bias[k]);
+                    for (int k = 0; k < kRowVecs; ++k) load_bias8(bias_kind, bias_row, lo + off[k], nv[k], bias[k]);
                 }
             }
-            auto processed = [&](int k, float *z, const Counts8 &c) {
+            // before the temperature
+            auto processed = [&](int k, float *z, const Counts8 &c, u32 fill) {
                 if constexpr (PEN) c.apply(z, pen);
                 if constexpr (BIAS) {
 #pragma unroll
                     for (int i = 0; i < kVec; ++i) z[i] += bias[k][i];
                 }
+                if constexpr (MODE == kProcess) {
 #pragma unroll
-                for (int i = 0; i < kVec; ++i) z[i] *= inv_temp;
+                    for (int i = 0; i < kVec; ++i) z[i] *= inv_temp;
+                }
                 if (!FULL || !__all(bits[k] == 0xffu)) {
 #pragma unroll
-                    for (int i = 0; i < kVec; ++i) z[i] = where_allowed(bits[k], i, z[i], kNegInfBits);
+                    for (int i = 0; i < kVec; ++i) z[i] = where_allowed(bits[k], i, z[i], fill);
                 }
             };
             const u32 *counts8 = counts + lane * 4;
@@ -342,43 +420,72 @@ __global__ __launch_bounds__(W *kWave, 4) void token_kernel(TokenArgs a) {
             if constexpr (MODE == kLogProb) {
                 float z[kRowVecs][kVec];
                 float m = neg_inf();
+                const i64 at = y - lo;
 #pragma unroll
                 for (int k = 0; k < kRowVecs; ++k) {
-                    if (!live[k]) continue;
+                    const bool has_action = at >= k * kBlk && at < (k + 1) * kBlk;  // one vector of one wave
+                    if (!live[k]) {
+                        if (has_action && lane == 0) z_action[i_row] = neg_inf();
+                        continue;
+                    }
                     unpack8(zr[k], z[k]);
-                    processed(k, z[k], PEN ? Counts8(counts8 + k * kBlk) : Counts8());
+                    processed(k, z[k], PEN ? Counts8(counts8 + k * kBlk, seen_places >> (k * kVec) & 0xffu) : Counts8(), __builtin_bit_cast(u32, kFarBelow));
 #pragma unroll
-                    for (int i = 0; i < kVec; ++i) m = fmaxf(m, z[k][i]);
-                }
-                m = wave_max_f(m);
-                if (y >= lo && y < lo + kSub) {
-                    const int at = (int)(y - lo);
-#pragma unroll
-                    for (int k = 0; k < kRowVecs; ++k)
+                    for (int i = 0; i < kVec; i += 2) m = max3(m, z[k][i], z[k][i + 1]);
+                    if (has_action) {
 #pragma unroll
                         for (int i = 0; i < kVec; ++i)
-                            if (off[k] + i == at) a.z_action[r] = live[k] ? z[k][i] : neg_inf();
+                            if (off[k] + i == (int)at) z_action[i_row] = bits[k] & (1u << i) ? z[k][i] : neg_inf();
+                    }
                 }
-                bool steep;
-                const float shift = softmax_shift(m, &steep);
+                m = wave_max_f(m);
                 float s = 0.0f, u = 0.0f;
+                bool steep;
+                float shift = softmax_shift(m, scale, &steep);
+                bool careful = steep || !(m > 0.01f * kFarBelow);  // (not live at all among them)
+                if (!careful) {
 #pragma unroll
-                for (int k = 0; k < kRowVecs; ++k) {
-                    if (!live[k]) continue;
-                    if (steep) {
+                    for (int k = 0; k < kRowVecs; ++k) {
+                        if (!live[k]) continue;
 #pragma unroll
-                        for (int i = 0; i < kVec; ++i) z[k][i] -= m;
+                        for (int i = 0; i < kVec; ++i) {
+                            const float d = fmaf(z[k][i], scale, -shift), e = exp2_hw(d);
+                            s += e;
+                            u = fmaf(e, d, u);
+                        }
                     }
-#pragma unroll
-                    for (int i = 0; i < kVec; ++i) {
-                        const float d = fmaf(z[k][i], kLog2e, -shift), e = exp2_hw(d);
-                        s += e;
-                        u = fmaf(e, fmaxf(d, kFloor), u);
-                    }
+                    s = wave_sum_f(s);
+                    u = wave_sum_f(u);
+                    careful = __builtin_isnan(u) && !__builtin_isnan(s);
                 }
-                s = wave_sum_f(s);
-                u = wave_sum_f(u);
-                if (lane == 0) ((float4 *)a.partials)[r * a.nsubs + lo / kSub] = make_float4(m, s, u, 0.0f);
+                if (careful) {
+                    m = neg_inf();
+                    s = u = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < kRowVecs; ++k) {
+                        if (!live[k]) continue;
+#pragma unroll
+                        for (int i = 0; i < kVec; ++i) {
+                            z[k][i] = where_allowed(bits[k], i, z[k][i], kNegInfBits);
+                            m = fmaxf(m, z[k][i]);
+                        }
+                    }
+                    m = wave_max_f(m);
+                    shift = softmax_shift(m, scale, &steep);
+#pragma unroll
+                    for (int k = 0; k < kRowVecs; ++k) {
+                        if (!live[k]) continue;
+#pragma unroll
+                        for (int i = 0; i < kVec; ++i) {
+                            const float d = fmaf(steep ? z[k][i] - m : z[k][i], scale, -shift), e = exp2_hw(d);
+                            s += e;
+                            u = fmaf(e, fmaxf(d, kFloor), u);
+                        }
+                    }
+                    s = wave_sum_f(s);
+                    u = wave_sum_f(u);
+                }
+                if (lane == 0) *part = make_float4(m, s, u, 0.0f);
             } else {
                 const float shift = read_lane(mine.shift, i_row), top = read_lane(mine.top, i_row), ca = read_lane(mine.ca, i_row),
                             cb = read_lane(mine.cb, i_row), g = read_lane(mine.g, i_row);
@@ -389,7 +496,7 @@ __global__ __launch_bounds__(W *kWave, 4) void token_kernel(TokenArgs a) {
 #pragma unroll
                         for (int i = 0; i < kVec; ++i) z[i] = MODE == kProcess ? neg_inf() : 0.0f;
                     } else {
-                        const Counts8 c = PEN ? Counts8(counts8 + k * kBlk) : Counts8();
+                        const Counts8 c = PEN ? Counts8(counts8 + k * kBlk, seen_places >> (k * kVec) & 0xffu) : Counts8();
                         float raw[kVec];
                         unpack8(zr[k], raw);
                         if constexpr (MODE == kProcessBwd) {
@@ -399,7 +506,7 @@ __global__ __launch_bounds__(W *kWave, 4) void token_kernel(TokenArgs a) {
                         } else {
 #pragma unroll
                             for (int i = 0; i < kVec; ++i) z[i] = raw[i];
-                            processed(k, z, c);
+                            processed(k, z, c, kNegInfBits);
                         }
                         if constexpr (MODE == kLogProbBwd) {
                             if (kind & kRowSteep) {
@@ -408,7 +515,7 @@ __global__ __launch_bounds__(W *kWave, 4) void token_kernel(TokenArgs a) {
                             }
 #pragma unroll
                             for (int i = 0; i < kVec; ++i) {
-                                const float d = fmaf(z[i], kLog2e, -shift), e = exp2_hw(d);
+                                const float d = fmaf(z[i], scale, -shift), e = exp2_hw(d);
                                 z[i] = -e * fmaf(cb, fmaxf(d, kFloor), ca);
                             }
                             const i64 at = y - lo - k * kBlk;
@@ -447,18 +554,19 @@ __global__ __launch_bounds__(256) void token_join_kernel(TokenArgs a) {
         const float4 *part = (const float4 *)a.partials + r * a.nsubs;
         for (i64 i = lane; i < a.nsubs; i += kWave) m = fmaxf(m, part[i].x);
         m = wave_max_f(m);
+        const float scale = kLog2e * (1.0f / (a.temp_t ? a.temp_t[r / a.T] : a.temp));  // the row kernel's own bits
         bool steep;
-        const float shift = softmax_shift(m, &steep);
+        const float shift = softmax_shift(m, scale, &steep);
         float s = 0.0f, u = 0.0f;
         for (i64 i = lane; i < a.nsubs; i += kWave) {
             const float4 q = part[i];
             float d = 0.0f;
             if (q.x != m) {
                 bool own;  // whether the wave's values are relative to q.x itself
-                const float its = softmax_shift(q.x, &own);
+                const float its = softmax_shift(q.x, scale, &own);
                 if (q.x == neg_inf()) d = neg_inf();
-                else if (own) d = steep ? (q.x - m) * kLog2e : fmaf(q.x, kLog2e, -shift);
-                else d = steep ? fmaf(-m, kLog2e, its) : its - shift;
+                else if (own) d = steep ? (q.x - m) * scale : fmaf(q.x, scale, -shift);
+                else d = steep ? fmaf(-m, scale, its) : its - shift;
             }
             const float w = exp2_hw(d);
             s = fmaf(w, q.y, s);
@@ -473,7 +581,7 @@ __global__ __launch_bounds__(256) void token_join_kernel(TokenArgs a) {
             if (steep) z -= m;
             log2s = log2f(s);
             entropy = kLn2 * (log2s - u / s);
-            log_prob = kLn2 * (fmaf(z, kLog2e, -shift) - log2s);
+            log_prob = kLn2 * (fmaf(z, scale, -shift) - log2s);
         }
         if (y >= a.V) log_prob = __builtin_nanf("");
     }
@@ -502,7 +610,7 @@ int launch_w(hipStream_t s, TokenArgs &a) {
 template <typename T, int MODE>
 int launch_mode(hipStream_t s, TokenArgs &a) {
     if constexpr (MODE != kProcessBwd) {
-        if (a.bias_kind != kBiasNone) return a.tokens ? launch_w<T, MODE, true, true, 8>(s, a) : launch_w<T, MODE, false, true, 4>(s, a);
+        if (a.bias_kind != kBiasNone) return a.tokens ? launch_w<T, MODE, true, true, 4>(s, a) : launch_w<T, MODE, false, true, 4>(s, a);
     }
     return a.tokens ? launch_w<T, MODE, true, false, 8>(s, a) : launch_w<T, MODE, false, false, 4>(s, a);
 }
