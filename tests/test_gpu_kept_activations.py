@@ -230,3 +230,43 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         for a, e in zip(outs, eager):
             assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_without_the_host_module(dtype, monkeypatch):
+    """The python route (a tree without lib/_trl_host.so) makes the same calls: the same bits."""
+    x = inputs(140, 75, dtype, seed=3).clamp(-50, 50).cuda().view(2, 70, 75)
+    w, b = (torch.randn(s, generator=torch.Generator().manual_seed(4)).to(dtype).cuda() for s in ((33, 75), (33,)))
+    dy = torch.randn(2, 70, 33, generator=torch.Generator().manual_seed(5)).to(dtype).cuda()
+
+    def everything():
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        y = checkpointed_linear(*leaves)
+        q = quantize_activation(x)
+        only_b = b.clone().requires_grad_()
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy), q.codes, q.exponents, q.dequantize(), q.dequantize(torch.float32),
+                *torch.autograd.grad(checkpointed_linear(x, w, only_b), only_b, dy))
+
+    assert F.host_fast_path()
+    fast = everything()
+    monkeypatch.setattr(F, "_HOST", None)
+    for got, want in zip(everything(), fast):
+        assert got.dtype == want.dtype and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,O_", [(1, 1), (37, 300), (5000, 7), (40000, 513)])
+def test_bias_gradient_alone(dtype, N, O_):
+    x = torch.zeros(N, 8, dtype=dtype, device="cuda")
+    dy = torch.randn(N, O_, generator=torch.Generator().manual_seed(N)).to(dtype)
+    w, b = torch.zeros(O_, 8, dtype=dtype, device="cuda"), torch.zeros(O_, dtype=dtype, device="cuda", requires_grad=True)
+    (db,) = torch.autograd.grad(checkpointed_linear(x, w, b), b, dy.cuda())
+    O.assert_close(db, dy.double().sum(0), (N + 1) * O.U * dy.double().abs().sum(0), "db")
+
+
+def test_no_tokens():
+    w, b = torch.zeros(3, 40, device="cuda", requires_grad=True), torch.zeros(3, device="cuda", requires_grad=True)
+    y = checkpointed_linear(torch.zeros(0, 40, device="cuda"), w, b)
+    assert y.shape == (0, 3)
+    y.sum().backward()
+    assert (w.grad == 0).all() and (b.grad == 0).all()

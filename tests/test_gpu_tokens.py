@@ -380,3 +380,60 @@ def test_a_token_policy_through_vtrace():
     # n products in 32 bits: n roundings of sums that stay below the sum of magnitudes, two more for -adv / n
     O.assert_close(head.weight.grad, dz.T @ kept, dz_tol.T @ kept.abs() + (n + 3) * O.U * (dz.abs().T @ kept.abs()), "weight gradient")
     O.assert_close(head.bias.grad, dz.sum(0), dz_tol.sum(0) + (n + 3) * O.U * dz.abs().sum(0), "bias gradient")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [0, 5])
+@pytest.mark.parametrize("kind", KINDS)
+def test_without_the_host_module(kind, T, dtype, monkeypatch):
+    """The python route (a tree without lib/_trl_host.so) makes the same calls: the same bits."""
+    c = make(kind, dtype, 3, T, 1203, L=40, seed=21)
+    kw, z, action = kwargs(c), gpu(c, c["z"]), gpu(c, c["action"])
+
+    def everything():
+        leaf = z.clone().requires_grad_()
+        out = process_logits(leaf, **kw)
+        lp, H = token_log_prob(leaf, action, entropy=True, **kw)
+        lp_only = token_log_prob(z, action, **kw)
+        return (out.detach(), lp.detach(), H.detach(), lp_only, torch.autograd.grad(out, leaf, gpu(c, c["g_out"]))[0],
+                torch.autograd.grad((lp, H), leaf, tuple(gpu(c, g) for g in c["g"]))[0])
+
+    assert F.host_fast_path()
+    fast = everything()
+    monkeypatch.setattr(F, "_HOST", None)
+    check(c)
+    for a, b in zip(fast, everything()):
+        assert same(a, b)
+
+
+@pytest.mark.parametrize("route", ["host module", "python"])
+def test_autograd_manners(route, monkeypatch):
+    if route == "python":
+        monkeypatch.setattr(F, "_HOST", None)
+    c = make("all", torch.float32, 2, 3, 90, L=9, seed=22)
+    kw, action = kwargs(c), c["action"].cuda()
+    leaf = c["z"].cuda().requires_grad_()
+    lp, H = token_log_prob(leaf, action, entropy=True, **kw)
+    (first,) = torch.autograd.grad(lp.nan_to_num(0, 0, 0).sum(), leaf, retain_graph=True)
+    (again,) = torch.autograd.grad(lp.nan_to_num(0, 0, 0).sum(), leaf)
+    assert torch.equal(first, again)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(H.sum(), leaf)
+    lp = token_log_prob(leaf, action, **kw)
+    w = torch.ones_like(lp).requires_grad_()
+    (d,) = torch.autograd.grad((lp * w).nan_to_num(0, 0, 0).sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        d.sum().backward()
+    packed = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: packed.append(t) or t.cpu(), lambda t: t.cuda()):
+        lp = token_log_prob(leaf, action, **kw)
+    (offloaded,) = torch.autograd.grad(lp.nan_to_num(0, 0, 0).sum(), leaf)
+    assert packed and torch.equal(offloaded, first)
+    with torch.no_grad():
+        assert not token_log_prob(leaf, action, **kw).requires_grad
+    assert not process_logits(leaf.detach(), **kw).requires_grad
+    out = process_logits(leaf, mask=kw["mask"])  # the logits are not needed for this gradient
+    with torch.no_grad():
+        leaf.add_(1.0)
+    out.sum().backward()
+    assert torch.equal(leaf.grad != 0, kw["mask"])

@@ -277,11 +277,49 @@ __global__ __launch_bounds__(256) void act_join_kernel(const float *parts, int s
     (w ? dw : db)[at] = (T)s;
 }
 
+// Column sums of dy alone: 32 groups of 8 columns a block, 8 rows at a time.
+template <typename T>
+__global__ __launch_bounds__(256) void act_column_sum_kernel(WeightGradArgs a) {
+    __shared__ float sums[8][256];
+    const i64 o0 = (i64)(blockIdx.x % a.tiles) * 256;
+    const int split = blockIdx.x / a.tiles, col = threadIdx.x % 32 * kVec, row = threadIdx.x / 32;
+    const i64 left = a.O - (o0 + col), n0 = split * a.part, n1 = n0 + a.part < a.N ? n0 + a.part : a.N;
+    const int n_col = left >= kVec ? kVec : left < 0 ? 0 : (int)left;
+    float s[kVec] = {};
+    if (n_col > 0) {
+        for (i64 n = n0 + row; n < n1; n += 8) {
+            Raw8<T> r{};
+            load8((const T *)a.dy + n * a.dy_stride + o0 + col, n_col, r);
+            float v[kVec];
+            unpack8(r, v);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) s[i] += v[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) sums[row][col + i] = s[i];
+    __syncthreads();
+    const i64 o = o0 + threadIdx.x;
+    if (o >= a.O) return;
+    float t = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t += sums[k][threadIdx.x];
+    if (a.splits == 1) ((T *)a.db)[o] = (T)t;
+    else a.parts[(i64)split * a.O + o] = t;
+}
+
 // Tile and splits by the sizes: 32 rows for layers with few outputs, whose codes are all the traffic; 256 x 256 where that fills the
 // chip; else 128 x 128.  Tokens are split until there are about two blocks a compute unit, in parts of at least 256 tokens.
 struct WeightGradPlan { int bm, bn, bk; i64 tiles_d, tiles, part; int splits; };
 WeightGradPlan weight_grad_plan(int dtype, i64 N, i64 O, i64 D) {
     WeightGradPlan p{};
+    if (D == 0) {  // column sums alone
+        p.tiles = (O + 255) / 256;
+        const i64 want = (512 + p.tiles - 1) / p.tiles, most = (N + 127) / 128 > 0 ? (N + 127) / 128 : 1;
+        p.part = N / (want < most ? want : most) + 1;
+        p.splits = (int)(N ? (N + p.part - 1) / p.part : 1);
+        return p;
+    }
     auto tiles = [&](int bm, int bn) { return ((O + bm - 1) / bm) * ((D + bn - 1) / bn); };
     p.bk = dtype == TRL_BF16 ? 64 : 32;
     if (O <= 32) { p.bm = 32; p.bn = 128; p.bk = 64; }
@@ -307,7 +345,8 @@ void launch_weight_grad(hipStream_t s, const WeightGradArgs &a) {
 }
 template <typename T>
 void launch_weight_grad_t(hipStream_t s, const WeightGradArgs &a, const WeightGradPlan &p) {
-    if (p.bm == 32) launch_weight_grad<T, 32, 128, 64, 1, 4>(s, a);
+    if (a.D == 0) hipLaunchKernelGGL(act_column_sum_kernel<T>, dim3((unsigned)(a.tiles * a.splits)), dim3(256), 0, s, a);
+    else if (p.bm == 32) launch_weight_grad<T, 32, 128, 64, 1, 4>(s, a);
     else if constexpr (sizeof(T) == 4) launch_weight_grad<T, 128, 128, 32, 2, 2>(s, a);
     else {
         constexpr int BK = kTerms<T> == 1 ? 64 : 32;
@@ -340,7 +379,7 @@ void launch_act_dequantize(hipStream_t s, int dtype, const int8_t *codes, const 
 
 size_t act_weight_grad_workspace(int dtype, i64 N, i64 O, i64 D) {
     const WeightGradPlan p = weight_grad_plan(dtype, N, O, D);
-    return p.splits > 1 ? (size_t)p.splits * (size_t)O * (size_t)(D + 1) * sizeof(float) : 0;
+    return p.splits > 1 ? (size_t)p.splits * (size_t)O * (size_t)(D + 1) * sizeof(float) : 0;  // parts of dw, then of db
 }
 
 int launch_act_weight_grad(hipStream_t s, int dtype, const void *dy, i64 dy_stride, const int8_t *codes, const u8 *exponents, i64 N, i64 O,

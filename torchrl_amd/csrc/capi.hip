@@ -911,15 +911,16 @@ int trl_act_dequantize(void *stream, int dtype, const int8_t *codes, const uint8
 }
 
 size_t trl_act_weight_grad_workspace_bytes(int dtype, int64_t N, int64_t O, int64_t D) {
-    if (!low_dtype_ok(dtype) || N <= 0 || O <= 0 || D <= 0) return 0;
+    if (!low_dtype_ok(dtype) || N <= 0 || O <= 0 || D < 0) return 0;
     return act_weight_grad_workspace(dtype, N, O, D);
 }
 
 int trl_act_weight_grad(void *stream, int dtype, const void *dy, int64_t dy_stride, const int8_t *codes, const uint8_t *exponents,
                         int64_t N, int64_t O, int64_t D, void *dw, void *db, void *workspace, size_t workspace_bytes) {
-    if (int rc = check_act_dims("trl_act_weight_grad", dtype, N, D)) return rc;
-    if (O <= 0 || O > 0x7fffffffLL || !dw) return fail(TRL_ERR_INVALID_ARGUMENT, "trl_act_weight_grad: O <= 0 or null pointer");
-    if (N > 0 && (!dy || !codes || !exponents || ((uintptr_t)codes & 15)))
+    if (int rc = check_act_dims("trl_act_weight_grad", dtype, N, D > 0 ? D : 1)) return rc;
+    if (O <= 0 || O > 0x7fffffffLL || D < 0 || (D > 0) != (dw != nullptr) || (!dw && !db))
+        return fail(TRL_ERR_INVALID_ARGUMENT, "trl_act_weight_grad: O <= 0 or null pointer");
+    if (N > 0 && (!dy || (dw && (!codes || !exponents || ((uintptr_t)codes & 15)))))
         return fail(TRL_ERR_INVALID_ARGUMENT, "trl_act_weight_grad: null pointer, or codes not 16-byte aligned");
     const size_t need = trl_act_weight_grad_workspace_bytes(dtype, N, O, D);
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
@@ -927,7 +928,7 @@ int trl_act_weight_grad(void *stream, int dtype, const void *dy, int64_t dy_stri
     if (launch_act_weight_grad((hipStream_t)stream, dtype, dy, dy_stride, codes, exponents, N, O, D, dw, db, workspace))
         return fail(TRL_ERR_UNSUPPORTED, "trl_act_weight_grad: too large for one launch");
     if (int rc = check_launch("trl_act_weight_grad")) return rc;
-    g_kernel = "act_weight_grad";
+    g_kernel = dw ? "act_weight_grad" : "act_column_sum";
     return TRL_OK;
 }
 

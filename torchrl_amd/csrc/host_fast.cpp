@@ -25,6 +25,7 @@
 #include <vector>
 
 #include "../../include/trl_value.h"
+#include "host_policy.h"
 
 namespace {
 
@@ -733,4 +734,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_trl_host", "host-side fast path o
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__trl_host(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__trl_host(void) {
+    PyObject *m = PyModule_Create(&module);
+    if (m && PyModule_AddFunctions(m, trl_policy_methods) < 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

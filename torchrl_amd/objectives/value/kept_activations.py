@@ -46,12 +46,23 @@ def _rows(x: Tensor) -> Tensor:
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
+def _ptr(x: Optional[Tensor]):
+    return None if x is None else x.data_ptr()
+
+
 def _call(name, device, *args):
     lib = _extension.get_lib()
     with F._on(device):
         rc = getattr(lib, name)(F._stream(device), *args)
     if rc:
         _extension.check(rc, lib)
+
+
+def _done(got):
+    """What the host module returns: the result, or the status of a native call that failed."""
+    if got.__class__ is int:
+        _extension.check(got, _extension.get_lib())
+    return got
 
 
 @dataclass
@@ -69,6 +80,11 @@ class QuantizedActivation:
         dtype = self.dtype if dtype is None else dtype
         if dtype not in _DT:
             raise NotImplementedError(f"torchrl_amd 8-bit activations support float32, bfloat16 and float16, got {dtype}")
+        host = F._HOST if F._HOST_TRIED else F._host_module()
+        if host is not None and len(self.shape):
+            out = host.dequantize(self.codes, self.exponents, self.shape[-1], _DT[dtype])
+            if out is not None:
+                return _done(out)
         out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
         if out.numel():
             D = self.shape[-1]
@@ -79,6 +95,11 @@ class QuantizedActivation:
 def quantize_activation(x: Tensor) -> QuantizedActivation:
     """Keeps ``x`` ``[*B, D]`` (float32, bfloat16 or float16) in 8 bits: blocks of 32 features share a power of two, 2^-6 of the one at or below
     the block's largest magnitude; codes are rounded to nearest even and held to 127.  Blocks with a NaN or an infinity stand for NaN."""
+    host = F._HOST if F._HOST_TRIED else F._host_module()
+    if host is not None:
+        got = host.quantize(x)
+        if got is not None:
+            return QuantizedActivation(*_done(got), x.shape, x.dtype)
     _check(x, "x")
     if x.ndim < 1 or x.shape[-1] == 0:
         raise RuntimeError(f"quantize_activation needs a feature dim, got shape {tuple(x.shape)}")
@@ -93,17 +114,16 @@ def quantize_activation(x: Tensor) -> QuantizedActivation:
     return QuantizedActivation(codes, exponents, x.shape, x.dtype)
 
 
-def _weight_grad(dy: Tensor, codes: Tensor, exponents: Tensor, D: int, want_db: bool):
-    """(dy^T x^, column sums of dy or None) of (N, O) gradients and a kept (N, D) activation."""
+def _weight_grad(dy: Tensor, codes: Optional[Tensor], exponents: Optional[Tensor], D: int, want_db: bool):
+    """(dy^T x^, column sums of dy or None) of (N, O) gradients and a kept (N, D) activation; without one (D == 0) the sums alone."""
     dy = dy if dy.stride(1) == 1 or dy.shape[1] == 1 else dy.contiguous()
     N, O = dy.shape
     dt = _DT[dy.dtype]
-    dw = torch.empty(O, D, dtype=dy.dtype, device=dy.device)
+    dw = torch.empty(O, D, dtype=dy.dtype, device=dy.device) if D else None
     db = torch.empty(O, dtype=dy.dtype, device=dy.device) if want_db else None
     need = _extension.get_lib().trl_act_weight_grad_workspace_bytes(dt, N, O, D)
     ws = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
-    _call("trl_act_weight_grad", dy.device, dt, dy.data_ptr(), dy.stride(0), codes.data_ptr(), exponents.data_ptr(), N, O, D, dw.data_ptr(),
-          None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), need)
+    _call("trl_act_weight_grad", dy.device, dt, dy.data_ptr(), dy.stride(0), _ptr(codes), _ptr(exponents), N, O, D, _ptr(dw), _ptr(db), _ptr(ws), need)
     return dw, db
 
 
@@ -128,7 +148,7 @@ class _CheckpointedLinear(torch.autograd.Function):
         if need_w:
             dw, db = _weight_grad(dy, codes, exponents, ctx.features, need_b)
         elif need_b:
-            db = dy.sum(0)
+            _, db = _weight_grad(dy, None, None, 0, True)
         return dx, dw, db
 
 
@@ -137,6 +157,12 @@ def checkpointed_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None
 
     ``x`` ``[*B, D]``, ``weight`` ``[O, D]`` and ``bias`` ``[O]`` share one dtype (float32, bfloat16 or float16) and device; under autocast they
     are cast to its dtype.  Without a gradient to ``weight`` nothing is kept."""
+    if not torch.is_autocast_enabled("cuda"):
+        host = F._HOST if F._HOST_TRIED else F._host_module()
+        if host is not None:  # checks, launches and the autograd node in one C++ hop (csrc/host_policy.cpp)
+            got = host.checkpointed_linear(x, weight, bias)
+            if got is not None:
+                return _done(got)
     for t, name in ((x, "x"), (weight, "weight"), (bias, "bias")):
         if t is not None or name != "bias":
             _check(t, name)

@@ -190,6 +190,13 @@ def _call(name, device, args, *more):
         _extension.check(rc, lib)
 
 
+def _done(got):
+    """What the host module returns: the result, or the status of a native call that failed."""
+    if got.__class__ is int:
+        _extension.check(got, _extension.get_lib())
+    return got
+
+
 def _save(ctx, p: _Processing, *more, logits: bool = True):
     """Keeps a call's tensors with autograd, which notices when one is written in place before the backward pass."""
     saved = [getattr(p, k) for k in _TENSORS]
@@ -268,6 +275,12 @@ def process_logits(logits: Tensor, *, tokens: Optional[Tensor] = None, lengths: 
         from torchrl_amd.objectives.value import _ops
         return _ops.process_logits(logits, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty, bias, mask,
                                    temperature)
+    host = F._HOST if F._HOST_TRIED else F._host_module()
+    if host is not None and out is None:  # the plain layouts in one C++ hop (csrc/host_policy.cpp)
+        got = host.process_logits(logits, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty, bias, mask,
+                                  temperature)
+        if got is not None:
+            return _done(got)
     p = _processing(logits, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty, bias, mask, temperature)
     if F._needs_grad(logits):
         _need(out is None, RuntimeError, "process_logits(out=...) does not support automatic differentiation")
@@ -362,6 +375,12 @@ def token_log_prob(logits: Tensor, action: Tensor, *, entropy: bool = False, tok
         from torchrl_amd.objectives.value import _ops
         return _ops.token_log_prob(logits, action, entropy, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty,
                                    bias, mask, temperature)
+    host = F._HOST if F._HOST_TRIED else F._host_module()
+    if host is not None:  # the plain layouts in one C++ hop (csrc/host_policy.cpp)
+        got = host.token_log_prob(logits, action, bool(entropy), tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty,
+                                  frequency_penalty, bias, mask, temperature)
+        if got is not None:
+            return _done(got)
     _need(isinstance(logits, Tensor), TypeError, "logits must be a tensor")
     lead = logits.shape[:-1]
     act = _int_tensor(action, lead, "action", logits.device)
