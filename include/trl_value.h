@@ -549,7 +549,8 @@ int trl_token_log_prob_bwd(void *stream, const trl_token_args *args);
 int trl_act_quantize(void *stream, int dtype, const void *x, int64_t x_stride, int64_t N, int64_t D, int8_t *codes, uint8_t *exponents);
 int trl_act_dequantize(void *stream, int dtype, const int8_t *codes, const uint8_t *exponents, int64_t N, int64_t D, void *out);
 /* The weight gradient of a linear layer whose input was kept that way: dw (O, D) = dy (N, O)^T x^, and db (O) = column sums of dy
- * (or NULL; with dw NULL and D 0 the column sums alone).  dy has row stride dy_stride (elements) and type dtype, as dw and db.  Sums in 32 bits, in a fixed order.
+ * (or NULL; with dw NULL and D 0 the column sums alone).  dy has row stride dy_stride (elements) and type dtype, as dw and db and as
+ * the activation that was kept.  Sums in 32 bits, in a fixed order.
  * workspace: trl_act_weight_grad_workspace_bytes(), 16-byte aligned, free again when the call's launches have run. */
 size_t trl_act_weight_grad_workspace_bytes(int dtype, int64_t N, int64_t O, int64_t D);
 int trl_act_weight_grad(void *stream, int dtype, const void *dy, int64_t dy_stride, const int8_t *codes, const uint8_t *exponents,

@@ -68,32 +68,34 @@ __global__ __launch_bounds__(256) void act_dequantize_kernel(const int8_t *codes
 }
 
 // ---- dw = dy^T x^ ------------------------------------------------------------------------------------------------------------------
-// A (N, O) and a (N, D) matrix, both with the summed dimension outermost, on 32 x 32 x 16 bf16 matrix instructions.
-//   exact   A code times its step has 7 bits, so x^ is exact in bf16.  dy is split into bf16 terms that add up to it exactly: one for
-//           bf16, two for fp16 (8 + 3 bits), three for fp32 (8 + 8 + 8).  Every product is then exact in the 32-bit accumulators, and
-//           the result is off by the sum's own roundings and one to the output type.
+// A (N, O) and a (N, D) matrix, both with the summed dimension outermost, on 32 x 32 x 16 matrix instructions.
+//   exact   A code times its step has 7 bits, so x^ is exact in bf16, and in fp16 where it was made from fp16.  dy is used as it is in
+//           these types; an fp32 dy is split into three bf16 terms (8 + 8 + 8 bits) that add up to it exactly.  Every product is then
+//           exact in the 32-bit accumulators, and the result is off by the sum's own roundings and one to the output type.
 //   tiles   The codes go from registers through the conversion into LDS, rows of tokens as in memory; ds_read_tr16 turns 4 x 16 pieces so
 //           that a lane gets four consecutive tokens of its own column.  Rows are filled up by 16 elements, so that the four rows of a
-//           piece lie in different banks.  Two LDS buffers; the next tile's loads are in flight while one is multiplied.
+//           piece lie in different banks.
+//   flow    Two LDS buffers.  While one is multiplied, the next tile goes from registers to the other in the second half of the step, and
+//           each register is loaded with the tile after that as soon as it is free: a load has a whole step to arrive, and the
+//           conversion runs in the shadow of the matrix instructions.
 //   splits  Few output tiles (value heads) split the tokens; the parts are 32 bits and are added in order by a second launch.
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 
 template <typename T> constexpr int kTerms = sizeof(T) == 4 ? 3 : 1;
-template <> constexpr int kTerms<_Float16> = 2;
 
 __device__ __forceinline__ u32 high_halves(u32 lo, u32 hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
 
-// the bf16 terms of 8 values: term j of element i in w[j]
-template <int NT>
+// the bf16 terms of 8 values: term j of elements 2 i and 2 i + 1 in w[j][i]
 __device__ __forceinline__ void split8(const float *v, u32x4 *w) {
     float r[kVec];
 #pragma unroll
     for (int i = 0; i < kVec; ++i) r[i] = v[i];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
+    for (int j = 0; j < 3; ++j) {
         u32 top[kVec];
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
@@ -106,6 +108,45 @@ __device__ __forceinline__ void split8(const float *v, u32x4 *w) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[j][i] = high_halves(top[2 * i], top[2 * i + 1]);
     }
+}
+
+// two exact values as 16 bits each
+template <typename T>
+__device__ __forceinline__ u32 pack_exact(float lo, float hi) {
+    if constexpr (__is_same(T, _Float16)) return __builtin_bit_cast(u32, __builtin_amdgcn_cvt_pkrtz(lo, hi));
+    else return high_halves(__builtin_bit_cast(u32, lo), __builtin_bit_cast(u32, hi));
+}
+
+// 16 codes times their step.  A code with 128 added is an unsigned byte, which one instruction turns into a float; one fma takes the 128
+// steps off again and scales, exactly.  (From step 2^121 on 128 steps are no number: those, and NaN blocks, subtract first.)
+template <typename T>
+__device__ __forceinline__ void convert16(u32x4 codes, int e, u32x4 *w) {
+    const float step = step_of(e), bias = -128.0f * step;
+    const bool far = __any(e >= 248);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const u32 c = codes[i] ^ 0x80808080u;
+        float v[4] = {(float)(c & 0xffu), (float)(c >> 8 & 0xffu), (float)(c >> 16 & 0xffu), (float)(c >> 24)};
+        if (far) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = (v[k] - 128.0f) * step;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = fmaf(v[k], step, bias);
+        }
+        w[i / 2][2 * (i % 2)] = pack_exact<T>(v[0], v[1]);
+        w[i / 2][2 * (i % 2) + 1] = pack_exact<T>(v[2], v[3]);
+    }
+}
+
+template <bool B>
+struct Flag { static constexpr bool value = B; };
+
+// orders LDS alone: loads from memory stay in flight
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 struct WeightGradArgs {
@@ -122,11 +163,12 @@ struct WeightGradArgs {
 };
 
 template <typename T, int BM, int BN, int BK, int WM, int WN>
-__global__ __launch_bounds__(WM *WN *kWave) void act_weight_grad_kernel(WeightGradArgs a) {
+__global__ __launch_bounds__(WM *WN *kWave, BM == 256 ? 2 : 1) void act_weight_grad_kernel(WeightGradArgs a) {
     constexpr int NT = kTerms<T>, NTHR = WM * WN * kWave;
     constexpr int SA = BM + 16, SB = BN + 16;              // LDS row strides
     constexpr int MI = BM / WM / 32, NI = BN / WN / 32;    // a wave's 32 x 32 pieces
     constexpr int VA = BK * BM / kVec / NTHR, VB = BK * BN / 16 / NTHR;
+    constexpr int RA = NTHR / (BM / kVec), RB = NTHR / (BN / 16);  // rows between a thread's vectors
     static_assert(VA * kVec * NTHR == BK * BM && VB * 16 * NTHR == BK * BN && NTHR % (BM / kVec) == 0 && NTHR % (BN / 16) == 0, "whole vectors");
     constexpr int kBuf = BK * (NT * SA + SB);              // elements of a buffer
     extern __shared__ __align__(16) short lds[];
@@ -144,55 +186,77 @@ __global__ __launch_bounds__(WM *WN *kWave) void act_weight_grad_kernel(WeightGr
     const i64 a_left = a.O - (o0 + a_col);
     const int a_n = a_left >= kVec ? kVec : a_left < 0 ? 0 : (int)a_left;
     const bool b_in = d0 + b_col < a.Dp;
+    // whole tiles: a scalar base and a 32-bit offset a vector
+    const bool whole = o0 + BM <= a.O && d0 + BN <= a.Dp && a.dy_stride >= 0 && a.dy_stride < (1LL << 24) && a.Dp < (1LL << 24);
+    const u32 a_off = (u32)(a_row * a.dy_stride + a_col) * sizeof(T), a_step = (u32)(RA * a.dy_stride) * sizeof(T);
+    const u32 b_off = (u32)(b_row * a.Dp + b_col), b_step = (u32)(RB * a.Dp);
     Raw8<T> ra[VA];
     u32x4 rb[VB];
     int re[VB];
-    auto load = [&](i64 n) {
+    auto load_a_whole = [&](i64 n) {
+        const char *base = (const char *)a.dy + (n * a.dy_stride + o0) * (i64)sizeof(T);
 #pragma unroll
-        for (int q = 0; q < VA; ++q) {
-            const i64 row = n + a_row + q * (NTHR / (BM / kVec));
-            ra[q] = Raw8<T>{};
-            if (row < n1 && a_n > 0) load8((const T *)a.dy + row * a.dy_stride + o0 + a_col, a_n, ra[q]);
-        }
+        for (int q = 0; q < VA; ++q) load8((const T *)(base + (a_off + q * a_step)), kVec, ra[q]);
+    };
+    auto load_b_whole = [&](i64 n) {
+        const int8_t *base = a.codes + n * a.Dp + d0;
+        const u8 *exps = a.exponents + (n * a.Dp + d0) / kActBlock;
 #pragma unroll
         for (int q = 0; q < VB; ++q) {
-            const i64 row = n + b_row + q * (NTHR / (BN / 16));
-            rb[q] = u32x4{0, 0, 0, 0};
-            re[q] = 127;
-            if (row < n1 && b_in) {
-                rb[q] = *(const u32x4 *)(a.codes + row * a.Dp + d0 + b_col);
-                re[q] = a.exponents[(row * a.Dp + d0 + b_col) / kActBlock];
+            rb[q] = *(const u32x4 *)(base + (b_off + q * b_step));
+            re[q] = exps[(b_off + q * b_step) / kActBlock];
+        }
+    };
+    auto load_a = [&](i64 n) {
+        if (whole && n + BK <= n1) load_a_whole(n);
+        else {
+#pragma unroll
+            for (int q = 0; q < VA; ++q) {
+                const i64 row = n + a_row + q * RA;
+                ra[q] = Raw8<T>{};
+                if (row < n1 && a_n > 0) load8((const T *)a.dy + row * a.dy_stride + o0 + a_col, a_n, ra[q]);
+            }
+        }
+    };
+    auto load_b = [&](i64 n) {
+        if (whole && n + BK <= n1) load_b_whole(n);
+        else {
+#pragma unroll
+            for (int q = 0; q < VB; ++q) {
+                const i64 row = n + b_row + q * RB;
+                rb[q] = u32x4{0, 0, 0, 0};
+                re[q] = 127;
+                if (row < n1 && b_in) {
+                    rb[q] = *(const u32x4 *)(a.codes + row * a.Dp + d0 + b_col);
+                    re[q] = a.exponents[(row * a.Dp + d0 + b_col) / kActBlock];
+                }
             }
         }
     };
     float col_sum[kVec] = {};
-    auto store = [&](short *buf) {
+    auto store_a = [&](short *buf, bool sum) {
 #pragma unroll
         for (int q = 0; q < VA; ++q) {
             u32x4 w[NT];
             float v[kVec];
-            if (NT > 1 || want_db) unpack8(ra[q], v);
-            if (want_db) {
+            if (NT > 1 || sum) unpack8(ra[q], v);
+            if (sum) {
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) col_sum[i] += v[i];
             }
-            if constexpr (NT > 1) split8<NT>(v, w);
+            if constexpr (NT > 1) split8(v, w);
             else w[0] = ra[q].a;
-            short *to = buf + (a_row + q * (NTHR / (BM / kVec))) * (NT * SA) + a_col;
+            short *to = buf + (a_row + q * RA) * (NT * SA) + a_col;
 #pragma unroll
             for (int j = 0; j < NT; ++j) *(u32x4 *)(to + j * SA) = w[j];
         }
+    };
+    auto store_b = [&](short *buf) {
 #pragma unroll
         for (int q = 0; q < VB; ++q) {
-            const float step = step_of(re[q]);
             u32x4 w[2];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const u32 c = rb[q][i / 2];
-                const float lo = (float)(int8_t)(c >> (16 * (i & 1))) * step, hi = (float)(int8_t)(c >> (16 * (i & 1) + 8)) * step;
-                w[i / 4][i % 4] = high_halves(__builtin_bit_cast(u32, lo), __builtin_bit_cast(u32, hi));
-            }
-            short *to = buf + BK * NT * SA + (b_row + q * (NTHR / (BN / 16))) * SB + b_col;
+            convert16<T>(rb[q], re[q], w);
+            short *to = buf + BK * NT * SA + (b_row + q * RB) * SB + b_col;
             *(u32x4 *)to = w[0];
             *(u32x4 *)(to + 8) = w[1];
         }
@@ -204,33 +268,100 @@ __global__ __launch_bounds__(WM *WN *kWave) void act_weight_grad_kernel(WeightGr
     auto fragment = [&](const short *row0, int stride) {
         const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(row0 + fk * stride + fc));
         const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(row0 + (fk + 4) * stride + fc));
-        return __builtin_bit_cast(v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     };
     if (n0 < n1) {
-        load(n0);
-        store(lds);
+        load_a(n0);
+        load_b(n0);
+        store_a(lds, want_db);
+        store_b(lds);
+        if (n0 + BK < n1) {
+            load_a(n0 + BK);
+            load_b(n0 + BK);
+        }
     }
     __syncthreads();
     int cur = 0;
-    for (i64 n = n0; n < n1; n += BK, cur ^= 1) {
-        const bool more = n + BK < n1;
-        if (more) load(n + BK);
+    i64 n = n0;
+    auto multiply = [&](auto fa, auto fb, v16f &c) {
+        if constexpr (__is_same(T, _Float16))
+            c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, fa), __builtin_bit_cast(v8h, fb), c, 0, 0, 0);
+        else
+            c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, fa), __builtin_bit_cast(v8bf, fb), c, 0, 0, 0);
+    };
+    // The long middle of a whole tile, one straight line a step: fragments are fetched one ahead, those of the next step before the step
+    // ends.  Two barriers: before the last quarter (the next buffer is written), and before that buffer's successor is written over
+    // (every wave is through with the last quarter's reads).
+    if constexpr (BK == 64 && NT == 1 && MI % 2 == 0) {
+        typedef decltype(fragment(lds, SA)) Frag;
+        Frag fa[2], fb[2][NI];
+        auto fetch_a = [&](const short *buf, int k, int i) { fa[i % 2] = fragment(buf + k * SA + (wm * MI + i % MI) * 32, SA); };
+        auto fetch_b = [&](const short *buf, int k, int to) {
+#pragma unroll
+            for (int j = 0; j < NI; ++j) fb[to][j] = fragment(buf + BK * SA + k * SB + (wn * NI + j) * 32, SB);
+        };
+        // 16 tokens at k; the fragments after these come from k2 of buf2
+        auto quarter = [&](const short *buf, int k, const short *buf2, int k2, int from) {
+            fetch_b(buf2, k2, from ^ 1);
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                if (i + 1 < MI) fetch_a(buf, k, i + 1);
+                else fetch_a(buf2, k2, MI);
+#pragma unroll
+                for (int j = 0; j < NI; ++j) multiply(fa[i % 2], fb[from][j], acc[i][j]);
+            }
+        };
+        static_assert(MI % 2 == 0 || MI == 1, "the ring of two fragments");
+        auto middle = [&](auto sum) {
+            fetch_b(lds, 0, 0);
+            fetch_a(lds, 0, 0);
+            for (; n + 3 * BK <= n1; n += BK, cur ^= 1) {
+                const short *buf = lds + cur * kBuf;
+                short *next = lds + (cur ^ 1) * kBuf;
+                quarter(buf, 0, buf, 16, 0);
+                lds_barrier();
+                store_a(next, sum.value);
+                load_a_whole(n + 2 * BK);
+                quarter(buf, 16, buf, 32, 1);
+                store_b(next);
+                load_b_whole(n + 2 * BK);
+                quarter(buf, 32, buf, 48, 0);
+                lds_barrier();
+                quarter(buf, 48, next, 0, 1);
+            }
+        };
+        if (whole && n + 3 * BK <= n1) {
+            if (want_db) middle(Flag<true>());
+            else middle(Flag<false>());
+            __syncthreads();
+        }
+    }
+    for (; n < n1; n += BK, cur ^= 1) {
+        const bool more = n + BK < n1, after = n + 2 * BK < n1;
         const short *la = lds + cur * kBuf, *lb = la + BK * NT * SA;
+        short *next = lds + (cur ^ 1) * kBuf;
 #pragma unroll
         for (int k = 0; k < BK; k += 16) {
-            v8bf fb[NI];
+            decltype(fragment(lb, SB)) fb[NI];
 #pragma unroll
             for (int j = 0; j < NI; ++j) fb[j] = fragment(lb + k * SB + (wn * NI + j) * 32, SB);
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const v8bf fa = fragment(la + k * (NT * SA) + t * SA + (wm * MI + i) * 32, NT * SA);
+                    const auto fa = fragment(la + k * (NT * SA) + t * SA + (wm * MI + i) * 32, NT * SA);
 #pragma unroll
-                    for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa, fb[j], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < NI; ++j) multiply(fa, fb[j], acc[i][j]);
                 }
+            if (k == BK - 32 && more) {
+                store_a(next, want_db);
+                if (after) load_a(n + 2 * BK);
+            }
+            if (k == BK - 16 && more) {
+                store_b(next);
+                if (after) load_b(n + 2 * BK);
+            }
         }
-        if (more) store(lds + (cur ^ 1) * kBuf);
         __syncthreads();
     }
 
@@ -256,7 +387,7 @@ __global__ __launch_bounds__(WM *WN *kWave) void act_weight_grad_kernel(WeightGr
         __syncthreads();
         for (int c = tid; c < BM; c += NTHR) {
             float s = 0.0f;
-            for (int r = 0; r < NTHR / (BM / kVec); ++r) s += sums[r * BM + c];
+            for (int r = 0; r < RA; ++r) s += sums[r * BM + c];
             if (o0 + c < a.O) {
                 if (a.splits == 1) ((T *)a.db)[o0 + c] = (T)s;
                 else a.parts[(i64)a.splits * a.O * a.D + (i64)split * a.O + o0 + c] = s;
@@ -321,7 +452,7 @@ WeightGradPlan weight_grad_plan(int dtype, i64 N, i64 O, i64 D) {
         return p;
     }
     auto tiles = [&](int bm, int bn) { return ((O + bm - 1) / bm) * ((D + bn - 1) / bn); };
-    p.bk = dtype == TRL_BF16 ? 64 : 32;
+    p.bk = dtype == TRL_F32 ? 32 : 64;
     if (O <= 32) { p.bm = 32; p.bn = 128; p.bk = 64; }
     else if (dtype != TRL_F32 && tiles(256, 256) >= 192) { p.bm = 256; p.bn = 256; }
     else { p.bm = 128; p.bn = 128; }
@@ -349,9 +480,8 @@ void launch_weight_grad_t(hipStream_t s, const WeightGradArgs &a, const WeightGr
     else if (p.bm == 32) launch_weight_grad<T, 32, 128, 64, 1, 4>(s, a);
     else if constexpr (sizeof(T) == 4) launch_weight_grad<T, 128, 128, 32, 2, 2>(s, a);
     else {
-        constexpr int BK = kTerms<T> == 1 ? 64 : 32;
-        if (p.bm == 256) launch_weight_grad<T, 256, 256, BK, 2, 4>(s, a);
-        else launch_weight_grad<T, 128, 128, BK, 2, 2>(s, a);
+        if (p.bm == 256) launch_weight_grad<T, 256, 256, 64, 2, 4>(s, a);
+        else launch_weight_grad<T, 128, 128, 64, 2, 2>(s, a);
     }
     if (a.splits > 1) {
         const i64 n_w = a.O * a.D, n_b = a.db ? a.O : 0;
