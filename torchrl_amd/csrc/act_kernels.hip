@@ -117,23 +117,16 @@ __device__ __forceinline__ u32 pack_exact(float lo, float hi) {
     else return high_halves(__builtin_bit_cast(u32, lo), __builtin_bit_cast(u32, hi));
 }
 
-// 16 codes times their step.  A code with 128 added is an unsigned byte, which one instruction turns into a float; one fma takes the 128
-// steps off again and scales, exactly.  (From step 2^121 on 128 steps are no number: those, and NaN blocks, subtract first.)
+// 16 codes times their step, exactly
 template <typename T>
 __device__ __forceinline__ void convert16(u32x4 codes, int e, u32x4 *w) {
-    const float step = step_of(e), bias = -128.0f * step;
-    const bool far = __any(e >= 248);
+    const float step = step_of(e);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const u32 c = codes[i] ^ 0x80808080u;
-        float v[4] = {(float)(c & 0xffu), (float)(c >> 8 & 0xffu), (float)(c >> 16 & 0xffu), (float)(c >> 24)};
-        if (far) {
+        const u32 c = codes[i];
+        float v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = (v[k] - 128.0f) * step;
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = fmaf(v[k], step, bias);
-        }
+        for (int k = 0; k < 4; ++k) v[k] = (float)(int8_t)(c >> (8 * k)) * step;
         w[i / 2][2 * (i % 2)] = pack_exact<T>(v[0], v[1]);
         w[i / 2][2 * (i % 2) + 1] = pack_exact<T>(v[2], v[3]);
     }
