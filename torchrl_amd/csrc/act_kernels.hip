@@ -397,6 +397,7 @@ __global__ __launch_bounds__(256) void act_join_kernel(const float *parts, int s
     const i64 n = w ? n_w : n_b, at = w ? i : i - n_w;
     const float *p = parts + (w ? 0 : splits * n_w) + at;
     float s = 0.0f;
+#pragma unroll 8
     for (int k = 0; k < splits; ++k) s += p[k * n];
     (w ? dw : db)[at] = (T)s;
 }
@@ -432,8 +433,9 @@ __global__ __launch_bounds__(256) void act_column_sum_kernel(WeightGradArgs a) {
     else a.parts[(i64)split * a.O + o] = t;
 }
 
-// Tile and splits by the sizes: 32 rows for layers with few outputs, whose codes are all the traffic; 256 x 256 where that fills the
-// chip; else 128 x 128.  Tokens are split until there are about two blocks a compute unit, in parts of at least 256 tokens.
+// Tile and splits: the cheapest of a few by a count of clocks.  A block costs `clocks` a token (measured with the chip full, `slots`
+// blocks at a time; the head and tail of a block as two steps more), the parts of a split sum are written and read at 1900 bytes a clock,
+// and joining them is a launch of its own.
 struct WeightGradPlan { int bm, bn, bk; i64 tiles_d, tiles, part; int splits; };
 WeightGradPlan weight_grad_plan(int dtype, i64 N, i64 O, i64 D) {
     WeightGradPlan p{};
@@ -444,18 +446,26 @@ WeightGradPlan weight_grad_plan(int dtype, i64 N, i64 O, i64 D) {
         p.splits = (int)(N ? (N + p.part - 1) / p.part : 1);
         return p;
     }
-    auto tiles = [&](int bm, int bn) { return ((O + bm - 1) / bm) * ((D + bn - 1) / bn); };
-    p.bk = dtype == TRL_F32 ? 32 : 64;
-    if (O <= 32) { p.bm = 32; p.bn = 128; p.bk = 64; }
-    else if (dtype != TRL_F32 && tiles(256, 256) >= 192) { p.bm = 256; p.bn = 256; }
-    else { p.bm = 128; p.bn = 128; }
-    p.tiles_d = (D + p.bn - 1) / p.bn;
-    p.tiles = tiles(p.bm, p.bn);
-    const i64 want = p.bm == 256 ? 1 : (512 + p.tiles - 1) / p.tiles, most = N / 256 > 0 ? N / 256 : 1;
-    i64 splits = want < most ? want : most;
-    p.part = ((N + splits - 1) / splits + p.bk - 1) / p.bk * p.bk;
-    if (p.part == 0) p.part = p.bk;
-    p.splits = (int)(N ? (N + p.part - 1) / p.part : 1);
+    struct Tile { int bm, bn, bk, slots; double clocks; };
+    static const Tile low[] = {{256, 256, 64, 256, 77.0}, {128, 128, 64, 512, 52.0}, {32, 128, 64, 768, 55.0}};
+    static const Tile f32[] = {{128, 128, 32, 512, 160.0}, {32, 128, 64, 512, 80.0}};
+    const Tile *from = dtype == TRL_F32 ? f32 : low, *to = dtype == TRL_F32 ? f32 + 2 : low + 3;
+    double best = 0.0;
+    for (const Tile *t = from; t < to; ++t) {
+        const i64 tiles_d = (D + t->bn - 1) / t->bn, tiles = tiles_d * ((O + t->bm - 1) / t->bm);
+        for (i64 s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+            i64 part = ((N + s - 1) / s + t->bk - 1) / t->bk * t->bk;
+            if (part == 0) part = t->bk;
+            const i64 splits = N ? (N + part - 1) / part : 1;
+            if (s > 1 && (part < 2 * t->bk || splits < 2)) break;
+            const i64 rounds = (tiles * splits + t->slots - 1) / t->slots;
+            const double cost = (double)rounds * (double)(part + 2 * t->bk) * t->clocks + (splits > 1 ? (double)splits * (double)(O * D) * 8.0 / 1900.0 + 9000.0 : 0.0);
+            if (p.splits == 0 || cost < best) {
+                best = cost;
+                p = {t->bm, t->bn, t->bk, tiles_d, tiles, part, (int)splits};
+            }
+        }
+    }
     return p;
 }
 
