@@ -473,8 +473,6 @@ template <typename T, int BM, int BN, int BK, int WM, int WN>
 void launch_weight_grad(hipStream_t s, const WeightGradArgs &a) {
     constexpr size_t bytes = 2 * sizeof(short) * BK * (kTerms<T> * (BM + 16) + BN + 16);
     static_assert(bytes <= 160 * 1024 && bytes >= sizeof(float) * kVec * WM * WN * kWave, "LDS: two buffers, and the column sums after them");
-    static const hipError_t raised = hipFuncSetAttribute((const void *)act_weight_grad_kernel<T, BM, BN, BK, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    (void)raised;
     hipLaunchKernelGGL((act_weight_grad_kernel<T, BM, BN, BK, WM, WN>), dim3((unsigned)(a.tiles * a.splits)), dim3(WM * WN * kWave), bytes, s, a);
 }
 template <typename T>

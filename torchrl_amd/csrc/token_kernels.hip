@@ -108,6 +108,7 @@ struct Counts8 {
 #pragma unroll
         for (int i = 0; i < 4; ++i) { c[i] = lo[i]; c[4 + i] = hi[i]; }
     }
+    __device__ __forceinline__ bool any() const { return ((c[0] | c[1] | c[2]) | (c[3] | c[4] | c[5]) | (c[6] | c[7])) != 0; }
     __device__ __forceinline__ static float factor(float z, u32 c, const Penalties &p) {
         const float f = z > 0.0f ? p.inv_rep : p.rep;
         return c ? f : 1.0f;
@@ -383,7 +384,7 @@ __global__ __launch_bounds__(W *kWave, PEN && BIAS ? 3 : 4) void token_kernel(To
 #pragma unroll
             for (int k = 0; k < kRowVecs; ++k) {
                 zr[k] = Raw8<T>{};
-                if (needs_z && bits[k]) load8(z_row + off[k], nv[k], zr[k]);
+                if (MODE != kProcessBwd && bits[k]) load8(z_row + off[k], nv[k], zr[k]);
                 if constexpr (MODE == kProcessBwd) {
                     gr[k] = Raw8<T>{};
                     if (bits[k]) load8(g_row + off[k], nv[k], gr[k]);
@@ -497,6 +498,9 @@ __global__ __launch_bounds__(W *kWave, PEN && BIAS ? 3 : 4) void token_kernel(To
                         for (int i = 0; i < kVec; ++i) z[i] = MODE == kProcess ? neg_inf() : 0.0f;
                     } else {
                         const Counts8 c = PEN ? Counts8(counts8 + k * kBlk, seen_places >> (k * kVec) & 0xffu) : Counts8();
+                        if constexpr (MODE == kProcessBwd && PEN) {  // the sign of a logit matters where it was repeated, and nowhere else
+                            if (needs_z && c.places && bits[k] && c.any()) load8(z_row + off[k], nv[k], zr[k]);
+                        }
                         float raw[kVec];
                         unpack8(zr[k], raw);
                         if constexpr (MODE == kProcessBwd) {
