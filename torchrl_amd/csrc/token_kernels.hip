@@ -202,14 +202,62 @@ struct RowAhead {
 };
 enum { kRowZero = 1, kRowSteep = 2 };  // no gradient; subtract first
 
-template <typename T, int MODE, bool PEN, bool BIAS, int W>
-__global__ __launch_bounds__(W *kWave, PEN && BIAS ? 3 : 4) void token_kernel(TokenArgs a) {
-    extern __shared__ __align__(16) u32 lds_counts[];  // PEN: W * kSub words
+// Joins a row's partials (one a sub-slice): called by a whole wave.
+__device__ __forceinline__ void join_row(const TokenArgs &a, i64 r, i64 y, const float4 *part, i64 nsubs, float z_action) {
+    const int lane = threadIdx.x & (kWave - 1);
+    float log_prob = 0.0f, entropy = 0.0f, m = neg_inf(), log2s = 0.0f;
+    if (y >= 0) {
+        for (i64 i = lane; i < nsubs; i += kWave) m = fmaxf(m, part[i].x);
+        m = wave_max_f(m);
+        const float scale = kLog2e * (1.0f / (a.temp_t ? a.temp_t[r / a.T] : a.temp));  // the row kernel's own bits
+        bool steep;
+        const float shift = softmax_shift(m, scale, &steep);
+        float s = 0.0f, u = 0.0f;
+        for (i64 i = lane; i < nsubs; i += kWave) {
+            const float4 q = part[i];
+            float d = 0.0f;
+            if (q.x != m) {
+                bool own;  // whether the wave's values are relative to q.x itself
+                const float its = softmax_shift(q.x, scale, &own);
+                if (q.x == neg_inf()) d = neg_inf();
+                else if (own) d = steep ? (q.x - m) * scale : fmaf(q.x, scale, -shift);
+                else d = steep ? fmaf(-m, scale, its) : its - shift;
+            }
+            const float w = exp2_hw(d);
+            s = fmaf(w, q.y, s);
+            u = fmaf(w, fmaf(q.y, fmaxf(d, kFloor), q.z), u);
+        }
+        s = wave_sum_f(s);
+        u = wave_sum_f(u);
+        if (m == neg_inf() && s == 0.0f) {  // nothing allowed, or nothing possible
+            log_prob = neg_inf();
+        } else {
+            const float z = steep ? z_action - m : z_action;
+            log2s = log2f(s);
+            entropy = kLn2 * (log2s - u / s);
+            log_prob = kLn2 * (fmaf(z, scale, -shift) - log2s);
+        }
+        if (y >= a.V) log_prob = __builtin_nanf("");
+    }
+    if (lane == 0) {
+        a.log_prob[r] = log_prob;
+        if (a.entropy) a.entropy[r] = entropy;
+        if (a.stats) { a.stats[2 * r] = m; a.stats[2 * r + 1] = log2s; }
+    }
+}
+
+// Waves of a block (the launch picks up to that many): a bias in registers beside the counts leaves room for three waves a SIMD.
+template <int MODE, bool PEN, bool BIAS> constexpr int kMostWaves = !PEN || (BIAS && MODE != kProcess) ? 4 : 16;
+
+template <typename T, int MODE, bool PEN, bool BIAS>
+__global__ __launch_bounds__((kMostWaves<MODE, PEN, BIAS>) * kWave, PEN && BIAS && MODE != kProcess ? 3 : 4) void token_kernel(TokenArgs a) {
+    extern __shared__ __align__(16) u32 lds_counts[];  // PEN: a sub-slice a wave
+    const int W = blockDim.x / kWave;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const u32 nslices = (u32)a.nslices, nchunks = (u32)a.nchunks, rest = scalar((int)(blockIdx.x / nslices)), slice = blockIdx.x - rest * nslices;
     const i64 b = scalar((int)(rest / nchunks)), t0 = (i64)(rest - (u32)b * nchunks) * a.chunk;
     const int rows = a.T - t0 < a.chunk ? (int)(a.T - t0) : (int)a.chunk;
-    const i64 slice_lo = (i64)slice * (W * kSub), lo = slice_lo + wave * kSub, r0 = b * a.T + t0;
+    const i64 slice_lo = (i64)slice * W * kSub, lo = slice_lo + wave * kSub, r0 = b * a.T + t0;
     u32 *counts = lds_counts + wave * kSub;
 
     RowAhead mine;
@@ -229,10 +277,10 @@ __global__ __launch_bounds__(W *kWave, PEN && BIAS ? 3 : 4) void token_kernel(To
         prompt = p < 0 ? 0 : p > a.L ? (int)a.L : (int)p;
         u32x4 *c4 = (u32x4 *)lds_counts;
 #pragma unroll
-        for (int i = 0; i < kSub / 4 / kWave; ++i) c4[threadIdx.x + i * (W * kWave)] = u32x4{0, 0, 0, 0};
+        for (int i = 0; i < kSub / 4 / kWave; ++i) c4[threadIdx.x + i * blockDim.x] = u32x4{0, 0, 0, 0};
         __syncthreads();
         h = read_lane(mine.want, 0);
-        for (int j = threadIdx.x; j < h; j += W * kWave)
+        for (int j = threadIdx.x; j < h; j += blockDim.x)
             count_token(lds_counts, load_int(a.tokens, a.tokens_wide, b * a.tokens_sb + j), slice_lo, W * kSub, j < prompt);
         __syncthreads();
     }
@@ -547,76 +595,45 @@ __global__ __launch_bounds__(W *kWave, PEN && BIAS ? 3 : 4) void token_kernel(To
     else run_rows(Bool<false>());
 }
 
-// Joins a row's partials: one wave a row.
+// Rows of many blocks: one wave a row.
 __global__ __launch_bounds__(256) void token_join_kernel(TokenArgs a) {
-    const int lane = threadIdx.x & (kWave - 1);
     const i64 r = (i64)blockIdx.x * 4 + threadIdx.x / kWave;
     if (r >= a.B * a.T) return;
     const i64 y = load_int(a.action, a.action_wide, r);
-    float log_prob = 0.0f, entropy = 0.0f, m = neg_inf(), log2s = 0.0f;
-    if (y >= 0) {
-        const float4 *part = (const float4 *)a.partials + r * a.nsubs;
-        for (i64 i = lane; i < a.nsubs; i += kWave) m = fmaxf(m, part[i].x);
-        m = wave_max_f(m);
-        const float scale = kLog2e * (1.0f / (a.temp_t ? a.temp_t[r / a.T] : a.temp));  // the row kernel's own bits
-        bool steep;
-        const float shift = softmax_shift(m, scale, &steep);
-        float s = 0.0f, u = 0.0f;
-        for (i64 i = lane; i < a.nsubs; i += kWave) {
-            const float4 q = part[i];
-            float d = 0.0f;
-            if (q.x != m) {
-                bool own;  // whether the wave's values are relative to q.x itself
-                const float its = softmax_shift(q.x, scale, &own);
-                if (q.x == neg_inf()) d = neg_inf();
-                else if (own) d = steep ? (q.x - m) * scale : fmaf(q.x, scale, -shift);
-                else d = steep ? fmaf(-m, scale, its) : its - shift;
-            }
-            const float w = exp2_hw(d);
-            s = fmaf(w, q.y, s);
-            u = fmaf(w, fmaf(q.y, fmaxf(d, kFloor), q.z), u);
-        }
-        s = wave_sum_f(s);
-        u = wave_sum_f(u);
-        if (m == neg_inf() && s == 0.0f) {  // nothing allowed, or nothing possible
-            log_prob = neg_inf();
-        } else {
-            float z = y < a.V ? a.z_action[r] : __builtin_nanf("");
-            if (steep) z -= m;
-            log2s = log2f(s);
-            entropy = kLn2 * (log2s - u / s);
-            log_prob = kLn2 * (fmaf(z, scale, -shift) - log2s);
-        }
-        if (y >= a.V) log_prob = __builtin_nanf("");
-    }
-    if (lane == 0) {
-        a.log_prob[r] = log_prob;
-        if (a.entropy) a.entropy[r] = entropy;
-        if (a.stats) { a.stats[2 * r] = m; a.stats[2 * r + 1] = log2s; }
-    }
+    join_row(a, r, y, (const float4 *)a.partials + r * a.nsubs, a.nsubs, y >= 0 && y < a.V ? a.z_action[r] : 0.0f);
 }
 
-template <typename T, int MODE, bool PEN, bool BIAS, int W>
-int launch_w(hipStream_t s, TokenArgs &a) {
-    const i64 span = (i64)W * kSub;
-    a.nslices = (a.V + span - 1) / span;
+// Blocks of as many waves as an even split of the vocabulary gives them, up to 8 beside a history: two such blocks share a compute unit,
+// and one streams while the other counts.  Up to 16, one block a unit, where the counting is shared by enough: long histories, or runs of
+// many rows (256 x 131072 bf16, 4096 tokens: 37 us and 40; 8192 x 131072, backward: 795 and 830; but 910 x 50263 fp32: 117 and 103).
+template <typename T, int MODE, bool PEN, bool BIAS>
+int launch_waves(hipStream_t s, TokenArgs &a) {
     a.nsubs = token_subs(a.V);
-    const i64 units = a.nslices * a.B * a.T;
-    a.chunk = units / 2048;  // enough blocks for every compute unit, then as long a run of rows as that leaves (a lane holds a row's scalars)
+    const i64 rows = a.B * a.T;
+    i64 most = kMostWaves<MODE, PEN, BIAS>;
+    if (most > 8) {
+        const i64 blocks = (a.nsubs + most - 1) / most * rows;
+        if (blocks < 1024 || (a.L < 2048 && blocks < 4096)) most = 8;
+    }
+    a.nslices = (a.nsubs + most - 1) / most;
+    const i64 waves = (a.nsubs + a.nslices - 1) / a.nslices, units = a.nslices * rows;
+    // enough blocks for every compute unit, then as long a run of rows as that leaves (a lane holds a row's scalars)
+    a.chunk = units * waves / (PEN ? 16384 : 8192);
     a.chunk = a.chunk < 1 ? 1 : a.chunk > kWave ? kWave : a.chunk;
     if (a.chunk > a.T) a.chunk = a.T;
     a.nchunks = (a.T + a.chunk - 1) / a.chunk;
     const i64 grid = a.nslices * a.nchunks * a.B;
     if (grid > 0x7fffffffLL) return 2;
-    hipLaunchKernelGGL((token_kernel<T, MODE, PEN, BIAS, W>), dim3((unsigned)grid), dim3(W * kWave), PEN ? W * kSub * sizeof(u32) : 0, s, a);
+    const size_t lds = (PEN ? waves * kSub * sizeof(u32) : 0);
+    hipLaunchKernelGGL((token_kernel<T, MODE, PEN, BIAS>), dim3((unsigned)grid), dim3((unsigned)waves * kWave), lds, s, a);
     return 0;
 }
 template <typename T, int MODE>
 int launch_mode(hipStream_t s, TokenArgs &a) {
     if constexpr (MODE != kProcessBwd) {
-        if (a.bias_kind != kBiasNone) return a.tokens ? launch_w<T, MODE, true, true, 4>(s, a) : launch_w<T, MODE, false, true, 4>(s, a);
+        if (a.bias_kind != kBiasNone) return a.tokens ? launch_waves<T, MODE, true, true>(s, a) : launch_waves<T, MODE, false, true>(s, a);
     }
-    return a.tokens ? launch_w<T, MODE, true, false, 8>(s, a) : launch_w<T, MODE, false, false, 4>(s, a);
+    return a.tokens ? launch_waves<T, MODE, true, false>(s, a) : launch_waves<T, MODE, false, false>(s, a);
 }
 template <int MODE>
 int launch_dtype(hipStream_t s, TokenArgs &a) {
