@@ -616,11 +616,17 @@ int launch_waves(hipStream_t s, TokenArgs &a) {
         if (blocks < 1024 || (a.L < 2048 && blocks < 4096)) most = 8;
     }
     a.nslices = (a.nsubs + most - 1) / most;
-    const i64 waves = (a.nsubs + a.nslices - 1) / a.nslices, units = a.nslices * rows;
-    // enough blocks for every compute unit, then as long a run of rows as that leaves (a lane holds a row's scalars)
-    a.chunk = units * waves / (PEN ? 16384 : 8192);
-    a.chunk = a.chunk < 1 ? 1 : a.chunk > kWave ? kWave : a.chunk;
-    if (a.chunk > a.T) a.chunk = a.T;
+    const i64 waves = (a.nsubs + a.nslices - 1) / a.nslices;
+    // The run of rows of a block (a lane holds a row's scalars): as few rounds of blocks as the chip takes at a time, counted in rows, with
+    // the block's start as some rows more -- short runs count the history over and over, long ones leave a last round half empty.
+    const i64 slots = 256 * (PEN ? (waves > 8 ? 1 : waves > 4 ? 2 : 4) : 4);
+    const double start = PEN ? 2.0 + (double)a.L / 1024.0 : 1.0;
+    double best = 0.0;
+    for (i64 c = 1; c <= kWave && c <= a.T; ++c) {
+        const i64 blocks = a.nslices * a.B * ((a.T + c - 1) / c), rounds = (blocks + slots - 1) / slots;
+        const double cost = (double)rounds * ((double)c + start);
+        if (c == 1 || cost < best) { best = cost; a.chunk = c; }
+    }
     a.nchunks = (a.T + a.chunk - 1) / a.chunk;
     const i64 grid = a.nslices * a.nchunks * a.B;
     if (grid > 0x7fffffffLL) return 2;
