@@ -808,7 +808,7 @@ static bool low_dtype_ok(int d) { return d == TRL_F32 || d == TRL_BF16 || d == T
 static int check_token_args(const char *fn, const trl_token_args *a, bool *empty) {
     if (!a) return fail(TRL_ERR_INVALID_ARGUMENT, "%s: null arguments", fn);
     if (!low_dtype_ok(a->dtype)) return fail(TRL_ERR_INVALID_ARGUMENT, "%s: bad dtype", fn);
-    if (a->B < 0 || a->T < 0 || a->V <= 0 || a->V > 0x7fffffffLL || a->L < 0 || a->L > 0x7fffffffLL - 64)
+    if (a->B < 0 || a->T < 0 || a->V <= 0 || a->V > 0x7fffffffLL || a->L < 0 || a->L > 0x7fffe000LL)
         return fail(TRL_ERR_INVALID_ARGUMENT, "%s: bad sizes (B %lld, T %lld, V %lld, L %lld)", fn, (long long)a->B, (long long)a->T, (long long)a->V,
                     (long long)a->L);
     if ((long double)a->B * (long double)a->T * (long double)a->V > 4.0e18L) return fail(TRL_ERR_INVALID_ARGUMENT, "%s: B*T*V too large", fn);

@@ -275,13 +275,30 @@ __global__ __launch_bounds__((kMostWaves<MODE, PEN, BIAS>) * kWave, PEN && BIAS 
     if constexpr (PEN) {
         const i64 p = a.prompt ? load_int(a.prompt, a.prompt_wide, b) : 0;
         prompt = p < 0 ? 0 : p > a.L ? (int)a.L : (int)p;
+        // four tokens a thread at a time; the first are on their way before the history's length is known
+        constexpr int kAhead = 4;
+        i64 ahead[kAhead];
+        auto fetch = [&](int from, int end) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int j = from + i * (int)blockDim.x + (int)threadIdx.x;
+                ahead[i] = j < end ? load_int(a.tokens, a.tokens_wide, b * a.tokens_sb + j) : -1;
+            }
+        };
+        fetch(0, (int)a.L < kAhead * (int)blockDim.x ? (int)a.L : kAhead * (int)blockDim.x);
         u32x4 *c4 = (u32x4 *)lds_counts;
 #pragma unroll
         for (int i = 0; i < kSub / 4 / kWave; ++i) c4[threadIdx.x + i * blockDim.x] = u32x4{0, 0, 0, 0};
         __syncthreads();
         h = read_lane(mine.want, 0);
-        for (int j = threadIdx.x; j < h; j += blockDim.x)
-            count_token(lds_counts, load_int(a.tokens, a.tokens_wide, b * a.tokens_sb + j), slice_lo, W * kSub, j < prompt);
+        for (int from = 0; from < h; from += kAhead * (int)blockDim.x) {
+            if (from) fetch(from, h);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int j = from + i * (int)blockDim.x + (int)threadIdx.x;
+                if (j < h) count_token(lds_counts, ahead[i], slice_lo, W * kSub, j < prompt);
+            }
+        }
         __syncthreads();
     }
     if (lo >= a.V) return;
