@@ -1,0 +1,45 @@
+"""GPU: torch.compile(fullgraph=True) over the token-policy operators and the 8-bit activations: the eager calls' results, gradients included."""
+import pytest
+import torch
+
+from torchrl_amd.objectives.value import CheckpointedLinear, process_logits, token_log_prob
+
+pytestmark = pytest.mark.gpu
+
+
+def test_a_policy_gradient_step_compiles_fullgraph():
+    torch.manual_seed(0)
+    B, T, D, V, P = 2, 6, 40, 130, 3
+    dev = "cuda"
+    x = torch.randn(B, T, D, device=dev)
+    tokens = torch.randint(0, V, (B, P + T), device=dev)
+    lengths = (P + torch.arange(T, device=dev)).expand(B, T).contiguous()
+    mask = torch.rand(B, T, V, device=dev) < 0.8
+    temperature = torch.rand(B, device=dev) + 0.5
+    adv = torch.randn(B, T, device=dev)
+    head = CheckpointedLinear(D, V, device=dev)
+
+    def step(x):
+        z = head(x)
+        kw = dict(tokens=tokens, lengths=lengths, repetition_penalty=1.2, frequency_penalty=0.1, mask=mask, temperature=temperature)
+        lp, H = token_log_prob(z, tokens[:, P:], entropy=True, **kw)
+        out = process_logits(z, **kw)
+        return lp, H, out, -(lp.clamp(min=-20) * adv).mean() - 0.01 * H.mean() + 0.001 * out.clamp(min=-20).mean()
+
+    def run(fn):
+        leaf = x.clone().requires_grad_()
+        head.zero_grad()
+        lp, H, out, loss = fn(leaf)
+        loss.backward()
+        return lp.detach(), H.detach(), out.detach(), leaf.grad, head.weight.grad.clone(), head.bias.grad.clone()
+
+    for a, b in zip(run(step), run(torch.compile(step, fullgraph=True))):
+        # the ops are the same kernels; the sums around them are fused: a few roundings of values of this size
+        torch.testing.assert_close(a, b, rtol=1e-5, atol=1e-6)
+
+
+def test_refusals_under_compile():
+    z = torch.randn(2, 3, 20, device="cuda", requires_grad=True)
+    bias = torch.zeros(20, device="cuda", requires_grad=True)
+    with pytest.raises(Exception, match="bias"):
+        torch.compile(lambda z: process_logits(z, bias=bias), fullgraph=True)(z)

@@ -404,3 +404,182 @@ def standardize_op(x: Tensor, eps: float) -> Tensor:
 @standardize_op.register_fake
 def _(x, eps):
     return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+# ---- policies over tokens ---------------------------------------------------------------------------------------------------
+# One op a pass, over the checked calls of tokens.py: eager entry points reach the same kernels without the dispatcher.
+_TOKEN_ARGS = ("Tensor? tokens, Tensor? lengths, Tensor? prompt, float rep, Tensor? rep_t, float pres, Tensor? pres_t, float freq, Tensor? freq_t, "
+               "Tensor? bias, Tensor? mask, float temp, Tensor? temp_t")
+
+
+def _token_call(logits, tokens, lengths, prompt, rep, rep_t, pres, pres_t, freq, freq_t, bias, mask, temp, temp_t):
+    from torchrl_amd.objectives.value import tokens as K
+    return K, K._processing(logits, tokens, lengths, prompt, _coef(rep, rep_t), _coef(pres, pres_t), _coef(freq, freq_t), bias, mask, _coef(temp, temp_t))
+
+
+def _token_args(tokens, lengths, prompt, rep, pres, freq, bias, mask, temp):
+    for name, x in (("repetition_penalty", rep), ("presence_penalty", pres), ("frequency_penalty", freq), ("bias", bias), ("temperature", temp)):
+        if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError(f"gradients with respect to {name} are not implemented: detach it")
+    return (tokens, lengths, prompt, *_split(rep), *_split(pres), *_split(freq), bias, mask, *_split(temp))
+
+
+@torch.library.custom_op(f"{_NS}::process_logits", mutates_args=(), schema=f"(Tensor logits, {_TOKEN_ARGS}) -> Tensor")
+def process_logits_op(logits, *args):
+    with torch.no_grad():
+        K, p = _token_call(logits, *args)
+        out = torch.empty(p.B, p.T, p.V, dtype=logits.dtype, device=logits.device)
+        K._process_fwd(p, out)
+        return out.view(logits.shape)
+
+
+@process_logits_op.register_fake
+def _(logits, *args):
+    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+
+
+@torch.library.custom_op(f"{_NS}::process_logits_bwd", mutates_args=(), schema=f"(Tensor grad, Tensor logits, {_TOKEN_ARGS}) -> Tensor")
+def process_logits_bwd_op(grad, logits, *args):
+    with torch.no_grad():
+        K, p = _token_call(logits, *args)
+        return K._process_bwd(p, grad).view(logits.shape)
+
+
+@process_logits_bwd_op.register_fake
+def _(grad, logits, *args):
+    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+
+
+def _token_setup(ctx, inputs, output):
+    ctx.tensors = [isinstance(x, torch.Tensor) for x in inputs]
+    ctx.rest = [None if t else x for t, x in zip(ctx.tensors, inputs)]
+    more = output[1:] if isinstance(output, tuple) else ()
+    ctx.save_for_backward(*(x for t, x in zip(ctx.tensors, inputs) if t), *more)
+
+
+def _token_saved(ctx):
+    kept = iter(ctx.saved_tensors)
+    return [next(kept) if t else x for t, x in zip(ctx.tensors, ctx.rest)], list(kept)
+
+
+def _process_logits_backward(ctx, grad):
+    inputs, _ = _token_saved(ctx)
+    return (process_logits_bwd_op(grad, *inputs),) + (None,) * 13
+
+
+process_logits_op.register_autograd(_process_logits_backward, setup_context=_token_setup)
+
+
+def process_logits(logits, *args):
+    return process_logits_op(logits, *_token_args(*args))
+
+
+@torch.library.custom_op(f"{_NS}::token_log_prob", mutates_args=(), schema=f"(Tensor logits, Tensor action, {_TOKEN_ARGS}) -> (Tensor, Tensor, Tensor)")
+def token_log_prob_op(logits, action, *args):
+    with torch.no_grad():
+        K, p = _token_call(logits, *args)
+        act = K._int_tensor(action, logits.shape[:-1], "action", logits.device)
+        log_prob, H, stats = K._log_prob_fwd(p, act, True, True)
+        return log_prob.view(action.shape), H.view(action.shape), stats
+
+
+@token_log_prob_op.register_fake
+def _(logits, action, *args):
+    new = lambda shape: torch.empty(shape, dtype=torch.float32, device=logits.device)  # noqa: E731
+    return new(action.shape), new(action.shape), new((action.numel(), 2))
+
+
+@torch.library.custom_op(f"{_NS}::token_log_prob_bwd", mutates_args=(),
+                         schema=f"(Tensor g_lp, Tensor g_H, Tensor H, Tensor stats, Tensor logits, Tensor action, {_TOKEN_ARGS}) -> Tensor")
+def token_log_prob_bwd_op(g_lp, g_H, H, stats, logits, action, *args):
+    with torch.no_grad():
+        K, p = _token_call(logits, *args)
+        act = K._int_tensor(action, logits.shape[:-1], "action", logits.device)
+        return K._log_prob_bwd(p, act, H.reshape(-1).contiguous(), stats.contiguous(), g_lp, g_H).view(logits.shape)
+
+
+@token_log_prob_bwd_op.register_fake
+def _(g_lp, g_H, H, stats, logits, action, *args):
+    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+
+
+def _token_log_prob_backward(ctx, g_lp, g_H, _):
+    inputs, (H, stats) = _token_saved(ctx)
+    zero = lambda g: torch.zeros_like(H) if g is None else g  # noqa: E731
+    return (token_log_prob_bwd_op(zero(g_lp), zero(g_H), H, stats, *inputs),) + (None,) * 14
+
+
+token_log_prob_op.register_autograd(_token_log_prob_backward, setup_context=_token_setup)
+
+
+def token_log_prob(logits, action, entropy, *args):
+    log_prob, H, _ = token_log_prob_op(logits, action, *_token_args(*args))
+    return (log_prob, H) if entropy else log_prob
+
+
+# ---- activations kept in 8 bits ---------------------------------------------------------------------------------------------
+@torch.library.custom_op(f"{_NS}::quantize_activation", mutates_args=())
+def quantize_activation_op(x: Tensor) -> Tuple[Tensor, Tensor]:
+    from torchrl_amd.objectives.value import kept_activations as K
+    with torch.no_grad():
+        kept = K.quantize_activation(x)
+        return kept.codes, kept.exponents
+
+
+def _kept_shapes(x):
+    blocks = (x.shape[-1] + 31) // 32
+    return (torch.empty((*x.shape[:-1], blocks * 32), dtype=torch.int8, device=x.device),
+            torch.empty((*x.shape[:-1], blocks), dtype=torch.uint8, device=x.device))
+
+
+@quantize_activation_op.register_fake
+def _(x):
+    return _kept_shapes(x)
+
+
+@torch.library.custom_op(f"{_NS}::checkpointed_linear", mutates_args=())
+def checkpointed_linear_op(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
+    from torchrl_amd.objectives.value import kept_activations as K
+    with torch.no_grad():
+        K.checkpointed_linear_check(x, weight, bias)
+        kept = K.quantize_activation(x)
+        return torch.nn.functional.linear(x, weight, bias), kept.codes, kept.exponents
+
+
+@checkpointed_linear_op.register_fake
+def _(x, weight, bias):
+    return (torch.empty((*x.shape[:-1], weight.shape[0]), dtype=x.dtype, device=x.device), *_kept_shapes(x))
+
+
+@torch.library.custom_op(f"{_NS}::activation_weight_grad", mutates_args=())
+def activation_weight_grad_op(dy: Tensor, codes: Tensor, exponents: Tensor, features: int) -> Tuple[Tensor, Tensor]:
+    from torchrl_amd.objectives.value import kept_activations as K
+    with torch.no_grad():
+        return K._weight_grad(dy, codes, exponents, features, True)
+
+
+@activation_weight_grad_op.register_fake
+def _(dy, codes, exponents, features):
+    return (torch.empty((dy.shape[1], features), dtype=dy.dtype, device=dy.device), torch.empty((dy.shape[1],), dtype=dy.dtype, device=dy.device))
+
+
+def _checkpointed_linear_setup(ctx, inputs, output):
+    x, weight, bias = inputs
+    ctx.save_for_backward(weight, output[1], output[2])
+    ctx.features = x.shape[-1]
+
+
+def _checkpointed_linear_backward(ctx, grad, _codes, _exponents):
+    weight, codes, exponents = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dy = grad.reshape(-1, grad.shape[-1])
+    dx = (dy @ weight).reshape(*grad.shape[:-1], ctx.features) if need[0] else None
+    dw, db = activation_weight_grad_op(dy, codes, exponents, ctx.features) if need[1] or need[2] else (None, None)
+    return dx, dw if need[1] else None, db if need[2] else None
+
+
+checkpointed_linear_op.register_autograd(_checkpointed_linear_backward, setup_context=_checkpointed_linear_setup)
+
+
+def checkpointed_linear(x, weight, bias):
+    return checkpointed_linear_op(x, weight, bias)[0]

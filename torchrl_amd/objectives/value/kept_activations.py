@@ -95,6 +95,9 @@ class QuantizedActivation:
 def quantize_activation(x: Tensor) -> QuantizedActivation:
     """Keeps ``x`` ``[*B, D]`` (float32, bfloat16 or float16) in 8 bits: blocks of 32 features share a power of two, 2^-6 of the one at or below
     the block's largest magnitude; codes are rounded to nearest even and held to 127.  Blocks with a NaN or an infinity stand for NaN."""
+    if torch.compiler.is_compiling():
+        from torchrl_amd.objectives.value import _ops
+        return QuantizedActivation(*_ops.quantize_activation_op(x), x.shape, x.dtype)
     host = F._HOST if F._HOST_TRIED else F._host_module()
     if host is not None:
         got = host.quantize(x)
@@ -157,18 +160,28 @@ def checkpointed_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None
 
     ``x`` ``[*B, D]``, ``weight`` ``[O, D]`` and ``bias`` ``[O]`` share one dtype (float32, bfloat16 or float16) and device; under autocast they
     are cast to its dtype.  Without a gradient to ``weight`` nothing is kept."""
-    if not torch.is_autocast_enabled("cuda"):
+    autocast = torch.is_autocast_enabled("cuda")
+    if not autocast and not torch.compiler.is_compiling():
         host = F._HOST if F._HOST_TRIED else F._host_module()
         if host is not None:  # checks, launches and the autograd node in one C++ hop (csrc/host_policy.cpp)
             got = host.checkpointed_linear(x, weight, bias)
             if got is not None:
                 return _done(got)
+    if autocast and all(isinstance(t, Tensor) for t in (x, weight)):
+        dt = torch.get_autocast_dtype("cuda")
+        x, weight, bias = x.to(dt), weight.to(dt), None if bias is None else bias.to(dt)
+    if torch.compiler.is_compiling():
+        from torchrl_amd.objectives.value import _ops
+        return _ops.checkpointed_linear(x, weight, bias)
+    checkpointed_linear_check(x, weight, bias)
+    return _CheckpointedLinear.apply(x, weight, bias)
+
+
+def checkpointed_linear_check(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> None:
+    """Raises for arguments that :func:`checkpointed_linear` does not take."""
     for t, name in ((x, "x"), (weight, "weight"), (bias, "bias")):
         if t is not None or name != "bias":
             _check(t, name)
-    if torch.is_autocast_enabled("cuda"):
-        dt = torch.get_autocast_dtype("cuda")
-        x, weight, bias = x.to(dt), weight.to(dt), None if bias is None else bias.to(dt)
     if weight.ndim != 2 or x.ndim < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
         raise RuntimeError(f"checkpointed_linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")
     if bias is not None and tuple(bias.shape) != (weight.shape[0],):
@@ -177,7 +190,6 @@ def checkpointed_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None
         if t is not None and (t.dtype != x.dtype or t.device != x.device):
             raise RuntimeError(f"checkpointed_linear: {name} is {t.dtype} on {t.device}, x is {x.dtype} on {x.device}")
     _check_device(x)
-    return _CheckpointedLinear.apply(x, weight, bias)
 
 
 class CheckpointedLinear(nn.Linear):
