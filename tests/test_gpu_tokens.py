@@ -429,6 +429,12 @@ def test_autograd_manners(route, monkeypatch):
         lp = token_log_prob(leaf, action, **kw)
     (offloaded,) = torch.autograd.grad(lp.nan_to_num(0, 0, 0).sum(), leaf)
     assert packed and torch.equal(offloaded, first)
+    wide = torch.zeros(2, 3, 300, dtype=torch.bool, device="cuda")  # the kept mask comes back dense
+    wide[..., 40:130] = kw["mask"]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+        out = process_logits(leaf, mask=wide[..., 40:130])
+    (d,) = torch.autograd.grad(out.masked_fill(~kw["mask"], 0).sum(), leaf)
+    assert torch.equal(d != 0, kw["mask"])
     with torch.no_grad():
         assert not token_log_prob(leaf, action, **kw).requires_grad
     assert not process_logits(leaf.detach(), **kw).requires_grad

@@ -36,6 +36,8 @@ PEN = dict(tokens=TOK, lengths=LEN, repetition_penalty=1.1)
     (Z, dict(temperature=0.0), ValueError, "positive"),
     (Z, dict(temperature=-1.0), ValueError, "positive"),
     (Z, dict(temperature=math.nan), ValueError, "positive"),
+    (Z, dict(temperature=1e-39), ValueError, "positive"),
+    (Z, dict(PEN, frequency_penalty=1e39), ValueError, "finite"),
     (Z, dict(temperature=torch.ones(3)), RuntimeError, "does not broadcast to the sequences"),
     (Z, dict(temperature=torch.ones(2, dtype=torch.long)), RuntimeError, "floating-point"),
     (Z, dict(temperature=torch.ones(2, requires_grad=True)), NotImplementedError, "temperature"),

@@ -21,6 +21,7 @@
 #include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <c10/hip/HIPStream.h>
 
+#include <cfloat>
 #include <cmath>
 #include <cstdint>
 
@@ -66,7 +67,7 @@ bool number(PyObject *o, bool positive, float &out) {
     else return false;
     if (PyErr_Occurred()) { PyErr_Clear(); return false; }
     out = (float)x;
-    return std::isfinite(x) && std::isfinite(out) && (!positive || out > 0.0f);
+    return std::isfinite(x) && std::isfinite(out) && (!positive || out >= FLT_MIN);
 }
 
 // The tensors of a call's processing, in the order in which autograd keeps them.
@@ -77,17 +78,20 @@ struct Processing {
 
     // strides of [V], [B, V] or [B, T, V]; false: not that
     bool row_strides(const at::Tensor &t, int64_t last, int64_t &sb, int64_t &st) const {
-        const int64_t nd = logits.dim(), es = t.element_size();
+        const int64_t nd = steps ? 3 : 2, es = t.element_size();
         if (t.dim() < 1 || t.size(-1) != last || (t.stride(-1) != 1 && last != 1)) return false;
         sb = st = 0;
         if (t.dim() == 1) return true;
         if (t.dim() != nd) return false;
         for (int64_t k = 0; k + 1 < nd; ++k) {
-            if (t.size(k) != 1 && t.size(k) != logits.size(k)) return false;
+            const int64_t rows = k == 0 ? a.B : a.T;
+            if (t.size(k) != 1 && t.size(k) != rows) return false;
             (k == 0 ? sb : st) = t.size(k) == 1 ? 0 : t.stride(k) * es;
         }
         return true;
     }
+    bool bias_strides() { return row_strides(bias, a.V, a.bias_sb, a.bias_st); }
+    bool mask_strides() { return row_strides(mask, mask.scalar_type() == at::kInt ? (a.V + 31) / 32 : a.V, a.mask_sb, a.mask_st); }
     // pointers and strides of the tensors as they are now
     bool bind() {
         if (logits.defined()) {
@@ -140,12 +144,12 @@ struct Processing {
         a.prompt_wide = prompt.defined() && prompt.scalar_type() == at::kLong;
         if (bias.defined()) {
             const int code = dtype_code(bias.scalar_type());
-            if (code < 0 || bias.device() != dev || wants_grad(bias) || !row_strides(bias, a.V, a.bias_sb, a.bias_st)) return false;
+            if (code < 0 || bias.device() != dev || wants_grad(bias) || !bias_strides()) return false;
             a.bias_kind = 1 + code;
         }
         if (mask.defined()) {
             const bool bits = mask.scalar_type() == at::kInt;
-            if ((!bits && mask.scalar_type() != at::kBool) || mask.device() != dev || !row_strides(mask, bits ? (a.V + 31) / 32 : a.V, a.mask_sb, a.mask_st)) return false;
+            if ((!bits && mask.scalar_type() != at::kBool) || mask.device() != dev || !mask_strides()) return false;
             a.mask_kind = bits ? TRL_MASK_BITS : TRL_MASK_BOOL;
         }
         return bind();
@@ -177,12 +181,12 @@ struct KeptProcessing {
         p.a = a;
         p.a.logits = nullptr;
         p.steps = steps;
-        if (p.logits.defined()) {
-            if (p.bias.defined()) TORCH_CHECK(p.row_strides(p.bias, a.V, p.a.bias_sb, p.a.bias_st), "torchrl_amd: the kept bias changed its shape");
-            if (p.mask.defined())
-                TORCH_CHECK(p.row_strides(p.mask, a.mask_kind == TRL_MASK_BITS ? (a.V + 31) / 32 : a.V, p.a.mask_sb, p.a.mask_st),
-                            "torchrl_amd: the kept mask changed its shape");
-        }
+        // a hook may hand back the values in another layout: the strides are those of the tensors as they are now
+        for (at::Tensor *t : {&p.lengths, &p.prompt})
+            if (t->defined()) *t = t->contiguous();
+        for (at::Tensor *t : {&p.logits, &p.tokens, &p.bias, &p.mask})
+            if (t->defined() && t->stride(-1) != 1) *t = t->contiguous();
+        TORCH_CHECK((!p.bias.defined() || p.bias_strides()) && (!p.mask.defined() || p.mask_strides()), "torchrl_amd: a kept bias or mask changed its shape");
         p.bind();
         return p;
     }
@@ -241,7 +245,8 @@ struct TokenLogProbBackward : torch::autograd::Node {
             c10::DeviceGuard guard((g_lp.defined() ? g_lp : g_h).device());
             c10::AutoGradMode off(false);
             Processing p = kept.get();
-            const at::Tensor act = action.unpack(), st = stats.unpack(), h = g_h.defined() ? entropy.unpack(shared_from_this()) : at::Tensor();
+            const at::Tensor act = action.unpack().contiguous(), st = stats.unpack().contiguous(),
+                             h = g_h.defined() ? entropy.unpack(shared_from_this()).contiguous() : at::Tensor();
             g_lp = row_grad(g_lp);
             g_h = row_grad(g_h);
             d = at::empty(kept.sizes, kept.options);
@@ -304,7 +309,7 @@ struct CheckpointedLinearBackward : torch::autograd::Node {
             }
             const bool w = need_w && task_should_compute_output(1), b = need_b && task_should_compute_output(2);
             if (w || b) {
-                const at::Tensor c = w ? codes.unpack() : at::Tensor(), e = w ? exponents.unpack() : at::Tensor();
+                const at::Tensor c = w ? codes.unpack().contiguous() : at::Tensor(), e = w ? exponents.unpack().contiguous() : at::Tensor();
                 const int code = dtype_code(dy.scalar_type());
                 if (w) dw = at::empty({O, features}, dy.options());
                 if (b) db = at::empty({O}, dy.options());

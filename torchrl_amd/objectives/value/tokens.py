@@ -76,7 +76,8 @@ def _rows_view(x: Tensor, batch, T: int, name: str) -> Tensor:
 def _per_sequence(x: Scalar, batch, name: str, device, positive: bool) -> Tuple[float, Optional[Tensor]]:
     if not isinstance(x, Tensor):
         x = float(x)
-        _need(math.isfinite(x) and (x > 0.0 or not positive), ValueError, f"{name} must be {'positive and ' if positive else ''}finite, got {x}")
+        _need(math.isfinite(x) and abs(x) < 2.0 ** 128 and (x >= 2.0 ** -126 or not positive), ValueError,
+              f"{name} must be {'positive and ' if positive else ''}finite in float32, got {x}")
         return x, None
     _need(not (torch.is_grad_enabled() and x.requires_grad), NotImplementedError, f"gradients with respect to {name} are not implemented: detach it")
     _need(x.device == device, RuntimeError, f"{name} is on {x.device}, the logits on {device}")
@@ -266,7 +267,7 @@ def process_logits(logits: Tensor, *, tokens: Optional[Tensor] = None, lengths: 
     its first ``lengths`` tokens (shape of the logits without the last dim; may be left out for one decoding step: all of them).  For the
     logits of a rollout that is what had been seen when the row's token was picked.  ``prompt_lengths`` ``[*B]``: where the
     presence and frequency penalties begin to count (0: at the start); the repetition penalty counts the prompt too.  Penalties and temperature are
-    numbers or tensors that broadcast to ``[*B]``.  ``bias`` broadcasts to the logits.  ``mask`` broadcasts to the logits too: truth values, or
+    numbers or tensors that broadcast to ``[*B]`` (tensors are not read on the host: repetition penalties and temperatures in them have to be positive).  ``bias`` broadcasts to the logits.  ``mask`` broadcasts to the logits too: truth values, or
     bits of int32 words ``[..., ceil(V / 32)]`` (token j: bit ``j % 32`` of word ``j // 32``); what the logits hold in masked places does not matter.
 
     Differentiable in ``logits``; masked places get no gradient.  ``out`` (not under autograd) may be ``logits`` itself."""
