@@ -192,6 +192,12 @@ __device__ __forceinline__ i64 scalar(int64_t v) { return scalar((i64)v); }
 template <typename P>
 __device__ __forceinline__ P *scalar(P *p) { return (P *)scalar((i64)p); }
 
+// the same value, as far as the compiler knows a new one
+__device__ __forceinline__ int again(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // What a lane knows of row t0 + lane before the block's rows begin: a row's scalars are then one v_readlane away, not a memory latency.
 struct RowAhead {
     int want = 0;    // PEN: length of the history
@@ -246,11 +252,10 @@ __device__ __forceinline__ void join_row(const TokenArgs &a, i64 r, i64 y, const
     }
 }
 
-// Waves of a block (the launch picks up to that many): a bias in registers beside the counts leaves room for three waves a SIMD.
-template <int MODE, bool PEN, bool BIAS> constexpr int kMostWaves = !PEN || (BIAS && MODE != kProcess) ? 4 : 16;
+template <bool PEN> constexpr int kMostWaves = PEN ? 16 : 4;  // of a block: the launch picks up to that many
 
 template <typename T, int MODE, bool PEN, bool BIAS>
-__global__ __launch_bounds__((kMostWaves<MODE, PEN, BIAS>) * kWave, PEN && BIAS && MODE != kProcess ? 3 : 4) void token_kernel(TokenArgs a) {
+__global__ __launch_bounds__(kMostWaves<PEN> * kWave, 4) void token_kernel(TokenArgs a) {
     extern __shared__ __align__(16) u32 lds_counts[];  // PEN: a sub-slice a wave
     const int W = blockDim.x / kWave;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -394,6 +399,7 @@ __global__ __launch_bounds__((kMostWaves<MODE, PEN, BIAS>) * kWave, PEN && BIAS 
     float4 *part_next = scalar((float4 *)a.partials + r0 * a.nsubs + lo / kSub);
     float *z_action = scalar(a.z_action + r0);
 
+    const int lane0 = lane;
     // FULL: every token of the sub-slice exists
     auto run_rows = [&](auto full) {
         constexpr bool FULL = decltype(full)::value;
@@ -401,7 +407,7 @@ __global__ __launch_bounds__((kMostWaves<MODE, PEN, BIAS>) * kWave, PEN && BIAS 
         u32 next_bits[kRowVecs];
 #pragma unroll
         for (int k = 0; k < kRowVecs; ++k) {
-            off[k] = k * kBlk + lane * kVec;
+            off[k] = k * kBlk + lane0 * kVec;
             nv[k] = FULL || left - off[k] > kVec ? kVec : left < off[k] ? 0 : (int)(left - off[k]);
             next_bits[k] = mask_bits(mask_kind, mask_next, off[k], nv[k]);
         }
@@ -413,6 +419,12 @@ __global__ __launch_bounds__((kMostWaves<MODE, PEN, BIAS>) * kWave, PEN && BIAS 
             }
         }
         for (int i_row = 0; i_row < rows; ++i_row) {
+            const int lane = again(lane0);  // what follows from it is cheaper to compute in each row than to keep
+#pragma unroll
+            for (int k = 0; k < kRowVecs; ++k) {
+                off[k] = k * kBlk + lane * kVec;
+                nv[k] = FULL || left - off[k] > kVec ? kVec : left < off[k] ? 0 : (int)(left - off[k]);
+            }
             u32 bits[kRowVecs];
             bool live[kRowVecs];  // of the wave
 #pragma unroll
@@ -627,7 +639,7 @@ template <typename T, int MODE, bool PEN, bool BIAS>
 int launch_waves(hipStream_t s, TokenArgs &a) {
     a.nsubs = token_subs(a.V);
     const i64 rows = a.B * a.T;
-    i64 most = kMostWaves<MODE, PEN, BIAS>;
+    i64 most = kMostWaves<PEN>;
     if (most > 8) {
         const i64 blocks = (a.nsubs + most - 1) / most * rows;
         if (blocks < 1024 || (a.L < 2048 && blocks < 4096)) most = 8;
