@@ -15,6 +15,14 @@
 //            relative to M = max * c as rounded, so that M's rounding cancels between the numerator and the sum.  It has to stay small
 //            in the exponent for that, so rows with a maximum of 2^20 or more in magnitude (rows of the type's lowest value among
 //            them) subtract first: d = (z - max) * c.  Everything is held in 32 bits.
+// Measured at 8192 x 131072 bf16 (2.15 GB of logits; a large copy reaches 4.75 TB/s here, reading alone 3.7), us:
+//                                    nothing on   mask of 3 in 4   history of 1024   both and a bias
+//   log-probability and entropy         469            434               609              541         4.6 TB/s, 3.5 with a history
+//   their gradient                      872            804               879              800         4.9 TB/s
+//   processed logits                    862            775               856              770         5.0 TB/s
+// HBM bounds all but the first row's two columns with a history: there the vector units do, with the repeated places' factors beside the
+// softmax.  One decoding step of 256 x 131072 with 4096 tokens of history takes 35 us (4.2 TB/s; reading and counting 4 MB of history 32
+// times, once a slice, is what it has beside its 147 MB), one of 8 x 32000 7 us (the history's latency, then the row's).
 #include "token_common.h"
 #include "vec8.h"
 
@@ -624,7 +632,8 @@ __global__ __launch_bounds__(kMostWaves<PEN> * kWave, 4) void token_kernel(Token
     else run_rows(Bool<false>());
 }
 
-// Rows of many blocks: one wave a row.
+// One wave a row: 16 bytes a sub-slice to read, so a launch's latency bounds it (2.2 us for 4 rows, 5 us for 8192 of 64 sub-slices).  A
+// last-block join inside the row kernel would save it but costs that kernel an atomic, a fence and registers a row; it measured slower.
 __global__ __launch_bounds__(256) void token_join_kernel(TokenArgs a) {
     const i64 r = (i64)blockIdx.x * 4 + threadIdx.x / kWave;
     if (r >= a.B * a.T) return;
@@ -634,7 +643,8 @@ __global__ __launch_bounds__(256) void token_join_kernel(TokenArgs a) {
 
 // Blocks of as many waves as an even split of the vocabulary gives them, up to 8 beside a history: two such blocks share a compute unit,
 // and one streams while the other counts.  Up to 16, one block a unit, where the counting is shared by enough: long histories, or runs of
-// many rows (256 x 131072 bf16, 4096 tokens: 37 us and 40; 8192 x 131072, backward: 795 and 830; but 910 x 50263 fp32: 117 and 103).
+// many rows (16 waves and 8: 256 x 131072 bf16 with 4096 tokens 35 us and 37; 8192 x 131072 bf16 with every step on, backward, 800 and 852,
+// forward 534 and 568; but 910 x 50263 fp32 with gradient 165 and 158).
 template <typename T, int MODE, bool PEN, bool BIAS>
 int launch_waves(hipStream_t s, TokenArgs &a) {
     a.nsubs = token_subs(a.V);
