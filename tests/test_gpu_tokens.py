@@ -3,6 +3,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad as fwAD
 
 import token_oracle as O
 from torchrl_amd.objectives.value import CheckpointedLinear, RolloutData, TokenActor, VTrace, functional as F, process_logits, token_log_prob
@@ -443,3 +444,21 @@ def test_autograd_manners(route, monkeypatch):
         leaf.add_(1.0)
     out.sum().backward()
     assert torch.equal(leaf.grad != 0, kw["mask"])
+
+
+def test_function_transforms_and_forward_mode_are_refused():
+    """Their derivatives are not there: an error, not a result without them."""
+    z, action = torch.randn(4, 130, device="cuda"), torch.arange(4, device="cuda")
+    for f in (lambda z: process_logits(z, temperature=2.0).sum(), lambda z: token_log_prob(z, action).sum()):
+        with pytest.raises(RuntimeError):
+            torch.func.grad(f)(z)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(z.expand(3, 4, 130))
+        with fwAD.dual_level(), pytest.raises(NotImplementedError):
+            f(fwAD.make_dual(z, torch.ones_like(z)))
+        with fwAD.dual_level():
+            assert torch.equal(f(z), f(z.clone()))
+    with fwAD.dual_level(), pytest.raises(NotImplementedError):
+        process_logits(z, bias=fwAD.make_dual(z[0].clone(), z[1].clone()))
+    with fwAD.dual_level(), pytest.raises(NotImplementedError):
+        process_logits(z, temperature=fwAD.make_dual(torch.ones(4, device="cuda"), torch.ones(4, device="cuda")))

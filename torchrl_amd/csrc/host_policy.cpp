@@ -54,12 +54,16 @@ void check_status(int rc, const char *what) {
     TORCH_CHECK(rc == 0, "torchrl_amd native call failed (status ", rc, "): ", g_last_error ? g_last_error() : what);
 }
 bool wants_grad(const at::Tensor &t) { return t.defined() && t.requires_grad() && c10::GradMode::is_enabled(); }
-bool optional_tensor(PyObject *o, at::Tensor &t) {
-    if (o == Py_None) return true;
+// a tensor with memory of its own kind: no function transform's or subclass's wrapper, no forward-mode tangent
+bool plain_tensor(PyObject *o, at::Tensor &t) {
     if (!THPVariable_Check(o)) return false;
     t = THPVariable_Unpack(o);
-    return true;
+    using c10::DispatchKey;
+    constexpr c10::DispatchKeySet wrapped({DispatchKey::FuncTorchGradWrapper, DispatchKey::FuncTorchBatched, DispatchKey::Functionalize, DispatchKey::Python,
+                                           DispatchKey::Negative, DispatchKey::ZeroTensor});
+    return !t.key_set().has_any(wrapped) && !t._fw_grad(0).defined();
 }
+bool optional_tensor(PyObject *o, at::Tensor &t) { return o == Py_None || plain_tensor(o, t); }
 bool number(PyObject *o, bool positive, float &out) {
     double x;
     if (PyFloat_CheckExact(o)) x = PyFloat_AS_DOUBLE(o);
@@ -110,8 +114,7 @@ struct Processing {
 
     // o: tokens, lengths, prompt_lengths, repetition, presence, frequency, bias, mask, temperature; false: not a fast-path call
     bool parse(PyObject *z, PyObject *const *o) {
-        if (!THPVariable_Check(z)) return false;
-        logits = THPVariable_Unpack(z);
+        if (!plain_tensor(z, logits)) return false;
         const int64_t nd = logits.dim();
         a.dtype = dtype_code(logits.scalar_type());
         if (nd < 2 || nd > 3 || a.dtype < 0 || !on_current_device(logits) || logits.numel() == 0 || logits.stride(-1) != 1) return false;
@@ -371,8 +374,8 @@ PyObject *py_token_log_prob(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     if (!count_ok(nargs, 12, "token_log_prob")) return nullptr;
     Processing p;
-    if (!THPVariable_Check(o[1]) || !p.parse(o[0], o + 3)) Py_RETURN_NONE;
-    const at::Tensor action = THPVariable_Unpack(o[1]);
+    at::Tensor action;
+    if (!plain_tensor(o[1], action) || !p.parse(o[0], o + 3)) Py_RETURN_NONE;
     const bool want_entropy = o[2] == Py_True, grad = wants_grad(p.logits);
     if (!is_int(action) || action.device() != p.logits.device() || action.sizes() != p.logits.sizes().slice(0, p.logits.dim() - 1) || !action.is_contiguous())
         Py_RETURN_NONE;
@@ -418,10 +421,8 @@ PyObject *py_token_log_prob(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
 PyObject *py_checkpointed_linear(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     if (!count_ok(nargs, 3, "checkpointed_linear")) return nullptr;
-    if (!THPVariable_Check(o[0]) || !THPVariable_Check(o[1])) Py_RETURN_NONE;
-    const at::Tensor x = THPVariable_Unpack(o[0]), w = THPVariable_Unpack(o[1]);
-    at::Tensor b;
-    if (!optional_tensor(o[2], b)) Py_RETURN_NONE;
+    at::Tensor x, w, b;
+    if (!plain_tensor(o[0], x) || !plain_tensor(o[1], w) || !optional_tensor(o[2], b)) Py_RETURN_NONE;
     const auto dt = x.scalar_type();
     if (dtype_code(dt) < 0 || !on_current_device(x) || x.numel() == 0 || x.dim() < 1 || w.dim() != 2 || w.numel() == 0 || w.size(1) != x.size(-1) ||
         w.scalar_type() != dt || w.device() != x.device())
@@ -458,8 +459,8 @@ PyObject *py_checkpointed_linear(PyObject *, PyObject *const *o, Py_ssize_t narg
 PyObject *py_quantize(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     if (!count_ok(nargs, 1, "quantize")) return nullptr;
-    if (!THPVariable_Check(o[0])) Py_RETURN_NONE;
-    const at::Tensor &x = THPVariable_Unpack(o[0]);
+    at::Tensor x;
+    if (!plain_tensor(o[0], x)) Py_RETURN_NONE;
     if (dtype_code(x.scalar_type()) < 0 || !on_current_device(x) || x.numel() == 0 || x.dim() < 1) Py_RETURN_NONE;
     c10::AutoGradMode off(false);
     at::Tensor codes, exponents;
@@ -476,8 +477,8 @@ PyObject *py_quantize(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
 PyObject *py_dequantize(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     if (!count_ok(nargs, 4, "dequantize")) return nullptr;
-    if (!THPVariable_Check(o[0]) || !THPVariable_Check(o[1])) Py_RETURN_NONE;
-    const at::Tensor &codes = THPVariable_Unpack(o[0]), &exponents = THPVariable_Unpack(o[1]);
+    at::Tensor codes, exponents;
+    if (!plain_tensor(o[0], codes) || !plain_tensor(o[1], exponents)) Py_RETURN_NONE;
     const int64_t D = PyLong_AsLongLong(o[2]);
     const int code = (int)PyLong_AsLong(o[3]);
     if (PyErr_Occurred()) return nullptr;

@@ -16,10 +16,11 @@
 //            in the exponent for that, so rows with a maximum of 2^20 or more in magnitude (rows of the type's lowest value among
 //            them) subtract first: d = (z - max) * c.  Everything is held in 32 bits.
 // Measured at 8192 x 131072 bf16 (2.15 GB of logits; a large copy reaches 4.75 TB/s here, reading alone 3.7), us:
-//                                    nothing on   mask of 3 in 4   history of 1024   both and a bias
-//   log-probability and entropy         469            434               609              541         4.6 TB/s, 3.5 with a history
-//   their gradient                      872            804               879              800         4.9 TB/s
-//   processed logits                    862            775               856              770         5.0 TB/s
+// (of 10 rows the mask leaves 4 whole, allows 3 every second token and 3 one in a hundred)
+//                                    nothing on   a mask   a history of 1024   both and a bias
+//   log-probability and entropy         469         434            609               541         4.6 TB/s, 3.5 with a history
+//   their gradient                      872         804            879               800         4.9 TB/s
+//   processed logits                    862         775            856               770         5.0 TB/s
 // HBM bounds all but the first row's two columns with a history: there the vector units do, with the repeated places' factors beside the
 // softmax.  One decoding step of 256 x 131072 with 4096 tokens of history takes 35 us (4.2 TB/s; reading and counting 4 MB of history 32
 // times, once a slice, is what it has beside its 147 MB), one of 8 x 32000 7 us (the history's latency, then the row's).

@@ -15,6 +15,7 @@ from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 from torch import nn, Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from torchrl_amd import _extension
@@ -150,6 +151,8 @@ def _processing(logits, tokens, lengths, prompt_lengths, repetition_penalty, pre
         n = V if mask.dtype == torch.bool else (V + 31) // 32
         _need(mask.ndim >= 1 and mask.shape[-1] == n, RuntimeError, f"a {mask.dtype} mask must have {n} entries in its last dim, got shape {tuple(mask.shape)}")
         mask = _rows_view(mask if steps else mask.unsqueeze(-2), batch, T, "mask")
+    for t, name in ((logits, "logits"), (bias, "bias"), *((s, "a penalty or the temperature") for s in (rep_t, pres_t, freq_t, temp_t))):
+        _need(t is None or forward_ad.unpack_dual(t).tangent is None, NotImplementedError, f"forward-mode derivatives with respect to {name} are not implemented")
     if logits.device.type != "cuda":
         raise RuntimeError(f"torchrl_amd token operators run on MI355X (HIP, device type 'cuda') tensors only; got a tensor on {logits.device}.")
     x = logits.detach()
