@@ -3,9 +3,10 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad as fwAD
 
 import token_oracle as O
-from torchrl_amd.objectives.value import CheckpointedLinear, checkpointed_linear, functional as F, quantize_activation
+from torchrl_amd.objectives.value import CheckpointedLinear, QuantizedActivation, checkpointed_linear, functional as F, quantize_activation
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -270,3 +271,26 @@ def test_no_tokens():
     assert y.shape == (0, 3)
     y.sum().backward()
     assert (w.grad == 0).all() and (b.grad == 0).all()
+
+
+def test_a_kept_activation_is_checked_before_it_is_read():
+    x = inputs(6, 70, torch.float32, seed=9).clamp(-50, 50).cuda()
+    q = quantize_activation(x)
+    want = q.dequantize()
+    apart = QuantizedActivation(q.codes.t().contiguous().t(), q.exponents.t().contiguous().t(), q.shape, q.dtype)  # another layout
+    assert torch.equal(apart.dequantize(), want)
+    for codes, exponents, shape in [(q.codes[:, :64], q.exponents, q.shape), (q.codes, q.exponents[:, :2], q.shape), (q.codes[:4], q.exponents[:4], q.shape),
+                                    (q.codes, q.exponents, torch.Size((6, 97))), (q.codes.int(), q.exponents, q.shape), (q.codes, q.exponents.int(), q.shape)]:
+        with pytest.raises(RuntimeError, match="do not hold"):
+            QuantizedActivation(codes, exponents, shape, q.dtype).dequantize()
+
+
+def test_function_transforms_and_forward_mode_are_refused():
+    """Their derivatives are not there: an error, not a result without them."""
+    x, w = torch.randn(5, 40, device="cuda"), torch.randn(3, 40, device="cuda")
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda x: checkpointed_linear(x, w).sum())(x)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda w: checkpointed_linear(x, w).sum())(w)
+    with fwAD.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        checkpointed_linear(fwAD.make_dual(x, torch.ones_like(x)), w.clone().requires_grad_())

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from torchrl_amd.objectives.value import CheckpointedLinear, process_logits, token_log_prob
+from torchrl_amd.objectives.value import CheckpointedLinear, process_logits, quantize_activation, token_log_prob
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +43,14 @@ def test_refusals_under_compile():
     bias = torch.zeros(20, device="cuda", requires_grad=True)
     with pytest.raises(Exception, match="bias"):
         torch.compile(lambda z: process_logits(z, bias=bias), fullgraph=True)(z)
+
+
+def test_kept_activations_compile_fullgraph():
+    x = torch.randn(3, 5, 70, device="cuda", dtype=torch.bfloat16)
+
+    def there_and_back(x):
+        q = quantize_activation(x)
+        return q.codes, q.exponents, q.dequantize(), q.dequantize(torch.float32)
+
+    for a, b in zip(there_and_back(x), torch.compile(there_and_back, fullgraph=True)(x)):
+        assert a.dtype == b.dtype and torch.equal(a, b)

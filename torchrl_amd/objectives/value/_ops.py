@@ -537,6 +537,17 @@ def _(x):
     return _kept_shapes(x)
 
 
+@torch.library.custom_op(f"{_NS}::dequantize_activation", mutates_args=())
+def dequantize_activation_op(codes: Tensor, exponents: Tensor, features: int, dtype: torch.dtype) -> Tensor:
+    from torchrl_amd.objectives.value import kept_activations as K
+    return K.QuantizedActivation(codes, exponents, torch.Size((*codes.shape[:-1], features)), dtype).dequantize()
+
+
+@dequantize_activation_op.register_fake
+def _(codes, exponents, features, dtype):
+    return torch.empty((*codes.shape[:-1], features), dtype=dtype, device=codes.device)
+
+
 @torch.library.custom_op(f"{_NS}::checkpointed_linear", mutates_args=())
 def checkpointed_linear_op(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
     from torchrl_amd.objectives.value import kept_activations as K

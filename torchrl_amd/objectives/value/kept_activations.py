@@ -80,15 +80,25 @@ class QuantizedActivation:
         dtype = self.dtype if dtype is None else dtype
         if dtype not in _DT:
             raise NotImplementedError(f"torchrl_amd 8-bit activations support float32, bfloat16 and float16, got {dtype}")
+        codes, exponents, lead, D = self.codes, self.exponents, tuple(self.shape[:-1]), self.shape[-1]
+        blocks = (D + BLOCK - 1) // BLOCK
+        if tuple(codes.shape) != (*lead, blocks * BLOCK) or tuple(exponents.shape) != (*lead, blocks) or codes.dtype != torch.int8 or \
+                exponents.dtype != torch.uint8 or codes.device != exponents.device:
+            raise RuntimeError(f"QuantizedActivation: codes {tuple(codes.shape)} {codes.dtype} and exponents {tuple(exponents.shape)} {exponents.dtype} "
+                               f"do not hold a tensor of shape {tuple(self.shape)}")
+        if torch.compiler.is_compiling():
+            from torchrl_amd.objectives.value import _ops
+            return _ops.dequantize_activation_op(codes, exponents, D, dtype)
         host = F._HOST if F._HOST_TRIED else F._host_module()
-        if host is not None and len(self.shape):
-            out = host.dequantize(self.codes, self.exponents, self.shape[-1], _DT[dtype])
+        if host is not None:
+            out = host.dequantize(codes, exponents, D, _DT[dtype])
             if out is not None:
                 return _done(out)
-        out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
+        _check_device(codes)
+        out = torch.empty(self.shape, dtype=dtype, device=codes.device)
         if out.numel():
-            D = self.shape[-1]
-            _call("trl_act_dequantize", out.device, _DT[dtype], self.codes.data_ptr(), self.exponents.data_ptr(), out.numel() // D, D, out.data_ptr())
+            codes, exponents = codes.contiguous(), exponents.contiguous()
+            _call("trl_act_dequantize", out.device, _DT[dtype], codes.data_ptr(), exponents.data_ptr(), out.numel() // D, D, out.data_ptr())
         return out
 
 
