@@ -522,7 +522,7 @@ typedef struct trl_token_args {
     const void *grad_out;                     /* trl_process_logits_bwd: (B, T, V) dense */
     const void *action;                       /* (B, T) dense; negative: a padded row */
     float *log_prob, *entropy;                /* (B, T); entropy may be NULL */
-    float *stats;                             /* (B, T, 2): {max z' * log2(e), log2 of the sum}; written by the forward call, read by the backward */
+    float *stats;                             /* (B, T, 2): {m = max z' * temp, log2 of the sum of exp(z' - m / temp)}: forward call writes, backward reads */
     const float *g_log_prob, *g_entropy;      /* (B, T) incoming gradients, either may be NULL (= zeros) */
 } trl_token_args;
 

@@ -294,3 +294,20 @@ def test_function_transforms_and_forward_mode_are_refused():
         torch.func.grad(lambda w: checkpointed_linear(x, w).sum())(w)
     with fwAD.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
         checkpointed_linear(fwAD.make_dual(x, torch.ones_like(x)), w.clone().requires_grad_())
+
+
+def test_offsets_past_32_bits():
+    """Rows behind 2^31 elements and 2^32 bytes: the bits of the same rows alone."""
+    N, D = 40000, 65600
+    x = torch.randn(100, D, device="cuda", dtype=torch.bfloat16).repeat(N // 100, 1)
+    x[-3:] *= torch.rand(3, D, device="cuda").to(x.dtype)
+    q, few = quantize_activation(x), quantize_activation(x[-3:].clone())
+    assert torch.equal(q.codes[-3:], few.codes) and torch.equal(q.exponents[-3:], few.exponents)
+    back = q.dequantize()
+    assert torch.equal(back[-3:], few.dequantize()) and torch.equal(back[:100], back[100:200])
+    del back, q
+    w = torch.zeros(2, D, device="cuda", dtype=x.dtype, requires_grad=True)
+    dy = torch.zeros(N, 2, device="cuda", dtype=x.dtype)
+    dy[-3] = torch.tensor([1.0, -2.0], device="cuda")  # one row alone: the sum has one term
+    (dw,) = torch.autograd.grad(checkpointed_linear(x, w), w, dy)
+    assert torch.equal(dw, dy[-3].unsqueeze(1) * few.dequantize()[0])

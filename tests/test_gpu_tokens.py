@@ -462,3 +462,49 @@ def test_function_transforms_and_forward_mode_are_refused():
         process_logits(z, bias=fwAD.make_dual(z[0].clone(), z[1].clone()))
     with fwAD.dual_level(), pytest.raises(NotImplementedError):
         process_logits(z, temperature=fwAD.make_dual(torch.ones(4, device="cuda"), torch.ones(4, device="cuda")))
+
+
+def test_offsets_past_32_bits():
+    """Rows that begin behind 2^32 bytes (and 2^31 elements) of logits, gradients, masks and histories: the bits of the same rows alone."""
+    B, V, last = 18000, 131072, slice(17990, 18000)
+    z = torch.randn(10, V, device="cuda", dtype=torch.bfloat16).repeat(B // 10, 1)
+    z[last] = torch.randn(10, V, device="cuda")
+    mask = torch.ones(B, V, dtype=torch.bool, device="cuda")
+    mask[last, ::3] = False
+    action = torch.arange(B, device="cuda") % V * 7 % V // 3 * 3 + 1
+    kw = dict(temperature=0.7)
+    leaf = z.requires_grad_()
+    lp, H = token_log_prob(leaf, action, entropy=True, mask=mask, **kw)
+    out = process_logits(leaf.detach(), mask=mask, **kw)
+    (d,) = torch.autograd.grad((lp, H), leaf, (torch.ones_like(lp), torch.ones_like(H)))
+    few = z.detach()[last].clone().requires_grad_()
+    lp1, H1 = token_log_prob(few, action[last], entropy=True, mask=mask[last].clone(), **kw)
+    (d1,) = torch.autograd.grad((lp1, H1), few, (torch.ones_like(lp1), torch.ones_like(H1)))
+    assert torch.equal(lp[last], lp1) and torch.equal(H[last], H1) and torch.equal(d[last], d1)
+    assert torch.equal(out[last], process_logits(few.detach(), mask=mask[last].clone(), **kw))
+    assert torch.equal(out[:10], out[10:20]) and torch.equal(out[:10], out[-20:-10])
+    del z, mask, leaf, lp, H, out, d
+
+    B, L, V = 600, 1 << 20, 500  # 5 GB of history
+    tokens = torch.randint(0, V, (B, L), device="cuda")
+    tokens[-1] = 3
+    z = torch.randn(B, V, device="cuda")
+    got = process_logits(z, tokens=tokens, frequency_penalty=0.5, prompt_lengths=torch.full((B,), 7, device="cuda"))
+    want = z[-1].clone()
+    want[3] -= 0.5 * (L - 7)
+    assert torch.equal(got[-1], want)
+    n = torch.zeros(V, device="cuda").index_add_(0, tokens[-2, 7:], torch.ones(L - 7, device="cuda"))
+    torch.testing.assert_close(got[-2], z[-2] - 0.5 * n, rtol=2 ** -22, atol=2 ** -22)  # two roundings, of the product and the difference
+
+
+def test_wide_strides():
+    """Sequences that lie more than 2^31 elements apart in one buffer, read and written in place."""
+    far = torch.zeros((1 << 31) + 70000, dtype=torch.float16, device="cuda")
+    z = far.as_strided((2, 3, 1000), (1 << 31, 20000, 1))
+    z.copy_(torch.randn(2, 3, 1000, generator=torch.Generator().manual_seed(1)).cuda())
+    mask = torch.rand(2, 3, 1000, generator=torch.Generator().manual_seed(2)).cuda() < 0.7
+    want = process_logits(z.contiguous(), temperature=2.0, mask=mask)
+    assert torch.equal(process_logits(z, temperature=2.0, mask=mask), want)
+    process_logits(z, temperature=2.0, mask=mask, out=z)
+    assert torch.equal(z, want)
+    assert torch.count_nonzero(far) == torch.count_nonzero(want)  # what lies between the rows is as it was
