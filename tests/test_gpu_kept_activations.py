@@ -311,3 +311,63 @@ def test_offsets_past_32_bits():
     dy[-3] = torch.tensor([1.0, -2.0], device="cuda")  # one row alone: the sum has one term
     (dw,) = torch.autograd.grad(checkpointed_linear(x, w), w, dy)
     assert torch.equal(dw, dy[-3].unsqueeze(1) * few.dequantize()[0])
+
+
+@pytest.mark.parametrize("route", ["host", "python"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,D", [(1, 1), (1, 700), (3, 5), (67, 64), (130, 511), (129, 513), (1000, 1000), (300, 4099), (2049, 1536), (5000, 40), (2, 65537)])
+def test_one_output(route, dtype, N, D, monkeypatch):
+    """A value head: one pass over x forward, one over what is kept backward."""
+    if route == "python":
+        assert F.host_fast_path()
+        monkeypatch.setattr(F, "_HOST", None)
+    g = torch.Generator().manual_seed(N + D)
+    x = inputs(N, D, dtype, seed=N + D).clamp(-100, 100)
+    w, b, dy = (torch.randn(s, generator=g).to(dtype) for s in ((1, D), (1,), (N, 1)))
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b)]
+    y = checkpointed_linear(*leaves)
+    if D <= 65536:
+        assert F.last_kernel() == "act_head"
+    # fp32 sums: a lane adds 8 products of every 512, then 7 additions over the lanes and the bias; the library's own sum above that width
+    terms = (8 * -(-D // 512) if D <= 65536 else D) + 8
+    X, W = x.double(), w.double()
+    largest = torch.finfo(dtype).max * (1 + torch.finfo(dtype).eps / 4)  # half a step above the last number a rounding is infinite (fp16's 65520)
+    want = X @ W.T + b.double()
+    want = torch.where(want.abs() < largest, want, want * math.inf)
+    O.assert_close(y.detach(), want, terms * O.U * (X.abs() @ W.abs().T + b.double().abs()), "y")
+    dx, dw, db = torch.autograd.grad(y, leaves, dy.cuda())
+    assert torch.equal(dx.cpu(), (dy.float() * w.float()).to(dtype))  # one product, one rounding
+    kept = O.kept(x)[2]
+    O.assert_close(dw, dy.double().T @ kept, bound(dy.double(), kept), "dw")
+    O.assert_close(db, dy.double().sum(0), (N + 1) * O.U * dy.double().abs().sum(0), "db")
+    x2, w2 = leaves[0].detach(), w.cuda().requires_grad_()
+    y2 = checkpointed_linear(x2, w2, leaves[2].detach())
+    (dw2,) = torch.autograd.grad(y2, w2, dy.cuda())
+    assert torch.equal(y2, y) and torch.equal(dw2, dw)
+    x3 = leaves[0].detach().clone().requires_grad_()
+    (dx3,) = torch.autograd.grad(checkpointed_linear(x3, w.cuda()), x3, dy.cuda())  # the weight is frozen
+    O.assert_close(dx3, dy.double() @ W, 0.0, "dx alone")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_output_layouts_and_non_finite(dtype):
+    g = torch.Generator().manual_seed(1)
+    big = torch.randn(4, 9, 2 * 133, generator=g).to(dtype).cuda()
+    x, w = big[..., 1:134], torch.randn(133, 2, generator=g).to(dtype).cuda()[:, 0].unsqueeze(0).requires_grad_()  # rows at odd places, a strided weight
+    b = torch.zeros(1, dtype=dtype, device="cuda", requires_grad=True)
+    leaf = x.detach().requires_grad_()
+    y = checkpointed_linear(leaf, w, b)
+    dy = torch.ones(1, 1, 1, dtype=dtype, device="cuda").expand(4, 9, 1)
+    got = torch.autograd.grad(y, (leaf, w, b), dy)
+    plain = x.contiguous().requires_grad_()
+    dense = w.detach().contiguous().requires_grad_()
+    y2 = checkpointed_linear(plain, dense, b)
+    assert torch.equal(y, y2) and y.shape == (4, 9, 1)
+    for a, e in zip(got, torch.autograd.grad(y2, (plain, dense, b), dy.contiguous())):
+        assert torch.equal(a, e)
+    bad = x.clone()
+    bad[0, 0, 40], bad[1, 2, 3] = math.nan, math.inf
+    y3 = checkpointed_linear(bad, dense)
+    assert y3[0, 0, 0].isnan() and not y3[1, 2, 0].isfinite() and torch.isfinite(y3).sum() == 34
+    (dw,) = torch.autograd.grad(y3, dense, dy)
+    assert dw[0, 32:64].isnan().all() and dw[0, :32].isnan().all() and torch.isfinite(dw[0, 64:]).all()  # whole blocks stand for NaN

@@ -54,3 +54,19 @@ def test_kept_activations_compile_fullgraph():
 
     for a, b in zip(there_and_back(x), torch.compile(there_and_back, fullgraph=True)(x)):
         assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_a_value_head_compiles_fullgraph():
+    torch.manual_seed(0)
+    x, dy = torch.randn(3, 50, 200, device="cuda"), torch.randn(3, 50, 1, device="cuda")
+    head = CheckpointedLinear(200, 1, device="cuda")
+
+    def run(fn):
+        leaf = x.clone().requires_grad_()
+        head.zero_grad()
+        y = fn(leaf)
+        y.backward(dy)
+        return y.detach(), leaf.grad, head.weight.grad.clone(), head.bias.grad.clone()
+
+    for a, b in zip(run(head), run(torch.compile(head, fullgraph=True))):
+        assert torch.equal(a, b)

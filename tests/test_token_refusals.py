@@ -139,6 +139,12 @@ def test_c_entry_points_refuse_more():
     need = lib.trl_act_weight_grad_workspace_bytes(2, 100000, 4, 32)
     if need:
         assert lib.trl_act_weight_grad(None, 2, 64, 8, 64, 64, 100000, 4, 32, 64, None, 64, need - 1) == 3
+    assert lib.trl_act_head_fwd(None, 0, None, 8, 4, 8, 64, None, 64, 64, 64) == 1 and lib.trl_act_head_fwd(None, 0, 64, 8, 4, 8, 64, None, 72, 64, 64) == 1
+    assert lib.trl_act_head_fwd(None, 1, 64, 8, 4, 8, 64, None, 64, 64, 64) == 1 and lib.trl_act_head_fwd(None, 0, None, 8, 0, 8, None, None, None, None, None) == 0
+    assert lib.trl_act_head_bwd(None, 0, 64, 1, 64, 64, 4, 8, None, 64, None, 64, 64, 1 << 30) == 1  # dx without w
+    assert lib.trl_act_head_bwd(None, 0, 64, 1, 64, 64, 4, 8, 64, None, None, 64, 64, 1 << 30) == 1  # no dw
+    need = lib.trl_act_weight_grad_workspace_bytes(0, 100000, 1, 32)
+    assert need and lib.trl_act_head_bwd(None, 0, 64, 1, 64, 64, 100000, 32, 64, 64, None, 64, 64, need - 1) == 3
 
 
 # ---- the oracle's known answers -----------------------------------------------------------------------------------------------

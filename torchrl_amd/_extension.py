@@ -113,6 +113,8 @@ _PROTOTYPES = {
     "trl_act_dequantize": (_int, [_vp, _int, _vp, _vp, _i64, _i64, _vp]),
     "trl_act_weight_grad_workspace_bytes": (_sz, [_int, _i64, _i64, _i64]),
     "trl_act_weight_grad": (_int, [_vp, _int, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _sz]),
+    "trl_act_head_fwd": (_int, [_vp, _int, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "trl_act_head_bwd": (_int, [_vp, _int, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _sz]),
     # host entry points (tensors in host memory)
     "trl_cpu_threads": (_int, []),
     "trl_set_cpu_threads": (_int, [_int]),

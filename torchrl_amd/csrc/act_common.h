@@ -10,4 +10,5 @@ void launch_act_dequantize(hipStream_t s, int dtype, const int8_t *codes, const 
 size_t act_weight_grad_workspace(int dtype, i64 N, i64 O, i64 D);
 // 0, or 2 where the grid would pass its limit
 int launch_act_weight_grad(hipStream_t s, int dtype, const void *dy, i64 dy_stride, const int8_t *codes, const u8 *exponents, i64 N, i64 O,
-                           i64 D, void *dw, void *db, void *workspace);
+                           i64 D, void *dw, void *db, void *workspace, const void *w = nullptr, void *dx = nullptr);
+void launch_act_head(hipStream_t s, int dtype, const void *x, i64 stride, i64 N, i64 D, const void *w, const void *bias, int8_t *codes, u8 *exponents, void *y);

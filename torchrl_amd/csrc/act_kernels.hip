@@ -7,6 +7,14 @@ namespace {
 
 constexpr int kGroups = kActBlock / kVec;  // 4 lanes hold a block
 
+__device__ __forceinline__ float wave_sum(float x) {
+    x += dpp_mov<0xB1>(x);
+    x += dpp_mov<0x4E>(x);
+    x += dpp_mov<0x141>(x);
+    x += dpp_mov<0x140>(x);
+    return (read_lane(x, 0) + read_lane(x, 16)) + (read_lane(x, 32) + read_lane(x, 48));
+}
+
 // Thread -> (row, group of 8 features) over N rows of G groups; one 64-bit division a block of threads.
 __device__ __forceinline__ bool row_and_group(i64 N, u32 G, i64 &row, u32 &group) {
     const i64 first = (i64)blockIdx.x * blockDim.x;
@@ -19,17 +27,8 @@ __device__ __forceinline__ bool row_and_group(i64 N, u32 G, i64 &row, u32 &group
 
 // Bound by HBM: 2 bytes in and 1 + 1/32 out an element at 16 bits.  Four lanes hold a block of 32, so its largest magnitude is two
 // DPP steps; magnitudes are compared as integers, which puts NaN above infinity above every number.  16384 x 8192 bf16: 82 us, 4.9 TB/s.
-template <typename T>
-__global__ __launch_bounds__(256) void act_quantize_kernel(const T *x, i64 stride, i64 N, i64 D, u32 G, int8_t *codes, u8 *exponents) {
-    i64 row;
-    u32 group;
-    if (!row_and_group(N, G, row, group)) return;  // whole blocks of 32 leave together
-    const i64 col = (i64)group * kVec, left = D - col;
-    Raw8<T> r{};
-    const int n = left >= kVec ? kVec : left < 0 ? 0 : (int)left;
-    if (n > 0) load8(x + row * stride + col, n, r);
-    float v[kVec];
-    unpack8(r, v);
+// 8 values of a lane to their place `at` (in groups of 8) among the codes; the four lanes of a block call together
+__device__ __forceinline__ void quantize8(const float *v, i64 at, int8_t *codes, u8 *exponents) {
     int top = 0;
 #pragma unroll
     for (int i = 0; i < kVec; ++i) top = max(top, __builtin_bit_cast(int, v[i]) & 0x7fffffff);
@@ -46,8 +45,64 @@ __global__ __launch_bounds__(256) void act_quantize_kernel(const T *x, i64 strid
             w[i / 4] |= (u32)(q & 0xff) << (8 * (i % 4));
         }
     }
-    *(uint2 *)(codes + (row * G + group) * kVec) = make_uint2(w[0], w[1]);
-    if ((group & (kGroups - 1)) == 0) exponents[(row * G + group) / kGroups] = (u8)(broken ? 255 : e);
+    *(uint2 *)(codes + at * kVec) = make_uint2(w[0], w[1]);
+    if ((at & (kGroups - 1)) == 0) exponents[at / kGroups] = (u8)(broken ? 255 : e);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void act_quantize_kernel(const T *x, i64 stride, i64 N, i64 D, u32 G, int8_t *codes, u8 *exponents) {
+    i64 row;
+    u32 group;
+    if (!row_and_group(N, G, row, group)) return;  // whole blocks of 32 leave together
+    const i64 col = (i64)group * kVec, left = D - col;
+    Raw8<T> r{};
+    const int n = left >= kVec ? kVec : left < 0 ? 0 : (int)left;
+    if (n > 0) load8(x + row * stride + col, n, r);
+    float v[kVec];
+    unpack8(r, v);
+    quantize8(v, row * G + group, codes, exponents);
+}
+
+// The forward pass of one output (a value head) while its input is quantized: y = x w + b on the way, one read of x.  A wave a row, 512
+// features at a time with the next ones on their way; w comes from the caches (two or four rows a wave read it less often, but hide less of
+// the latency: 8192 x 4096 bf16 18.7 us and 22.4 / 24.4).  Bound by HBM as the quantization alone: 5.4 TB/s, 19.0 us without the product.
+template <typename T>
+__global__ __launch_bounds__(256) void act_head_kernel(const T *__restrict__ x, i64 stride, i64 N, i64 D, u32 G, const T *__restrict__ w, const T *__restrict__ bias,
+                                                       int8_t *__restrict__ codes, u8 *__restrict__ exponents, T *__restrict__ y) {
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const i64 row = (i64)blockIdx.x * 4 + wave;
+    if (row >= N) return;
+    const T *x_row = x + row * stride;
+    struct Piece { Raw8<T> x, w; } now, next;
+    auto fetch = [&](u32 group) {
+        const i64 col = (i64)group * kVec, left = D - col;
+        const int n = left >= kVec ? kVec : left < 0 ? 0 : (int)left;
+        Piece p{};
+        if (n > 0) {
+            load8(x_row + col, n, p.x);
+            load8(w + col, n, p.w);
+        }
+        return p;
+    };
+    float sum = 0.0f;
+    auto use = [&](u32 group, const Piece &p) {
+        if (group >= G) return;  // whole blocks of 32 leave together
+        float v[kVec], vw[kVec];
+        unpack8(p.x, v);
+        unpack8(p.w, vw);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) sum = fmaf(v[i], vw[i], sum);
+        quantize8(v, row * G + group, codes, exponents);
+    };
+    now = fetch(lane);
+    for (u32 g = 0; g < G; g += 2 * kWave) {
+        next = fetch(g + lane + kWave);
+        use(g + lane, now);
+        now = fetch(g + lane + 2 * kWave);
+        use(g + lane + kWave, next);
+    }
+    sum = wave_sum(sum) + (bias ? (float)bias[0] : 0.0f);
+    if (lane == 0) y[row] = (T)sum;
 }
 
 __device__ __forceinline__ float step_of(int e) { return e == 255 ? __builtin_nanf("") : __builtin_bit_cast(float, (u32)e << 23); }
@@ -79,11 +134,11 @@ __global__ __launch_bounds__(256) void act_dequantize_kernel(const int8_t *codes
 //   flow    Two LDS buffers.  While one is multiplied, the next tile goes from registers to the other in the second half of the step, and
 //           each register is loaded with the tile after that as soon as it is free: a load has a whole step to arrive, and the
 //           conversion runs in the shadow of the matrix instructions.
-//   splits  Few output tiles (value heads) split the tokens; the parts are 32 bits and are added in order by a second launch.
+//   splits  Few output tiles split the tokens; the parts are 32 bits and are added in order by a second launch.
 // Bound by the matrix units with a full chip: (8192, 8192)^T (8192, 2048) bf16 takes 255-295 us as the clocks allow, 930-1080 TFLOP/s (the
 // library's product of unquantized operands 291), fp32 8192 x 2048 x 2048 299 us (three products; 473).  A quarter of the chip or less is
-// bound by the head and tail of its blocks: 1111 x 515 x 1027 fp32 18 us and 4 to join; a value head of 4096 features over 8192 tokens is
-// one read of its 33 MB of codes, 16 us (2.2 TB/s: 64 tokens of a split are in flight) and 4 to join (the library's product: 31).
+// bound by the head and tail of its blocks: 1111 x 515 x 1027 fp32 18 us and 4 to join.  One output has a kernel
+// of its own below.
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -158,6 +213,8 @@ struct WeightGradArgs {
     void *dw, *db;       // one split: the outputs
     float *parts;        // more: (splits, O, D) and, behind them, (splits, O)
     int splits;
+    const void *w;       // one output alone: the weight and the gradient of the input, or NULL
+    void *dx;
 };
 
 template <typename T, int BM, int BN, int BK, int WM, int WN>
@@ -394,17 +451,100 @@ __global__ __launch_bounds__(WM *WN *kWave, BM == 256 ? 2 : 1) void act_weight_g
 }
 
 // Adds the parts of a split sum in order; bound by a launch's latency (4 us for 3 parts of 515 x 1027).
+constexpr int kJoinCols = 32, kJoinGroups = 8;
 template <typename T>
 __global__ __launch_bounds__(256) void act_join_kernel(const float *parts, int splits, i64 n_w, i64 n_b, T *dw, T *db) {
-    const i64 i = (i64)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n_w + n_b) return;
-    const bool w = i < n_w;
+    __shared__ float sums[kJoinGroups][kJoinCols];
+    const int col = threadIdx.x % kJoinCols, group = threadIdx.x / kJoinCols;
+    const i64 i = (i64)blockIdx.x * kJoinCols + col;
+    const bool in = i < n_w + n_b, w = i < n_w;
     const i64 n = w ? n_w : n_b, at = w ? i : i - n_w;
     const float *p = parts + (w ? 0 : splits * n_w) + at;
     float s = 0.0f;
+    if (in) {
 #pragma unroll 8
-    for (int k = 0; k < splits; ++k) s += p[k * n];
+        for (int k = group; k < splits; k += kJoinGroups) s += p[k * n];
+    }
+    sums[group][col] = s;
+    __syncthreads();
+    if (!in || group) return;
+#pragma unroll
+    for (int k = 1; k < kJoinGroups; ++k) s += sums[k][col];
     (w ? dw : db)[at] = (T)s;
+}
+
+// The backward pass of one output (a value head): dw is a column sum of x^ weighted by dy, one read of the codes, and dx = dy w is written
+// beside it.  A wave takes 512 columns, 8 a lane, and every 8th row of its split, kHeadRows at a time; dy of 64 rows lies in its lanes.
+// Products are exact in the fma.  Bound by HBM: 8192 x 4096 bf16 25 us with the join of 32 parts (4.0 TB/s), 15 without dx; 65536 x 1024
+// 36 us (5.6 TB/s).  8 and 16 rows at a time: 25.5 / 23.7 us, but 65536 x 1024 37.5 / 38.8 and 8192 x 16384 89 / 102 against 85.
+constexpr int kHeadRows = 4, kHeadWaves = 8, kHeadCols = kVec * kWave;
+template <typename T>
+__global__ __launch_bounds__(kHeadWaves * kWave) void act_head_grad_kernel(WeightGradArgs a) {
+    __shared__ float sums[kHeadWaves][kHeadCols + 1];
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const i64 d0 = (i64)(blockIdx.x % a.tiles) * kHeadCols + lane * kVec;
+    const int split = blockIdx.x / a.tiles;
+    const i64 n0 = split * a.part, n1 = n0 + a.part < a.N ? n0 + a.part : a.N;
+    const bool in = d0 < a.Dp;
+    const i64 left = a.D - d0;
+    const int n_dx = !a.dx ? 0 : left >= kVec ? kVec : left < 0 ? 0 : (int)left;
+    Raw8<T> rw{};
+    if (n_dx > 0) load8((const T *)a.w + d0, n_dx, rw);
+    float w[kVec], s[kVec] = {}, s_dy = 0.0f;
+    unpack8(rw, w);
+    for (i64 n = n0 + wave; n < n1; n += kHeadWaves * kWave) {
+        const i64 mine = n + lane * kHeadWaves;
+        const float dy = mine < n1 ? (float)((const T *)a.dy)[mine * a.dy_stride] : 0.0f;
+        s_dy += dy;
+        const i64 ahead = (n1 - n + kHeadWaves - 1) / kHeadWaves;
+        const int rows = ahead < kWave ? (int)ahead : kWave;
+        for (int k0 = 0; k0 < rows; k0 += kHeadRows) {
+            uint2 c[kHeadRows];
+            int e[kHeadRows];
+#pragma unroll
+            for (int k = 0; k < kHeadRows; ++k) {
+                c[k] = make_uint2(0, 0);
+                e[k] = 127;
+                const i64 at = (n + (i64)(k0 + k) * kHeadWaves) * a.Dp + d0;
+                if (k0 + k < rows && in) {
+                    c[k] = *(const uint2 *)(a.codes + at);
+                    e[k] = a.exponents[at / kActBlock];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kHeadRows; ++k) {
+                const float g = k0 + k < rows ? read_lane(dy, k0 + k) : 0.0f, step = step_of(e[k]);
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) s[i] = fmaf(g, (float)(int8_t)((i < 4 ? c[k].x : c[k].y) >> (8 * (i % 4))) * step, s[i]);
+                if (n_dx > 0 && k0 + k < rows) {
+                    float dx[kVec];
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) dx[i] = g * w[i];
+                    store8((T *)a.dx + (n + (i64)(k0 + k) * kHeadWaves) * a.D + d0, n_dx, dx);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) sums[wave][lane * kVec + i] = s[i];
+    s_dy = wave_sum(s_dy);
+    if (lane == 0) sums[wave][kHeadCols] = s_dy;
+    __syncthreads();
+    const i64 d = (i64)(blockIdx.x % a.tiles) * kHeadCols + threadIdx.x;
+    auto total = [&](int c) {
+        float t = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kHeadWaves; ++w) t += sums[w][c];
+        return t;
+    };
+    if (d < a.D) {
+        if (a.splits == 1) ((T *)a.dw)[d] = (T)total(threadIdx.x);
+        else a.parts[(i64)split * a.D + d] = total(threadIdx.x);
+    }
+    if (a.db && blockIdx.x % a.tiles == 0 && threadIdx.x == 0) {
+        if (a.splits == 1) ((T *)a.db)[0] = (T)total(kHeadCols);
+        else a.parts[(i64)a.splits * a.D + split] = total(kHeadCols);
+    }
 }
 
 // Column sums of dy alone: 32 groups of 8 columns a block, 8 rows at a time.
@@ -451,6 +591,13 @@ WeightGradPlan weight_grad_plan(int dtype, i64 N, i64 O, i64 D) {
         p.splits = (int)(N ? (N + p.part - 1) / p.part : 1);
         return p;
     }
+    if (O == 1) {  // a value head: enough blocks for the chip, 64 rows or more a split
+        p.tiles = (D + kHeadCols - 1) / kHeadCols;
+        const i64 want = (256 + p.tiles - 1) / p.tiles, most = (N + 63) / 64 > 0 ? (N + 63) / 64 : 1, s = want < most ? want : most;
+        p.part = (N + s - 1) / s + (N == 0);
+        p.splits = (int)(N ? (N + p.part - 1) / p.part : 1);
+        return p;
+    }
     struct Tile { int bm, bn, bk, slots; double clocks; };
     static const Tile low[] = {{256, 256, 64, 256, 77.0}, {128, 128, 64, 512, 52.0}, {32, 128, 64, 768, 55.0}};
     static const Tile f32[] = {{128, 128, 32, 512, 160.0}, {32, 128, 64, 512, 80.0}};
@@ -483,6 +630,7 @@ void launch_weight_grad(hipStream_t s, const WeightGradArgs &a) {
 template <typename T>
 void launch_weight_grad_t(hipStream_t s, const WeightGradArgs &a, const WeightGradPlan &p) {
     if (a.D == 0) hipLaunchKernelGGL(act_column_sum_kernel<T>, dim3((unsigned)(a.tiles * a.splits)), dim3(256), 0, s, a);
+    else if (a.O == 1) hipLaunchKernelGGL(act_head_grad_kernel<T>, dim3((unsigned)(a.tiles * a.splits)), dim3(kHeadWaves * kWave), 0, s, a);
     else if (p.bm == 32) launch_weight_grad<T, 32, 128, 64, 1, 4>(s, a);
     else if constexpr (sizeof(T) == 4) launch_weight_grad<T, 128, 128, 32, 2, 2>(s, a);
     else {
@@ -491,7 +639,7 @@ void launch_weight_grad_t(hipStream_t s, const WeightGradArgs &a, const WeightGr
     }
     if (a.splits > 1) {
         const i64 n_w = a.O * a.D, n_b = a.db ? a.O : 0;
-        hipLaunchKernelGGL(act_join_kernel<T>, dim3((unsigned)((n_w + n_b + 255) / 256)), dim3(256), 0, s, a.parts, a.splits, n_w, n_b, (T *)a.dw, (T *)a.db);
+        hipLaunchKernelGGL(act_join_kernel<T>, dim3((unsigned)((n_w + n_b + kJoinCols - 1) / kJoinCols)), dim3(256), 0, s, a.parts, a.splits, n_w, n_b, (T *)a.dw, (T *)a.db);
     }
 }
 
@@ -518,12 +666,24 @@ size_t act_weight_grad_workspace(int dtype, i64 N, i64 O, i64 D) {
     return p.splits > 1 ? (size_t)p.splits * (size_t)O * (size_t)(D + 1) * sizeof(float) : 0;  // parts of dw, then of db
 }
 
+void launch_act_head(hipStream_t s, int dtype, const void *x, i64 stride, i64 N, i64 D, const void *w, const void *bias, int8_t *codes, u8 *exponents, void *y) {
+    const u32 G = (u32)((D + kActBlock - 1) / kActBlock * kGroups);
+    const dim3 grid((unsigned)((N + 3) / 4));
+    auto launch = [&](auto t) {
+        typedef decltype(t) T;
+        hipLaunchKernelGGL(act_head_kernel<T>, grid, dim3(256), 0, s, (const T *)x, stride, N, D, G, (const T *)w, (const T *)bias, codes, exponents, (T *)y);
+    };
+    if (dtype == TRL_F32) launch(0.0f);
+    else if (dtype == TRL_BF16) launch((__bf16)0.0f);
+    else launch((_Float16)0.0f);
+}
+
 int launch_act_weight_grad(hipStream_t s, int dtype, const void *dy, i64 dy_stride, const int8_t *codes, const u8 *exponents, i64 N, i64 O,
-                           i64 D, void *dw, void *db, void *workspace) {
+                           i64 D, void *dw, void *db, void *workspace, const void *w, void *dx) {
     const WeightGradPlan p = weight_grad_plan(dtype, N, O, D);
-    if (p.tiles * p.splits > 0x7fffffffLL || (O * (D + 1) + 255) / 256 > 0x7fffffffLL) return 2;
+    if (p.tiles * p.splits > 0x7fffffffLL || (O * (D + 1) + kJoinCols - 1) / kJoinCols > 0x7fffffffLL) return 2;
     const WeightGradArgs a{dy, dy_stride, codes, exponents, N, O, D, (D + kActBlock - 1) / kActBlock * kActBlock, (int)p.tiles_d, (int)p.tiles, p.part, dw, db,
-                           (float *)workspace, p.splits};
+                           (float *)workspace, p.splits, w, dx};
     if (dtype == TRL_F32) launch_weight_grad_t<float>(s, a, p);
     else if (dtype == TRL_BF16) launch_weight_grad_t<__bf16>(s, a, p);
     else launch_weight_grad_t<_Float16>(s, a, p);

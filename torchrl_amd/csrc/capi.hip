@@ -900,6 +900,18 @@ int trl_act_quantize(void *stream, int dtype, const void *x, int64_t x_stride, i
     return TRL_OK;
 }
 
+int trl_act_head_fwd(void *stream, int dtype, const void *x, int64_t x_stride, int64_t N, int64_t D, const void *w, const void *bias, int8_t *codes,
+                     uint8_t *exponents, void *y) {
+    if (int rc = check_act_dims("trl_act_head_fwd", dtype, N, D)) return rc;
+    if (N == 0) return TRL_OK;
+    if (!x || !w || !y || !codes || !exponents || ((uintptr_t)codes & 15))
+        return fail(TRL_ERR_INVALID_ARGUMENT, "trl_act_head_fwd: null pointer, or codes not 16-byte aligned");
+    launch_act_head((hipStream_t)stream, dtype, x, x_stride, N, D, w, bias, codes, exponents, y);
+    if (int rc = check_launch("trl_act_head_fwd")) return rc;
+    g_kernel = "act_head";
+    return TRL_OK;
+}
+
 int trl_act_dequantize(void *stream, int dtype, const int8_t *codes, const uint8_t *exponents, int64_t N, int64_t D, void *out) {
     if (int rc = check_act_dims("trl_act_dequantize", dtype, N, D)) return rc;
     if (N == 0) return TRL_OK;
@@ -929,6 +941,21 @@ int trl_act_weight_grad(void *stream, int dtype, const void *dy, int64_t dy_stri
         return fail(TRL_ERR_UNSUPPORTED, "trl_act_weight_grad: too large for one launch");
     if (int rc = check_launch("trl_act_weight_grad")) return rc;
     g_kernel = dw ? "act_weight_grad" : "act_column_sum";
+    return TRL_OK;
+}
+
+int trl_act_head_bwd(void *stream, int dtype, const void *dy, int64_t dy_stride, const int8_t *codes, const uint8_t *exponents, int64_t N,
+                     int64_t D, const void *w, void *dw, void *db, void *dx, void *workspace, size_t workspace_bytes) {
+    if (int rc = check_act_dims("trl_act_head_bwd", dtype, N, D)) return rc;
+    if (!dw || (dx && !w) || (N > 0 && (!dy || !codes || !exponents || ((uintptr_t)codes & 15))))
+        return fail(TRL_ERR_INVALID_ARGUMENT, "trl_act_head_bwd: null pointer, or codes not 16-byte aligned");
+    const size_t need = trl_act_weight_grad_workspace_bytes(dtype, N, 1, D);
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
+        return fail(TRL_ERR_WORKSPACE, "trl_act_head_bwd: workspace is %zu bytes, need %zu (16-byte aligned)", workspace_bytes, need);
+    if (launch_act_weight_grad((hipStream_t)stream, dtype, dy, dy_stride, codes, exponents, N, 1, D, dw, db, workspace, w, dx))
+        return fail(TRL_ERR_UNSUPPORTED, "trl_act_head_bwd: too large for one launch");
+    if (int rc = check_launch("trl_act_head_bwd")) return rc;
+    g_kernel = "act_head_bwd";
     return TRL_OK;
 }
 

@@ -922,7 +922,8 @@ def _host_module():
                      _host_workspace, torch._C._cuda_getCurrentRawStream, _host_grouped_scratch)
             mod.init_policy(*(_extension.fn_address(getattr(lib, name)) for name in (
                 "trl_process_logits_fwd", "trl_process_logits_bwd", "trl_token_workspace_bytes", "trl_token_log_prob_fwd", "trl_token_log_prob_bwd",
-                "trl_act_quantize", "trl_act_dequantize", "trl_act_weight_grad_workspace_bytes", "trl_act_weight_grad", "trl_last_error")))
+                "trl_act_quantize", "trl_act_dequantize", "trl_act_weight_grad_workspace_bytes", "trl_act_weight_grad", "trl_act_head_fwd",
+                "trl_act_head_bwd", "trl_last_error")))
             for (di, st), ws in _WORKSPACES.items():
                 mod.set_workspace(di, st, ws.data_ptr(), ws.numel())
             from ... import _utils

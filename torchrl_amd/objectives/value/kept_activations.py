@@ -25,6 +25,7 @@ from torchrl_amd.objectives.value import functional as F
 __all__ = ["QuantizedActivation", "quantize_activation", "checkpointed_linear", "CheckpointedLinear"]
 
 BLOCK = 32  # features that share a step
+HEAD_FEATURES = 65536  # kHeadFeatures of csrc/host_policy.cpp
 _DT = {torch.float32: 0, torch.bfloat16: 2, torch.float16: 3}
 
 
@@ -117,18 +118,36 @@ def quantize_activation(x: Tensor) -> QuantizedActivation:
     if x.ndim < 1 or x.shape[-1] == 0:
         raise RuntimeError(f"quantize_activation needs a feature dim, got shape {tuple(x.shape)}")
     _check_device(x)
-    lead, D = x.shape[:-1], x.shape[-1]
-    blocks = (D + BLOCK - 1) // BLOCK
-    codes = torch.empty(*lead, blocks * BLOCK, dtype=torch.int8, device=x.device)
-    exponents = torch.empty(*lead, blocks, dtype=torch.uint8, device=x.device)
+    codes, exponents = _empty_kept(x)
     if x.numel():
         rows = _rows(x.detach())
-        _call("trl_act_quantize", x.device, _DT[x.dtype], rows.data_ptr(), rows.stride(0), rows.shape[0], D, codes.data_ptr(), exponents.data_ptr())
+        _call("trl_act_quantize", x.device, _DT[x.dtype], rows.data_ptr(), rows.stride(0), rows.shape[0], x.shape[-1], codes.data_ptr(),
+              exponents.data_ptr())
     return QuantizedActivation(codes, exponents, x.shape, x.dtype)
 
 
-def _weight_grad(dy: Tensor, codes: Optional[Tensor], exponents: Optional[Tensor], D: int, want_db: bool):
-    """(dy^T x^, column sums of dy or None) of (N, O) gradients and a kept (N, D) activation; without one (D == 0) the sums alone."""
+def _empty_kept(x: Tensor):
+    blocks = (x.shape[-1] + BLOCK - 1) // BLOCK
+    return (torch.empty(*x.shape[:-1], blocks * BLOCK, dtype=torch.int8, device=x.device),
+            torch.empty(*x.shape[:-1], blocks, dtype=torch.uint8, device=x.device))
+
+
+def _linear_and_kept(x: Tensor, weight: Tensor, bias: Optional[Tensor]):
+    """(x W^T + b, codes, exponents); a layer of one output in one pass over x (host_policy.cpp has the measurements of the rule)."""
+    if weight.shape[0] != 1 or weight.shape[1] > HEAD_FEATURES or x.numel() == 0:
+        kept = quantize_activation(x)
+        return torch.nn.functional.linear(x, weight, bias), kept.codes, kept.exponents
+    codes, exponents = _empty_kept(x)
+    y = torch.empty(*x.shape[:-1], 1, dtype=x.dtype, device=x.device)
+    rows, w = _rows(x.detach()), weight.detach().contiguous()
+    _call("trl_act_head_fwd", x.device, _DT[x.dtype], rows.data_ptr(), rows.stride(0), rows.shape[0], x.shape[-1], w.data_ptr(), _ptr(bias),
+          codes.data_ptr(), exponents.data_ptr(), y.data_ptr())
+    return y, codes, exponents
+
+
+def _weight_grad(dy: Tensor, codes: Optional[Tensor], exponents: Optional[Tensor], D: int, want_db: bool, weight: Optional[Tensor] = None):
+    """(dy^T x^, column sums of dy or None) of (N, O) gradients and a kept (N, D) activation; without one (D == 0) the sums alone.
+    With the ``weight`` of a layer of one output (dw, db, dy weight)."""
     dy = dy if dy.stride(1) == 1 or dy.shape[1] == 1 else dy.contiguous()
     N, O = dy.shape
     dt = _DT[dy.dtype]
@@ -136,6 +155,11 @@ def _weight_grad(dy: Tensor, codes: Optional[Tensor], exponents: Optional[Tensor
     db = torch.empty(O, dtype=dy.dtype, device=dy.device) if want_db else None
     need = _extension.get_lib().trl_act_weight_grad_workspace_bytes(dt, N, O, D)
     ws = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
+    if weight is not None:
+        w, dx = weight.detach().contiguous(), torch.empty(N, D, dtype=dy.dtype, device=dy.device)
+        _call("trl_act_head_bwd", dy.device, dt, dy.data_ptr(), dy.stride(0), _ptr(codes), _ptr(exponents), N, D, w.data_ptr(), _ptr(dw), _ptr(db),
+              _ptr(dx), _ptr(ws), need)
+        return dw, db, dx
     _call("trl_act_weight_grad", dy.device, dt, dy.data_ptr(), dy.stride(0), _ptr(codes), _ptr(exponents), N, O, D, _ptr(dw), _ptr(db), _ptr(ws), need)
     return dw, db
 
@@ -143,11 +167,14 @@ def _weight_grad(dy: Tensor, codes: Optional[Tensor], exponents: Optional[Tensor
 class _CheckpointedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        kept = quantize_activation(x) if ctx.needs_input_grad[1] else None
-        ctx.save_for_backward(None if kept is None else kept.codes, None if kept is None else kept.exponents,
-                              weight if ctx.needs_input_grad[0] else None)
+        codes = exponents = None
+        if ctx.needs_input_grad[1]:
+            y, codes, exponents = _linear_and_kept(x, weight, bias)
+        else:
+            y = torch.nn.functional.linear(x, weight, bias)
+        ctx.save_for_backward(codes, exponents, weight if ctx.needs_input_grad[0] else None)
         ctx.features = x.shape[-1]
-        return torch.nn.functional.linear(x, weight, bias)
+        return y
 
     @staticmethod
     @once_differentiable
@@ -156,6 +183,9 @@ class _CheckpointedLinear(torch.autograd.Function):
         need_x, need_w, need_b = ctx.needs_input_grad
         dx = dw = db = None
         dy = grad.reshape(math.prod(grad.shape[:-1]), grad.shape[-1])
+        if need_x and need_w and weight.shape[0] == 1:
+            dw, db, dx = _weight_grad(dy, codes, exponents, ctx.features, need_b, weight)
+            return dx.view(*grad.shape[:-1], ctx.features), dw, db
         if need_x:
             dx = (dy @ weight).view(*grad.shape[:-1], ctx.features)
         if need_w:
