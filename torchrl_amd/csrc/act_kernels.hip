@@ -450,27 +450,30 @@ __global__ __launch_bounds__(WM *WN *kWave, BM == 256 ? 2 : 1) void act_weight_g
     }
 }
 
-// Adds the parts of a split sum in order; bound by a launch's latency (4 us for 3 parts of 515 x 1027).
-constexpr int kJoinCols = 32, kJoinGroups = 8;
-template <typename T>
+// Adds the parts of a split sum in a fixed order; bound by a launch's latency.  Few parts: a thread a column (3 parts of 515 x 1027: 4.1 us,
+// 7.4 with 8 threads a column).  Many: 8 threads a column, a share of the parts each (256 parts of 256 columns: 5 us and 13).
+template <typename T, int GROUPS>
 __global__ __launch_bounds__(256) void act_join_kernel(const float *parts, int splits, i64 n_w, i64 n_b, T *dw, T *db) {
-    __shared__ float sums[kJoinGroups][kJoinCols];
-    const int col = threadIdx.x % kJoinCols, group = threadIdx.x / kJoinCols;
-    const i64 i = (i64)blockIdx.x * kJoinCols + col;
+    constexpr int kCols = 256 / GROUPS;
+    const int col = threadIdx.x % kCols, group = threadIdx.x / kCols;
+    const i64 i = (i64)blockIdx.x * kCols + col;
     const bool in = i < n_w + n_b, w = i < n_w;
     const i64 n = w ? n_w : n_b, at = w ? i : i - n_w;
     const float *p = parts + (w ? 0 : splits * n_w) + at;
     float s = 0.0f;
     if (in) {
 #pragma unroll 8
-        for (int k = group; k < splits; k += kJoinGroups) s += p[k * n];
+        for (int k = group; k < splits; k += GROUPS) s += p[k * n];
     }
-    sums[group][col] = s;
-    __syncthreads();
-    if (!in || group) return;
+    if constexpr (GROUPS > 1) {
+        __shared__ float sums[GROUPS][kCols];
+        sums[group][col] = s;
+        __syncthreads();
+        if (group) return;
 #pragma unroll
-    for (int k = 1; k < kJoinGroups; ++k) s += sums[k][col];
-    (w ? dw : db)[at] = (T)s;
+        for (int k = 1; k < GROUPS; ++k) s += sums[k][col];
+    }
+    if (in) (w ? dw : db)[at] = (T)s;
 }
 
 // The backward pass of one output (a value head): dw is a column sum of x^ weighted by dy, one read of the codes, and dx = dy w is written
@@ -639,7 +642,11 @@ void launch_weight_grad_t(hipStream_t s, const WeightGradArgs &a, const WeightGr
     }
     if (a.splits > 1) {
         const i64 n_w = a.O * a.D, n_b = a.db ? a.O : 0;
-        hipLaunchKernelGGL(act_join_kernel<T>, dim3((unsigned)((n_w + n_b + kJoinCols - 1) / kJoinCols)), dim3(256), 0, s, a.parts, a.splits, n_w, n_b, (T *)a.dw, (T *)a.db);
+        auto join = [&](auto kernel, int cols) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((n_w + n_b + cols - 1) / cols)), dim3(256), 0, s, a.parts, a.splits, n_w, n_b, (T *)a.dw, (T *)a.db);
+        };
+        if (a.splits > 16) join(act_join_kernel<T, 8>, 32);
+        else join(act_join_kernel<T, 1>, 256);
     }
 }
 
@@ -681,7 +688,7 @@ void launch_act_head(hipStream_t s, int dtype, const void *x, i64 stride, i64 N,
 int launch_act_weight_grad(hipStream_t s, int dtype, const void *dy, i64 dy_stride, const int8_t *codes, const u8 *exponents, i64 N, i64 O,
                            i64 D, void *dw, void *db, void *workspace, const void *w, void *dx) {
     const WeightGradPlan p = weight_grad_plan(dtype, N, O, D);
-    if (p.tiles * p.splits > 0x7fffffffLL || (O * (D + 1) + kJoinCols - 1) / kJoinCols > 0x7fffffffLL) return 2;
+    if (p.tiles * p.splits > 0x7fffffffLL || (O * (D + 1) + 31) / 32 > 0x7fffffffLL) return 2;
     const WeightGradArgs a{dy, dy_stride, codes, exponents, N, O, D, (D + kActBlock - 1) / kActBlock * kActBlock, (int)p.tiles_d, (int)p.tiles, p.part, dw, db,
                            (float *)workspace, p.splits, w, dx};
     if (dtype == TRL_F32) launch_weight_grad_t<float>(s, a, p);
