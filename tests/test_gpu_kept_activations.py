@@ -371,3 +371,19 @@ def test_one_output_layouts_and_non_finite(dtype):
     assert y3[0, 0, 0].isnan() and not y3[1, 2, 0].isfinite() and torch.isfinite(y3).sum() == 34
     (dw,) = torch.autograd.grad(y3, dense, dy)
     assert dw[0, 32:64].isnan().all() and dw[0, :32].isnan().all() and torch.isfinite(dw[0, 64:]).all()  # whole blocks stand for NaN
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,D,O_", [(2048, 1500, 1101), (700, 1003, 1001), (1000, 300, 77), (999, 129, 257), (4096, 70, 500), (331, 513, 9), (5000, 40, 6)])
+def test_weight_gradient_at_the_edges_of_tiles(dtype, N, D, O_):
+    """Tiles that reach over the last output: the gradients lie in a buffer whose gaps between the rows hold NaN, which must not come in."""
+    x = inputs(N, D, dtype, seed=N).clamp(-50, 50)
+    wide = torch.full((N, O_ + 11), math.nan, dtype=dtype)
+    wide[:, :O_] = torch.randn(N, O_, generator=torch.Generator().manual_seed(O_)).to(dtype)
+    dy = wide[:, :O_]
+    kept = O.kept(x)[2]
+    for there in (wide.cuda()[:, :O_], dy.contiguous().cuda()):
+        w, b = torch.zeros(O_, D, dtype=dtype, device="cuda", requires_grad=True), torch.zeros(O_, dtype=dtype, device="cuda", requires_grad=True)
+        dw, db = torch.autograd.grad(checkpointed_linear(x.cuda(), w, b), (w, b), there)
+        O.assert_close(dw, dy.double().T @ kept, bound(dy.double(), kept), "dw")
+        O.assert_close(db, dy.double().sum(0), (N + 1) * O.U * dy.double().abs().sum(0), "db")

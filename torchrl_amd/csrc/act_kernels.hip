@@ -241,10 +241,13 @@ __global__ __launch_bounds__(WM *WN *kWave, BM == 256 ? 2 : 1) void act_weight_g
     const i64 a_left = a.O - (o0 + a_col);
     const int a_n = a_left >= kVec ? kVec : a_left < 0 ? 0 : (int)a_left;
     const bool b_in = d0 + b_col < a.Dp;
-    // whole tiles: a scalar base and a 32-bit offset a vector
-    const bool whole = o0 + BM <= a.O && d0 + BN <= a.Dp && a.dy_stride >= 0 && a.dy_stride < (1LL << 24) && a.Dp < (1LL << 24);
-    const u32 a_off = (u32)(a_row * a.dy_stride + a_col) * sizeof(T), a_step = (u32)(RA * a.dy_stride) * sizeof(T);
-    const u32 b_off = (u32)(b_row * a.Dp + b_col), b_step = (u32)(RB * a.Dp);
+    // Whole steps of BK rows below n_whole: a scalar base and a 32-bit offset a vector.  Columns behind the edge end in output elements that
+    // are not stored, so any numbers do for them: vectors that lie behind it read the tile's first column, those across it the beginning of
+    // the next row -- which the matrix's last row does not have.
+    const bool narrow = a.dy_stride >= kVec && a.dy_stride < (1LL << 24) && a.Dp < (1LL << 24);
+    const i64 n_last = a.O % kVec && o0 + BM > a.O && n1 == a.N ? n1 - 1 : n1, n_whole = narrow ? n_last : n0;
+    const u32 a_off = (u32)(a_row * a.dy_stride + (a_n > 0 ? a_col : 0)) * sizeof(T), a_step = (u32)(RA * a.dy_stride) * sizeof(T);
+    const u32 b_off = (u32)(b_row * a.Dp + (b_in ? b_col : 0)), b_step = (u32)(RB * a.Dp);
     Raw8<T> ra[VA];
     u32x4 rb[VB];
     int re[VB];
@@ -263,7 +266,7 @@ __global__ __launch_bounds__(WM *WN *kWave, BM == 256 ? 2 : 1) void act_weight_g
         }
     };
     auto load_a = [&](i64 n) {
-        if (whole && n + BK <= n1) load_a_whole(n);
+        if (n + BK <= n_whole) load_a_whole(n);
         else {
 #pragma unroll
             for (int q = 0; q < VA; ++q) {
@@ -274,7 +277,7 @@ __global__ __launch_bounds__(WM *WN *kWave, BM == 256 ? 2 : 1) void act_weight_g
         }
     };
     auto load_b = [&](i64 n) {
-        if (whole && n + BK <= n1) load_b_whole(n);
+        if (n + BK <= n_whole) load_b_whole(n);
         else {
 #pragma unroll
             for (int q = 0; q < VB; ++q) {
@@ -344,7 +347,7 @@ __global__ __launch_bounds__(WM *WN *kWave, BM == 256 ? 2 : 1) void act_weight_g
         else
             c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, fa), __builtin_bit_cast(v8bf, fb), c, 0, 0, 0);
     };
-    // The long middle of a whole tile, one straight line a step: fragments are fetched one ahead, those of the next step before the step
+    // The long middle, one straight line a step: fragments are fetched one ahead, those of the next step before the step
     // ends.  Two barriers: before the last quarter (the next buffer is written), and before that buffer's successor is written over
     // (every wave is through with the last quarter's reads).
     if constexpr (BK == 64 && NT == 1 && MI % 2 == 0) {
@@ -369,7 +372,7 @@ __global__ __launch_bounds__(WM *WN *kWave, BM == 256 ? 2 : 1) void act_weight_g
         auto middle = [&](auto sum) {
             fetch_b(lds, 0, 0);
             fetch_a(lds, 0, 0);
-            for (; n + 3 * BK <= n1; n += BK, cur ^= 1) {
+            for (; n + 3 * BK <= n_whole; n += BK, cur ^= 1) {
                 const short *buf = lds + cur * kBuf;
                 short *next = lds + (cur ^ 1) * kBuf;
                 quarter(buf, 0, buf, 16, 0);
@@ -384,7 +387,7 @@ __global__ __launch_bounds__(WM *WN *kWave, BM == 256 ? 2 : 1) void act_weight_g
                 quarter(buf, 48, next, 0, 1);
             }
         };
-        if (whole && n + 3 * BK <= n1) {
+        if (n + 3 * BK <= n_whole) {
             if (want_db) middle(Flag<true>());
             else middle(Flag<false>());
             __syncthreads();
