@@ -136,9 +136,9 @@ __global__ __launch_bounds__(256) void act_dequantize_kernel(const int8_t *codes
 //           conversion runs in the shadow of the matrix instructions.
 //   splits  Few output tiles split the tokens; the parts are 32 bits and are added in order by a second launch.
 // Bound by the matrix units with a full chip: (8192, 8192)^T (8192, 2048) bf16 takes 255-295 us as the clocks allow, 930-1080 TFLOP/s (the
-// library's product of unquantized operands 291), fp32 8192 x 2048 x 2048 299 us (three products; 473).  A quarter of the chip or less is
-// bound by the head and tail of its blocks: 1111 x 515 x 1027 fp32 18 us and 4 to join.  One output has a kernel
-// of its own below.
+// library's product of unquantized operands 291), fp32 8192 x 2048 x 2048 299 us (three products; 473).  Partly filled tiles and
+// rounds cost the rest: (2048, 3000)^T (2048, 3000) bf16 69 us, 530 TFLOP/s (the library 57-63); 1111 x 515 x 1027 fp32 18 us and 4 to join
+// (19 by the library).  One output has a kernel of its own below.
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
