@@ -387,3 +387,36 @@ def test_weight_gradient_at_the_edges_of_tiles(dtype, N, D, O_):
         dw, db = torch.autograd.grad(checkpointed_linear(x.cuda(), w, b), (w, b), there)
         O.assert_close(dw, dy.double().T @ kept, bound(dy.double(), kept), "dw")
         O.assert_close(db, dy.double().sum(0), (N + 1) * O.U * dy.double().abs().sum(0), "db")
+
+
+def test_one_output_captured_and_replayed():
+    N, D = 700, 520
+    x, dy = inputs(N, D, torch.bfloat16, seed=21).clamp(-50, 50).cuda(), torch.randn(N, 1, dtype=torch.bfloat16, device="cuda")
+    w0, b0 = torch.randn(1, D, dtype=torch.bfloat16, device="cuda"), torch.randn(1, dtype=torch.bfloat16, device="cuda")
+
+    def step(x, w, b):
+        leaf = x.detach().requires_grad_()
+        y = checkpointed_linear(leaf, w, b)
+        return (y.detach(), *torch.autograd.grad(y, (leaf, w, b), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, w0.clone().requires_grad_(), b0.clone().requires_grad_())
+    torch.cuda.current_stream().wait_stream(side)
+    w, b = w0.clone().requires_grad_(), b0.clone().requires_grad_()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step(x, w, b)
+        graphs.append((graph, outs))
+    for _ in range(4):
+        x.copy_(torch.roll(x, 1, 0) * 1.25)
+        for graph, _ in graphs:
+            graph.replay()
+        eager = step(x, w0.clone().requires_grad_(), b0.clone().requires_grad_())
+        torch.cuda.synchronize()
+        for _, outs in graphs:
+            for got, want in zip(outs, eager):
+                assert torch.equal(got, want)
