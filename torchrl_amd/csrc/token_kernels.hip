@@ -659,7 +659,7 @@ int launch_waves(hipStream_t s, TokenArgs &a) {
     const i64 waves = (a.nsubs + a.nslices - 1) / a.nslices;
     // The run of rows of a block (a lane holds a row's scalars): as few rounds of blocks as the chip takes at a time, counted in rows, with
     // the block's start as some rows more -- short runs count the history over and over, long ones leave a last round half empty.
-    const i64 slots = 256 * (PEN ? (waves > 8 ? 1 : waves > 4 ? 2 : 4) : 4);
+    const i64 slots = 256 * (16 / waves);  // four waves a SIMD
     const double start = PEN ? 2.0 + (double)a.L / 1024.0 : 1.0;
     double best = 0.0;
     for (i64 c = 1; c <= kWave && c <= a.T; ++c) {
