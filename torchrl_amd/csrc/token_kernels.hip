@@ -5,7 +5,7 @@
 // long as the vector units keep up (about 14 full-rate slots an element at 16 bits; v_exp_f32 takes four of them).
 //   unit     A wave owns kSub consecutive tokens of the vocabulary and a run of rows of one sequence.  It never waits for another
 //            wave after the prologue: no barrier, no LDS exchange inside a row; the softmax partials of a row ({max, sum, weighted
-//            sum} a wave) are joined by a second, small launch.
+//            sum} a wave) are joined by a second, small launch, where there is more than one.
 //   history  How often each token was seen lives in LDS, 4 bytes a token of the block's slice, bit 31 = seen in the prompt.  A
 //            block scans the first row's history once; the next row of a rollout adds the one token that came since (a wave keeps a
 //            64-token window of the history in registers).  Integer counts: the order of the atomics cannot change a result.
@@ -217,17 +217,39 @@ struct RowAhead {
 };
 enum { kRowZero = 1, kRowSteep = 2 };  // no gradient; subtract first
 
+// The results of a row from its largest value, the sum and the weighted sum relative to it.
+__device__ __forceinline__ void finish_row(const TokenArgs &a, i64 r, i64 y, float m, float s, float u, float scale, float z_action) {
+    float log_prob = 0.0f, entropy = 0.0f, log2s = 0.0f;
+    if (y < 0) {
+        m = neg_inf();
+    } else {
+        bool steep;
+        const float shift = softmax_shift(m, scale, &steep);
+        if (m == neg_inf() && s == 0.0f) {  // nothing allowed, or nothing possible
+            log_prob = neg_inf();
+        } else {
+            const float z = steep ? z_action - m : z_action;
+            log2s = log2f(s);
+            entropy = kLn2 * (log2s - u / s);
+            log_prob = kLn2 * (fmaf(z, scale, -shift) - log2s);
+        }
+        if (y >= a.V) log_prob = __builtin_nanf("");
+    }
+    a.log_prob[r] = log_prob;
+    if (a.entropy) a.entropy[r] = entropy;
+    if (a.stats) { a.stats[2 * r] = m; a.stats[2 * r + 1] = log2s; }
+}
+
 // Joins a row's partials (one a sub-slice): called by a whole wave.
 __device__ __forceinline__ void join_row(const TokenArgs &a, i64 r, i64 y, const float4 *part, i64 nsubs, float z_action) {
     const int lane = threadIdx.x & (kWave - 1);
-    float log_prob = 0.0f, entropy = 0.0f, m = neg_inf(), log2s = 0.0f;
+    float m = neg_inf(), s = 0.0f, u = 0.0f, scale = 0.0f;
     if (y >= 0) {
         for (i64 i = lane; i < nsubs; i += kWave) m = fmaxf(m, part[i].x);
         m = wave_max_f(m);
-        const float scale = kLog2e * (1.0f / (a.temp_t ? a.temp_t[r / a.T] : a.temp));  // the row kernel's own bits
+        scale = kLog2e * (1.0f / (a.temp_t ? a.temp_t[r / a.T] : a.temp));  // the row kernel's own bits
         bool steep;
         const float shift = softmax_shift(m, scale, &steep);
-        float s = 0.0f, u = 0.0f;
         for (i64 i = lane; i < nsubs; i += kWave) {
             const float4 q = part[i];
             float d = 0.0f;
@@ -244,27 +266,19 @@ __device__ __forceinline__ void join_row(const TokenArgs &a, i64 r, i64 y, const
         }
         s = wave_sum_f(s);
         u = wave_sum_f(u);
-        if (m == neg_inf() && s == 0.0f) {  // nothing allowed, or nothing possible
-            log_prob = neg_inf();
-        } else {
-            const float z = steep ? z_action - m : z_action;
-            log2s = log2f(s);
-            entropy = kLn2 * (log2s - u / s);
-            log_prob = kLn2 * (fmaf(z, scale, -shift) - log2s);
-        }
-        if (y >= a.V) log_prob = __builtin_nanf("");
     }
-    if (lane == 0) {
-        a.log_prob[r] = log_prob;
-        if (a.entropy) a.entropy[r] = entropy;
-        if (a.stats) { a.stats[2 * r] = m; a.stats[2 * r + 1] = log2s; }
-    }
+    if (lane == 0) finish_row(a, r, y, m, s, u, scale, z_action);
 }
 
-template <bool PEN> constexpr int kMostWaves = PEN ? 16 : 4;  // of a block: the launch picks up to that many
+// fp32 log-probabilities under penalties and a bias hold more than the 128 registers of four waves a SIMD: three, in blocks that fill them
+// (8192 x 131072 with a mask: 711 us, in blocks of 12 waves 734, of 8 837; four waves with 142 registers spilled 1090).
+template <typename T, int MODE, bool PEN, bool BIAS> constexpr bool kHeavy = MODE == kLogProb && PEN && BIAS && sizeof(T) == 4;
+// waves of a block: the launch picks up to that many
+template <typename T, int MODE, bool PEN, bool BIAS> constexpr int kMostWaves = PEN && !kHeavy<T, MODE, PEN, BIAS> ? 16 : 4;
+template <typename T, int MODE, bool PEN, bool BIAS> constexpr int kSimdWaves = kHeavy<T, MODE, PEN, BIAS> ? 3 : 4;
 
 template <typename T, int MODE, bool PEN, bool BIAS>
-__global__ __launch_bounds__(kMostWaves<PEN> * kWave, 4) void token_kernel(TokenArgs a) {
+__global__ __launch_bounds__((kMostWaves<T, MODE, PEN, BIAS>) * kWave, (kSimdWaves<T, MODE, PEN, BIAS>)) void token_kernel(TokenArgs a) {
     extern __shared__ __align__(16) u32 lds_counts[];  // PEN: a sub-slice a wave
     const int W = blockDim.x / kWave;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -409,6 +423,8 @@ __global__ __launch_bounds__(kMostWaves<PEN> * kWave, 4) void token_kernel(Token
     float *z_action = scalar(a.z_action + r0);
 
     const int lane0 = lane;
+    const bool alone = nsubs == 1;  // a row is one wave's: no joining launch, lane i keeps row i's numbers
+    float own_m = neg_inf(), own_s = 0.0f, own_u = 0.0f, own_z = neg_inf();
     // FULL: every token of the sub-slice exists
     auto run_rows = [&](auto full) {
         constexpr bool FULL = decltype(full)::value;
@@ -506,23 +522,21 @@ __global__ __launch_bounds__(kMostWaves<PEN> * kWave, 4) void token_kernel(Token
 
             if constexpr (MODE == kLogProb) {
                 float z[kRowVecs][kVec];
-                float m = neg_inf();
+                float m = neg_inf(), z_y = neg_inf();
                 const i64 at = y - lo;
 #pragma unroll
                 for (int k = 0; k < kRowVecs; ++k) {
-                    const bool has_action = at >= k * kBlk && at < (k + 1) * kBlk;  // one vector of one wave
-                    if (!live[k]) {
-                        if (has_action && lane == 0) z_action[i_row] = neg_inf();
-                        continue;
-                    }
+                    if (!live[k]) continue;
                     unpack8(zr[k], z[k]);
                     processed(k, z[k], PEN ? Counts8(counts8 + k * kBlk, seen_places >> (k * kVec) & 0xffu) : Counts8(), __builtin_bit_cast(u32, kFarBelow));
 #pragma unroll
                     for (int i = 0; i < kVec; i += 2) m = max3(m, z[k][i], z[k][i + 1]);
-                    if (has_action) {
+                    if (at >= k * kBlk && at < (k + 1) * kBlk) {  // one vector of one wave
+                        float mine_z = neg_inf();
 #pragma unroll
                         for (int i = 0; i < kVec; ++i)
-                            if (off[k] + i == (int)at) z_action[i_row] = bits[k] & (1u << i) ? z[k][i] : neg_inf();
+                            if (((int)at & (kVec - 1)) == i) mine_z = bits[k] & (1u << i) ? z[k][i] : neg_inf();
+                        z_y = read_lane(mine_z, ((int)at & (kBlk - 1)) / kVec);
                     }
                 }
                 m = wave_max_f(m);
@@ -572,7 +586,16 @@ __global__ __launch_bounds__(kMostWaves<PEN> * kWave, 4) void token_kernel(Token
                     s = wave_sum_f(s);
                     u = wave_sum_f(u);
                 }
-                if (lane == 0) *part = make_float4(m, s, u, 0.0f);
+                if (alone) {
+                    const bool its = lane == i_row;
+                    own_m = its ? m : own_m;
+                    own_s = its ? s : own_s;
+                    own_u = its ? u : own_u;
+                    own_z = its ? z_y : own_z;
+                } else if (lane == 0) {
+                    *part = make_float4(m, s, u, 0.0f);
+                    if (at >= 0 && at < kSub) z_action[i_row] = z_y;
+                }
             } else {
                 const float shift = read_lane(mine.shift, i_row), top = read_lane(mine.top, i_row), ca = read_lane(mine.ca, i_row),
                             cb = read_lane(mine.cb, i_row), g = read_lane(mine.g, i_row);
@@ -631,6 +654,10 @@ __global__ __launch_bounds__(kMostWaves<PEN> * kWave, 4) void token_kernel(Token
     };
     if (left >= kSub) run_rows(Bool<true>());
     else run_rows(Bool<false>());
+    if (MODE == kLogProb && alone && lane < rows) {
+        const i64 y = mine.action == 0x7fffffff ? a.V : mine.action;
+        finish_row(a, r0 + lane, y, own_m, own_s, own_u, scale, own_z);
+    }
 }
 
 // One wave a row: 16 bytes a sub-slice to read, so a launch's latency bounds it (2.2 us for 4 rows, 5 us for 8192 of 64 sub-slices).  A
@@ -650,7 +677,7 @@ template <typename T, int MODE, bool PEN, bool BIAS>
 int launch_waves(hipStream_t s, TokenArgs &a) {
     a.nsubs = token_subs(a.V);
     const i64 rows = a.B * a.T;
-    i64 most = kMostWaves<PEN>;
+    i64 most = kMostWaves<T, MODE, PEN, BIAS>;
     if (most > 8) {
         const i64 blocks = (a.nsubs + most - 1) / most * rows;
         if (blocks < 1024 || (a.L < 2048 && blocks < 4096)) most = 8;
@@ -659,7 +686,7 @@ int launch_waves(hipStream_t s, TokenArgs &a) {
     const i64 waves = (a.nsubs + a.nslices - 1) / a.nslices;
     // The run of rows of a block (a lane holds a row's scalars): as few rounds of blocks as the chip takes at a time, counted in rows, with
     // the block's start as some rows more -- short runs count the history over and over, long ones leave a last round half empty.
-    const i64 slots = 256 * (16 / waves);  // four waves a SIMD
+    const i64 slots = 256 * (4 * kSimdWaves<T, MODE, PEN, BIAS> / waves);
     const double start = PEN ? 2.0 + (double)a.L / 1024.0 : 1.0;
     double best = 0.0;
     for (i64 c = 1; c <= kWave && c <= a.T; ++c) {
@@ -700,6 +727,7 @@ int launch_token_log_prob(hipStream_t s, TokenArgs a) {
     const int rc = launch_dtype<kLogProb>(s, a);
     if (rc) return rc;
     a.nsubs = token_subs(a.V);
+    if (a.nsubs == 1) return 0;
     const i64 blocks = (a.B * a.T + 3) / 4;
     if (blocks > 0x7fffffffLL) return 2;
     hipLaunchKernelGGL(token_join_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
