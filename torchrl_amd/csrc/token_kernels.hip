@@ -18,9 +18,9 @@
 // Measured at 8192 x 131072 bf16 (2.15 GB of logits; a large copy reaches 4.75 TB/s here, reading alone 3.7), us:
 // (of 10 rows the mask leaves 4 whole, allows 3 every second token and 3 one in a hundred)
 //                                    nothing on   a mask   a history of 1024   both and a bias
-//   log-probability and entropy         469         434            609               541         4.6 TB/s, 3.5 with a history
-//   their gradient                      872         804            879               800         4.9 TB/s
-//   processed logits                    862         775            856               770         5.0 TB/s
+//   log-probability and entropy         464         416            574               514         4.6 TB/s, 3.7 with a history
+//   their gradient                      871         810            880               800         4.9 TB/s
+//   processed logits                    863         772            857               768         5.0 TB/s
 // HBM bounds all but the first row's two columns with a history: there the vector units do, with the repeated places' factors beside the
 // softmax.  One decoding step of 256 x 131072 with 4096 tokens of history takes 35 us (4.2 TB/s; reading and counting 4 MB of history 32
 // times, once a slice, is what it has beside its 147 MB), one of 8 x 32000 7 us (the history's latency, then the row's).
@@ -240,17 +240,19 @@ __device__ __forceinline__ void finish_row(const TokenArgs &a, i64 r, i64 y, flo
     if (a.stats) { a.stats[2 * r] = m; a.stats[2 * r + 1] = log2s; }
 }
 
-// Joins a row's partials (one a sub-slice): called by a whole wave.
+// Joins a row's partials (one a sub-slice): called by a whole wave, or by one lane for itself.
+template <bool WAVE>
 __device__ __forceinline__ void join_row(const TokenArgs &a, i64 r, i64 y, const float4 *part, i64 nsubs, float z_action) {
-    const int lane = threadIdx.x & (kWave - 1);
+    const int lane = WAVE ? threadIdx.x & (kWave - 1) : 0;
+    constexpr int kStep = WAVE ? kWave : 1;
     float m = neg_inf(), s = 0.0f, u = 0.0f, scale = 0.0f;
     if (y >= 0) {
-        for (i64 i = lane; i < nsubs; i += kWave) m = fmaxf(m, part[i].x);
-        m = wave_max_f(m);
+        for (i64 i = lane; i < nsubs; i += kStep) m = fmaxf(m, part[i].x);
+        if (WAVE) m = wave_max_f(m);
         scale = kLog2e * (1.0f / (a.temp_t ? a.temp_t[r / a.T] : a.temp));  // the row kernel's own bits
         bool steep;
         const float shift = softmax_shift(m, scale, &steep);
-        for (i64 i = lane; i < nsubs; i += kWave) {
+        for (i64 i = lane; i < nsubs; i += kStep) {
             const float4 q = part[i];
             float d = 0.0f;
             if (q.x != m) {
@@ -264,8 +266,10 @@ __device__ __forceinline__ void join_row(const TokenArgs &a, i64 r, i64 y, const
             s = fmaf(w, q.y, s);
             u = fmaf(w, fmaf(q.y, fmaxf(d, kFloor), q.z), u);
         }
-        s = wave_sum_f(s);
-        u = wave_sum_f(u);
+        if (WAVE) {
+            s = wave_sum_f(s);
+            u = wave_sum_f(u);
+        }
     }
     if (lane == 0) finish_row(a, r, y, m, s, u, scale, z_action);
 }
@@ -660,13 +664,17 @@ __global__ __launch_bounds__((kMostWaves<T, MODE, PEN, BIAS>) * kWave, (kSimdWav
     }
 }
 
-// One wave a row: 16 bytes a sub-slice to read, so a launch's latency bounds it (2.2 us for 4 rows, 5 us for 8192 of 64 sub-slices).  A
-// last-block join inside the row kernel would save it but costs that kernel an atomic, a fence and registers a row; it measured slower.
+// A wave a row: 16 bytes a sub-slice to read, so a launch's latency bounds it (2.2 us for 4 rows, 5 us for 8192 of 64 sub-slices).  A lane a row
+// where there are up to kSerialSubs (32768 rows of 2, 4 and 8: 4.2, 4.8 and 7.9 us, with a wave each 11, 13 and 15; of 16 11 and 14, but 64 rows
+// of 16 6.5 and 4.0).  A last-block join inside the row kernel would save the launch but costs that kernel an atomic, a fence and registers a
+// row; it measured slower.
+constexpr i64 kSerialSubs = 8;
+template <bool WAVE>
 __global__ __launch_bounds__(256) void token_join_kernel(TokenArgs a) {
-    const i64 r = (i64)blockIdx.x * 4 + threadIdx.x / kWave;
+    const i64 r = WAVE ? (i64)blockIdx.x * 4 + threadIdx.x / kWave : (i64)blockIdx.x * 256 + threadIdx.x;
     if (r >= a.B * a.T) return;
     const i64 y = load_int(a.action, a.action_wide, r);
-    join_row(a, r, y, (const float4 *)a.partials + r * a.nsubs, a.nsubs, y >= 0 && y < a.V ? a.z_action[r] : 0.0f);
+    join_row<WAVE>(a, r, y, (const float4 *)a.partials + r * a.nsubs, a.nsubs, y >= 0 && y < a.V ? a.z_action[r] : 0.0f);
 }
 
 // Blocks of as many waves as an even split of the vocabulary gives them, up to 8 beside a history: two such blocks share a compute unit,
@@ -728,9 +736,11 @@ int launch_token_log_prob(hipStream_t s, TokenArgs a) {
     if (rc) return rc;
     a.nsubs = token_subs(a.V);
     if (a.nsubs == 1) return 0;
-    const i64 blocks = (a.B * a.T + 3) / 4;
+    const bool wave = a.nsubs > kSerialSubs;
+    const i64 blocks = wave ? (a.B * a.T + 3) / 4 : (a.B * a.T + 255) / 256;
     if (blocks > 0x7fffffffLL) return 2;
-    hipLaunchKernelGGL(token_join_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
+    if (wave) hipLaunchKernelGGL(token_join_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(token_join_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, s, a);
     return 0;
 }
 int launch_token_log_prob_bwd(hipStream_t s, TokenArgs a) { return launch_dtype<kLogProbBwd>(s, a); }
