@@ -420,3 +420,20 @@ def test_one_output_captured_and_replayed():
         for _, outs in graphs:
             for got, want in zip(outs, eager):
                 assert torch.equal(got, want)
+
+
+def test_one_output_past_32_bits():
+    """Rows behind 2^31 elements: the bits of the same rows alone."""
+    N, D = 40000, 60000
+    x = torch.randn(100, D, device="cuda", dtype=torch.bfloat16).repeat(N // 100, 1)
+    w = torch.randn(1, D, device="cuda", dtype=x.dtype, requires_grad=True)
+    x[-3:] *= torch.rand(3, D, device="cuda").to(x.dtype)
+    dy = torch.zeros(N, 1, device="cuda", dtype=x.dtype)
+    dy[-3:] = torch.tensor([[1.5], [0.0], [0.0]], device="cuda")
+    few = x[-3:].clone()
+    leaf = x.requires_grad_()
+    y = checkpointed_linear(leaf, w)
+    assert torch.equal(y[-3:], checkpointed_linear(few, w)) and torch.equal(y[:100], y[100:200])
+    dx, dw = torch.autograd.grad(y, (leaf, w), dy)
+    assert torch.equal(dx[-3:], dy[-3:] * w) and not dx[:-3].any()
+    assert torch.equal(dw, (1.5 * quantize_activation(few).dequantize()[:1].float()).to(x.dtype))  # one term

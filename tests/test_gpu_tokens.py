@@ -508,3 +508,20 @@ def test_wide_strides():
     process_logits(z, temperature=2.0, mask=mask, out=z)
     assert torch.equal(z, want)
     assert torch.count_nonzero(far) == torch.count_nonzero(want)  # what lies between the rows is as it was
+
+
+def test_many_short_rows():
+    """More than 2^31 elements in rows that one wave owns: the bits of the same rows alone."""
+    B, T, V = 1 << 15, 513, 130
+    z = torch.randn(1, 64, V, device="cuda", dtype=torch.bfloat16).repeat(B, 9, 1)[:, :T].contiguous()
+    z[-1] = torch.randn(T, V, device="cuda")
+    action = torch.randint(0, V, (B, T), device="cuda", dtype=torch.int32)
+    action[-1, 7] = -1
+    leaf = z.requires_grad_()
+    lp, H = token_log_prob(leaf, action, entropy=True)
+    (d,) = torch.autograd.grad((lp, H), leaf, (torch.ones_like(lp), torch.ones_like(H)))
+    few = z.detach()[-1:].clone().requires_grad_()
+    lp1, H1 = token_log_prob(few, action[-1:], entropy=True)
+    (d1,) = torch.autograd.grad((lp1, H1), few, (torch.ones_like(lp1), torch.ones_like(H1)))
+    assert torch.equal(lp[-1:], lp1) and torch.equal(H[-1:], H1) and torch.equal(d[-1:], d1) and lp1[0, 7] == 0 and not d1[0, 7].any()
+    assert torch.equal(H[0], H[B // 2]) and z.numel() > 1 << 31
