@@ -525,3 +525,27 @@ def test_many_short_rows():
     (d1,) = torch.autograd.grad((lp1, H1), few, (torch.ones_like(lp1), torch.ones_like(H1)))
     assert torch.equal(lp[-1:], lp1) and torch.equal(H[-1:], H1) and torch.equal(d[-1:], d1) and lp1[0, 7] == 0 and not d1[0, 7].any()
     assert torch.equal(H[0], H[B // 2]) and z.numel() > 1 << 31
+
+
+@pytest.mark.parametrize("form", ["number", "tensor"])
+@pytest.mark.parametrize("kind", ["plain", "bits", "bool", "all"])
+@pytest.mark.parametrize("V", [100, 2049, 5000])
+@pytest.mark.parametrize("temp", [1e22, 1e24, 1e27, 1e28, 1e30, 2.0 ** 127, 3e38])
+def test_very_high_temperatures(temp, V, kind, form):
+    """The uniform distribution over what is allowed: neither masked places nor those behind the vocabulary's end have weight."""
+    for dtype in DTYPES if V == 2049 else [torch.float32]:
+        c = make(kind, dtype, 3, 4, V, L=30, seed=V)
+        c["oracle"]["temp"] = temp
+        c["kwargs"]["temperature"] = temp if form == "number" else torch.full((3,), temp)
+        z, kw, action = c["z"].cuda(), kwargs(c), c["action"].cuda()
+        want = O.token_policy(c["z"], action=c["action"], g_lp=c["g"][0], g_H=c["g"][1], **c["oracle"])
+        leaf = z.requires_grad_()
+        lp, H = token_log_prob(leaf, action, entropy=True, **kw)
+        O.assert_close(lp, want.log_prob, want.log_prob_tol, "log_prob")
+        O.assert_close(H, want.entropy, want.entropy_tol, "entropy")
+        allowed = want.ok.sum(-1)
+        assert torch.allclose(want.entropy, torch.where(allowed > 0, allowed.double().log(), 0.0), rtol=0, atol=1e-12)
+        (d,) = torch.autograd.grad((lp, H), leaf, tuple(g.cuda() for g in c["g"]))
+        # products with 1 / temperature may be subnormal: half a step of 2^-149 each, for 1 / temperature itself, the three coefficients,
+        # their sum, the product and the repetition factor
+        O.assert_close(d, want.d_logits, want.d_logits_tol, "gradient", floor=8 * 2.0 ** -150)

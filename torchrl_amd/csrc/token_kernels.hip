@@ -156,8 +156,10 @@ __device__ __forceinline__ float where_allowed(u32 bits, int i, float z, u32 oth
 }
 constexpr u32 kNegInfBits = 0xff800000u;
 // What stands for -inf in masked places of the log-probability's forward pass: 0 * d stays finite there without a clamp.  Waves whose
-// maximum comes near it, and waves whose weighted sum is NaN (infinities in allowed places), start over with -inf and a clamp.
-constexpr float kFarBelow = -1e30f;
+// maximum comes near it, and waves whose weighted sum is NaN (infinities in allowed places), start over with -inf and a clamp.  So do
+// all waves at a scale of up to 1e-23 (temperatures from 1.4e23 on): it has to be far below in the exponent, where it stands at -1e7
+// at that scale, ten times the 2^20 that a shift may add.
+constexpr float kFarBelow = -1e30f, kLeastScale = 1e-23f;
 
 // (the builtin would first pass values of unknown origin through a multiplication by one)
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -412,6 +414,7 @@ __global__ __launch_bounds__((kMostWaves<T, MODE, PEN, BIAS>) * kWave, (kSimdWav
         }
     };
 
+    const float least_max = scale > kLeastScale ? 0.01f * kFarBelow : __builtin_inff();  // above it, masked places may hold kFarBelow
     const i64 left = a.V - lo;
     const int mask_kind = scalar(a.mask_kind);
     const i64 logits_st = scalar(a.logits_st), out_st = scalar(a.out_st), mask_st = scalar(a.mask_st), nsubs = scalar(a.nsubs);
@@ -547,7 +550,7 @@ __global__ __launch_bounds__((kMostWaves<T, MODE, PEN, BIAS>) * kWave, (kSimdWav
                 float s = 0.0f, u = 0.0f;
                 bool steep;
                 float shift = softmax_shift(m, scale, &steep);
-                bool careful = steep || !(m > 0.01f * kFarBelow);  // (not live at all among them)
+                bool careful = steep || !(m > least_max);  // (not live at all among them)
                 if (!careful) {
 #pragma unroll
                     for (int k = 0; k < kRowVecs; ++k) {
