@@ -549,3 +549,39 @@ def test_very_high_temperatures(temp, V, kind, form):
         # products with 1 / temperature may be subnormal: half a step of 2^-149 each, for 1 / temperature itself, the three coefficients,
         # their sum, the product and the repetition factor
         O.assert_close(d, want.d_logits, want.d_logits_tol, "gradient", floor=8 * 2.0 ** -150)
+
+
+@pytest.mark.parametrize("form", ["number", "tensor"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temp", [1e-18, 1e-21, 1e-30, 1e-35, 1e-37, 2.0 ** -126])
+def test_very_low_temperatures(temp, dtype, form):
+    """The largest logit alone has weight, two equal ones half of it each; gradients are 0 where nothing has weight, with no NaN from 0 * infinity."""
+    n, V = 6, 2300
+    g = torch.Generator().manual_seed(7)
+    z = (torch.randint(-64, 65, (n, V), generator=g) / 64.0).to(dtype)  # exact in every type; differences of 2^-6 and more
+    top = torch.randint(0, V, (n,), generator=g)
+    z[torch.arange(n), top] = 1.5
+    z[5, 7] = z[5, 2200] = 1.5
+    z[5, top[5]] = 0.0 if int(top[5]) not in (7, 2200) else 1.5
+    action = top.clone()
+    action[1::2] = (top[1::2] + 5) % V
+    action[5] = 7
+    a, b = torch.randn(n, generator=g).clamp(-1.5, 1.5), torch.randn(n, generator=g).clamp(-1.5, 1.5)
+    T = float(torch.tensor(temp, dtype=torch.float32))
+    p = (z == 1.5).double()
+    p /= p.sum(-1, keepdim=True)
+    at = action.unsqueeze(-1)
+    gap = z.double().gather(-1, at).squeeze(-1) - 1.5
+    want_lp = gap / T - torch.log(torch.where(gap == 0, (z == 1.5).sum(-1), 1).double())
+    want_H = torch.log((z == 1.5).sum(-1).double())
+    dz = (torch.zeros(n, V, dtype=torch.float64).scatter(-1, at, 1.0) - p) * a.double().unsqueeze(-1)  # -b p (log p + H) is 0 for equal weights
+    leaf = z.cuda().requires_grad_()
+    lp, H = token_log_prob(leaf, action.cuda(), entropy=True, temperature=temp if form == "number" else torch.full((n,), temp, device="cuda"))
+    # the scale's three roundings, the difference's product, ln 2's
+    O.assert_close(lp, want_lp, 6 * O.U * want_lp.abs() + 2 * O.U, "log_prob")
+    O.assert_close(H, want_H, 4 * O.U * want_H, "entropy")
+    (d,) = torch.autograd.grad((lp, H), leaf, (a.cuda(), b.cuda()))
+    # 1 / temperature, the products and the difference; of the entropy's share what its own roundings leave, 8 U b / temperature a token of weight
+    tol = (6 * O.U * dz.abs() + p * 8 * O.U * (a.abs() + b.abs()).double().unsqueeze(-1)) / T
+    O.assert_close(d, dz / T, tol, "gradient")
+    assert (d.cpu()[(p == 0) & (dz == 0)] == 0).all()

@@ -215,9 +215,11 @@ struct RowAhead {
     int action = 0;  // -1: padding; 0x7fffffff: no token of the vocabulary
     // backward: d raw = -e (ca + cb d), + g at the action
     float shift = 0.0f, top = 0.0f, ca = 0.0f, cb = 0.0f, g = 0.0f;
-    int kind = 0;  // kRowZero, kRowSteep
+    int kind = 0;  // kRowZero, kRowSteep, kRowCold
 };
-enum { kRowZero = 1, kRowSteep = 2 };  // no gradient; subtract first
+// no gradient; subtract first; 1 / temperature comes last (in the coefficients it may overflow, and what has no weight would be 0 * infinity)
+enum { kRowZero = 1, kRowSteep = 2, kRowCold = 4 };
+constexpr float kColdest = 0x1p64f;  // 1 / temperature in the coefficients up to here: 2^63 is left for the gradients, kFloor and the sums
 
 // The results of a row from its largest value, the sum and the weighted sum relative to it.
 __device__ __forceinline__ void finish_row(const TokenArgs &a, i64 r, i64 y, float m, float s, float u, float scale, float z_action) {
@@ -357,10 +359,12 @@ __global__ __launch_bounds__((kMostWaves<T, MODE, PEN, BIAS>) * kWave, (kSimdWav
                 float g = a.g_log_prob ? a.g_log_prob[r] : 0.0f;
                 if (mine.action == 0x7fffffff) g = __builtin_nanf("");
                 const float entropy = a.g_entropy ? a.entropy[r] : 0.0f;
-                mine.ca = rs * (g + g_h * (entropy - kLn2 * log2s)) * inv_temp;
-                mine.cb = rs * g_h * kLn2 * inv_temp;
-                mine.g = g * inv_temp;
-                mine.kind = steep ? kRowSteep : 0;
+                const bool cold = inv_temp > kColdest;
+                const float f = cold ? 1.0f : inv_temp;
+                mine.ca = rs * (g + g_h * (entropy - kLn2 * log2s)) * f;
+                mine.cb = rs * g_h * kLn2 * f;
+                mine.g = g * f;
+                mine.kind = (steep ? kRowSteep : 0) | (cold ? kRowCold : 0);
             }
         }
     }
@@ -643,6 +647,10 @@ __global__ __launch_bounds__((kMostWaves<T, MODE, PEN, BIAS>) * kWave, (kSimdWav
 #pragma unroll
                                 for (int i = 0; i < kVec; ++i)
                                     if (lane * kVec + i == (int)at) z[i] += g;
+                            }
+                            if (kind & kRowCold) {
+#pragma unroll
+                                for (int i = 0; i < kVec; ++i) z[i] *= inv_temp;
                             }
                         }
                         if constexpr (PEN && MODE != kProcess) c.slope(z, raw, pen);
