@@ -437,3 +437,53 @@ def test_one_output_past_32_bits():
     dx, dw = torch.autograd.grad(y, (leaf, w), dy)
     assert torch.equal(dx[-3:], dy[-3:] * w) and not dx[:-3].any()
     assert torch.equal(dw, (1.5 * quantize_activation(few).dequantize()[:1].float()).to(x.dtype))  # one term
+
+
+@pytest.mark.parametrize("route", ["host", "python", "compiled"])
+@pytest.mark.parametrize("shape", [(6, 40), (2, 3, 40), (2, 2, 3, 40), (40,)])
+@pytest.mark.parametrize("bias", [True, False])
+def test_outputs_may_be_written_in_place(shape, bias, route, monkeypatch):
+    """As torch.nn.Linear's: an activation or a residual in place, with and without a gradient to the weight, and behind a no_grad block."""
+    if route == "python":
+        monkeypatch.setattr(F, "_HOST", None)
+    torch._dynamo.reset()
+    torch.manual_seed(0)
+    for out in (20, 1):
+        layer = CheckpointedLinear(40, out, bias=bias, device="cuda")
+        x = torch.randn(shape, device="cuda")
+        r = torch.randn(shape[:-1] + (out,), device="cuda", requires_grad=True)
+
+        def step(leaf):
+            y = layer(leaf)
+            y += r
+            return y.relu_()
+
+        f = torch.compile(step, fullgraph=True) if route == "compiled" else step
+        for frozen in (False, True):
+            layer.weight.requires_grad_(not frozen)
+            leaf = x.clone().requires_grad_()
+            y = f(leaf)
+            want = torch.relu(layer(leaf) + r)
+            torch.testing.assert_close(y, want, rtol=1e-6, atol=1e-6)  # sums of 40 products of this size, in two orders at most
+            (dx,), (dx2,) = (torch.autograd.grad(t.sum(), leaf) for t in (y, want))
+            torch.testing.assert_close(dx, dx2, rtol=1e-6, atol=1e-6)
+        with torch.no_grad():
+            y = layer(x)
+        y += r
+        assert torch.equal(torch.autograd.grad(y.sum(), r)[0], torch.ones_like(r))
+
+
+@pytest.mark.parametrize("route", ["host", "python"])
+@pytest.mark.parametrize("need", ["x", "weight", "x weight", "x weight bias"])
+def test_the_gradient_is_not_differentiable_again(need, route, monkeypatch):
+    if route == "python":
+        monkeypatch.setattr(F, "_HOST", None)
+    leaves = {"x": torch.randn(2, 5, 40, device="cuda"), "weight": torch.randn(3, 40, device="cuda"), "bias": torch.randn(3, device="cuda")}
+    for k in need.split():
+        leaves[k].requires_grad_()
+    dy = torch.randn(2, 5, 3, device="cuda", requires_grad=True)
+    y = checkpointed_linear(leaves["x"], leaves["weight"], leaves["bias"])
+    grads = torch.autograd.grad(y, [leaves[k] for k in need.split()], dy, create_graph=True)
+    for g in grads:
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward(retain_graph=True)

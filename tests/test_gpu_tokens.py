@@ -585,3 +585,36 @@ def test_very_low_temperatures(temp, dtype, form):
     tol = (6 * O.U * dz.abs() + p * 8 * O.U * (a.abs() + b.abs()).double().unsqueeze(-1)) / T
     O.assert_close(d, dz / T, tol, "gradient")
     assert (d.cpu()[(p == 0) & (dz == 0)] == 0).all()
+
+
+@pytest.mark.parametrize("route", ["host module", "python"])
+@pytest.mark.parametrize("form", ["number", "tensor"])
+@pytest.mark.parametrize("T", [0, 3])
+def test_results_may_be_written_in_place(T, form, route, monkeypatch):
+    if route == "python":
+        monkeypatch.setattr(F, "_HOST", None)
+    lead = (2, 3) if T else (2,)
+    z, action = torch.randn(*lead, 50, device="cuda"), torch.zeros(lead, dtype=torch.long, device="cuda")
+    temperature = 2.0 if form == "number" else torch.full((2,), 2.0, device="cuda")
+    w = torch.tensor(1.5, device="cuda", requires_grad=True)
+    leaf = z.clone().requires_grad_()
+    out = process_logits(leaf, temperature=temperature)
+    out.mul_(w)
+    (d,) = torch.autograd.grad(out.sum(), leaf)
+    assert torch.equal(d, torch.full_like(z, 0.75))
+    for entropy in (True, False):
+        got = token_log_prob(leaf, action, entropy=entropy, temperature=temperature)
+        lp = got[0] if entropy else got
+        want = torch.autograd.grad(lp.sum(), leaf, retain_graph=True)[0] * 1.5
+        lp.mul_(w)
+        assert torch.equal(torch.autograd.grad(lp.sum(), leaf)[0], torch.autograd.grad((token_log_prob(leaf, action, temperature=temperature) * w).sum(), leaf)[0])
+        torch.testing.assert_close(want, torch.autograd.grad((token_log_prob(leaf, action, temperature=temperature) * w).sum(), leaf)[0])
+    with torch.no_grad():
+        kept = [process_logits(z, temperature=temperature), *token_log_prob(z, action, entropy=True, temperature=temperature)]
+    for x in kept:
+        x.mul_(w)
+        assert x.requires_grad
+    lp, H = token_log_prob(leaf, action, entropy=True, temperature=temperature)
+    H.mul_(2.0)  # the gradient reads it
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        H.sum().backward()

@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <ATen/ATen.h>
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/DeviceGuardImplInterface.h>
@@ -328,7 +329,7 @@ struct CheckpointedLinearBackward : torch::autograd::Node {
                     row = weight.unpack().contiguous();
                     dx = at::empty(shape, dy.options());
                 } else {
-                    dx = at::mm(dy, weight.unpack()).view(shape);
+                    dx = at::_unsafe_view(at::mm(dy, weight.unpack()), shape);
                 }
             }
             if (w || b) {
@@ -462,6 +463,8 @@ PyObject *py_checkpointed_linear(PyObject *, PyObject *const *o, Py_ssize_t narg
         if (gw && w.size(0) == 1 && w.size(1) <= kHeadFeatures) {
             rc = quantize(x, codes, exponents, w, b, &y);
         } else {
+            // below the view tracking: the product folds batch dims and comes back as a view, which may not be written in place once it has a history
+            at::AutoDispatchBelowADInplaceOrView untracked;
             y = at::linear(x, w, b.defined() ? std::optional<at::Tensor>(b) : std::nullopt);
             if (gw) rc = quantize(x, codes, exponents);
         }

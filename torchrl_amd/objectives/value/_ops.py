@@ -428,9 +428,7 @@ def _token_args(tokens, lengths, prompt, rep, pres, freq, bias, mask, temp):
 def process_logits_op(logits, *args):
     with torch.no_grad():
         K, p = _token_call(logits, *args)
-        out = torch.empty(p.B, p.T, p.V, dtype=logits.dtype, device=logits.device)
-        K._process_fwd(p, out)
-        return out.view(logits.shape)
+        return K._process_new(p, logits.shape)
 
 
 @process_logits_op.register_fake
@@ -479,8 +477,7 @@ def token_log_prob_op(logits, action, *args):
     with torch.no_grad():
         K, p = _token_call(logits, *args)
         act = K._int_tensor(action, logits.shape[:-1], "action", logits.device)
-        log_prob, H, stats = K._log_prob_fwd(p, act, True, True)
-        return log_prob.view(action.shape), H.view(action.shape), stats
+        return K._log_prob_fwd(p, act, action.shape, True, True)
 
 
 @token_log_prob_op.register_fake

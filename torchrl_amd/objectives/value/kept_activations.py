@@ -132,11 +132,17 @@ def _empty_kept(x: Tensor):
             torch.empty(*x.shape[:-1], blocks, dtype=torch.uint8, device=x.device))
 
 
+def _linear(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> Tensor:
+    """The library's product.  With batch dims it is a view, and a Function's (or a no_grad block's) views may not be written in place later."""
+    y = torch.nn.functional.linear(x, weight, bias)
+    return torch.ops.aten._unsafe_view(y, y.shape) if y._is_view() else y
+
+
 def _linear_and_kept(x: Tensor, weight: Tensor, bias: Optional[Tensor]):
     """(x W^T + b, codes, exponents); a layer of one output in one pass over x (host_policy.cpp has the measurements of the rule)."""
     if weight.shape[0] != 1 or weight.shape[1] > HEAD_FEATURES or x.numel() == 0:
         kept = quantize_activation(x)
-        return torch.nn.functional.linear(x, weight, bias), kept.codes, kept.exponents
+        return _linear(x, weight, bias), kept.codes, kept.exponents
     codes, exponents = _empty_kept(x)
     y = torch.empty(*x.shape[:-1], 1, dtype=x.dtype, device=x.device)
     rows, w = _rows(x.detach()), weight.detach().contiguous()
@@ -171,7 +177,7 @@ class _CheckpointedLinear(torch.autograd.Function):
         if ctx.needs_input_grad[1]:
             y, codes, exponents = _linear_and_kept(x, weight, bias)
         else:
-            y = torch.nn.functional.linear(x, weight, bias)
+            y = _linear(x, weight, bias)
         ctx.save_for_backward(codes, exponents, weight if ctx.needs_input_grad[0] else None)
         ctx.features = x.shape[-1]
         return y

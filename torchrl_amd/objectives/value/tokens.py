@@ -221,6 +221,13 @@ def _process_fwd(p: _Processing, out: Tensor) -> None:
         _call("trl_process_logits_fwd", out.device, _args(p, out=out.data_ptr(), out_sb=out.stride(0), out_st=out.stride(1)))
 
 
+def _process_new(p: _Processing, shape) -> Tensor:
+    """The processed logits in a tensor of their own; not a view, so that it may be written in place whatever its history."""
+    out = torch.empty(shape, dtype=p.logits.dtype, device=p.logits.device)
+    _process_fwd(p, out.view(p.B, p.T, p.V))
+    return out
+
+
 def _process_bwd(p: _Processing, grad: Tensor) -> Tensor:
     """d_logits (B, T, V); ``p.logits`` may be ``grad`` itself where the logits are not read (no repetition penalty)."""
     grad = grad.reshape(p.B, p.T, p.V).contiguous()
@@ -237,11 +244,10 @@ def _reads_sign(p: _Processing) -> bool:
 class _ProcessLogits(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, p):
-        out = torch.empty(p.B, p.T, p.V, dtype=logits.dtype, device=logits.device)
-        _process_fwd(p, out)
+        out = _process_new(p, logits.shape)
         _save(ctx, p, logits=_reads_sign(p))
         ctx.shape = logits.shape
-        return out.view(logits.shape)
+        return out
 
     @staticmethod
     @once_differentiable
@@ -290,9 +296,7 @@ def process_logits(logits: Tensor, *, tokens: Optional[Tensor] = None, lengths: 
         _need(out is None, RuntimeError, "process_logits(out=...) does not support automatic differentiation")
         return _ProcessLogits.apply(logits, p)
     if out is None:
-        o = torch.empty(p.B, p.T, p.V, dtype=logits.dtype, device=logits.device)
-        _process_fwd(p, o)
-        return o.view(logits.shape)
+        return _process_new(p, logits.shape)
     _need(isinstance(out, Tensor) and out.shape == logits.shape and out.dtype == logits.dtype and out.device == logits.device, RuntimeError,
           "out must have the logits' shape, dtype and device")
     _need(not (torch.is_grad_enabled() and out.requires_grad), RuntimeError, "process_logits(out=...) does not support automatic differentiation")
@@ -315,12 +319,12 @@ def process_logits(logits: Tensor, *, tokens: Optional[Tensor] = None, lengths: 
 
 
 # ---- token_log_prob ---------------------------------------------------------------------------------------------------------
-def _log_prob_fwd(p: _Processing, action: Tensor, entropy: bool, stats: bool):
+def _log_prob_fwd(p: _Processing, action: Tensor, shape, entropy: bool, stats: bool):
+    """log_prob and entropy of ``shape`` (tensors of their own, no views), and {max, log2 of the sum} a row."""
     dev = action.device
     n = p.B * p.T
-    # one allocation: log_prob, entropy, {max, log2 of the sum} a row; the workspace is free again when the launches have run
-    log_prob = torch.empty(n, dtype=torch.float32, device=dev)
-    H = torch.empty(n, dtype=torch.float32, device=dev) if entropy else None
+    log_prob = torch.empty(shape, dtype=torch.float32, device=dev)
+    H = torch.empty(shape, dtype=torch.float32, device=dev) if entropy else None
     st = torch.empty(n, 2, dtype=torch.float32, device=dev) if stats else None
     if n:
         need = _extension.get_lib().trl_token_workspace_bytes(p.B, p.T, p.V)
@@ -348,11 +352,10 @@ class _TokenLogProb(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, p, action, entropy):
         ctx.set_materialize_grads(False)
-        log_prob, H, stats = _log_prob_fwd(p, action, entropy, True)
+        log_prob, H, stats = _log_prob_fwd(p, action, logits.shape[:-1], entropy, True)
         _save(ctx, p, action, H, stats)
         ctx.shape = logits.shape
-        lead = logits.shape[:-1]
-        return log_prob.view(lead), None if H is None else H.view(lead)
+        return log_prob, H
 
     @staticmethod
     @once_differentiable
@@ -392,8 +395,7 @@ def token_log_prob(logits: Tensor, action: Tensor, *, entropy: bool = False, tok
     if F._needs_grad(logits):
         log_prob, H = _TokenLogProb.apply(logits, p, act, bool(entropy))
     else:
-        log_prob, H, _ = _log_prob_fwd(p, act, bool(entropy), False)
-        log_prob, H = log_prob.view(lead), None if H is None else H.view(lead)
+        log_prob, H, _ = _log_prob_fwd(p, act, lead, bool(entropy), False)
     return (log_prob, H) if entropy else log_prob
 
 
