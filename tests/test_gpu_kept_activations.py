@@ -487,3 +487,37 @@ def test_the_gradient_is_not_differentiable_again(need, route, monkeypatch):
     for g in grads:
         with pytest.raises(RuntimeError, match="once_differentiable"):
             g.sum().backward(retain_graph=True)
+
+
+@pytest.mark.parametrize("route", ["host", "python"])
+@pytest.mark.parametrize("out", [1, 20])
+def test_what_a_saved_tensor_hook_hands_back_is_checked(out, route, monkeypatch):
+    """The kernels read what the kept sizes say: another layout is taken, another type, shape or device refused."""
+    if route == "python":
+        monkeypatch.setattr(F, "_HOST", None)
+    g = torch.Generator().manual_seed(1)
+    x, w, dy = (torch.randn(s, generator=g).cuda() for s in ((6, 70), (out, 70), (6, out)))
+
+    def gradients(k, change):
+        leaves = [t.clone().requires_grad_() for t in (x, w)]
+        count = []
+
+        def pack(t):
+            count.append(t)
+            return len(count) - 1, t.detach().clone()
+
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda it: change(it[1]) if it[0] == k else it[1]):
+            y = checkpointed_linear(*leaves)
+        assert len(count) == 3  # codes, exponents, weight
+        return torch.autograd.grad(y, leaves, dy)
+
+    want = gradients(-1, None)
+    for k in range(3):
+        for a, b in zip(gradients(k, lambda t: t.t().contiguous().t()), want):
+            if k < 2 or out == 1:
+                assert torch.equal(a, b)
+            else:  # the library's product of another layout: sums of 20 in another order
+                torch.testing.assert_close(a, b, rtol=0, atol=40 * 2.0 ** -24 * 20 * 10)
+        for change in (lambda t: t.to(torch.int16), lambda t: t[:, :-1], lambda t: t.cpu()):
+            with pytest.raises(RuntimeError):
+                gradients(k, change)

@@ -618,3 +618,46 @@ def test_results_may_be_written_in_place(T, form, route, monkeypatch):
     H.mul_(2.0)  # the gradient reads it
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         H.sum().backward()
+
+
+def other_layout(t):
+    """The same values, the last dim no longer dense (where there are two)."""
+    return t.transpose(0, -1).contiguous().transpose(0, -1) if t.ndim > 1 else t.repeat_interleave(2)[::2]
+
+
+def one_changed(k, change):
+    """Saved-tensor hooks that hand back ``change`` of the k-th kept tensor, and how many were kept."""
+    count = []
+
+    def pack(t):
+        count.append(t)
+        return len(count) - 1, t.detach().clone()
+
+    return torch.autograd.graph.saved_tensors_hooks(pack, lambda it: change(it[1]) if it[0] == k else it[1]), count
+
+
+@pytest.mark.parametrize("route", ["host module", "python"])
+@pytest.mark.parametrize("op", ["process_logits", "token_log_prob"])
+def test_what_a_saved_tensor_hook_hands_back_is_checked(op, route, monkeypatch):
+    """The kernels read what the kept sizes say: another layout is taken, another type, shape or device refused."""
+    if route == "python":
+        monkeypatch.setattr(F, "_HOST", None)
+    c = make("all", torch.bfloat16, 3, 4, 90, L=9, seed=23)
+    kw, action, g_out = kwargs(c), c["action"].cuda(), c["g_out"].cuda()
+    kw["bias"] = kw["bias"].expand(3, 4, 90).contiguous()
+    g = tuple(x.cuda() for x in c["g"])
+
+    def gradient(hooks):
+        leaf = c["z"].cuda().requires_grad_()
+        with hooks:
+            out = process_logits(leaf, **kw) if op == "process_logits" else token_log_prob(leaf, action, entropy=True, **kw)
+        return torch.autograd.grad(out, leaf, g_out if op == "process_logits" else g)[0]
+
+    hooks, count = one_changed(-1, None)
+    want = gradient(hooks)
+    assert len(count) == (6 if op == "process_logits" else 9)  # logits, tokens, lengths, prompt lengths, bias, mask; action, statistics, entropy
+    for k in range(len(count)):
+        assert same(gradient(one_changed(k, other_layout)[0]), want)
+        for change in (lambda t: t.double(), lambda t: t.to(torch.int16), lambda t: t[:-1], lambda t: t.cpu()):
+            with pytest.raises(RuntimeError, match="kept|require gradients"):  # (torch itself: integers in place of the logits)
+                gradient(one_changed(k, change)[0])

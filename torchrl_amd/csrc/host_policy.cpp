@@ -48,6 +48,7 @@ decltype(&trl_act_head_bwd) g_head_bwd = nullptr;
 decltype(&trl_last_error) g_last_error = nullptr;
 
 int dtype_code(at::ScalarType t) { return t == at::kFloat ? TRL_F32 : t == at::kBFloat16 ? TRL_BF16 : t == at::kHalf ? TRL_F16 : -1; }
+at::ScalarType int_type(int wide) { return wide ? at::kLong : at::kInt; }
 bool is_int(const at::Tensor &t) { return t.scalar_type() == at::kLong || t.scalar_type() == at::kInt; }
 bool on_current_device(const at::Tensor &t) {
     return t.is_cuda() && c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getDevice().index() == t.device().index();
@@ -164,6 +165,15 @@ struct Processing {
     bool reads_sign() const { return a.tokens && a.rep != 1.0f; }
 };
 
+// A hook hands back what it likes in place of a kept tensor; the kernels read what the kept sizes say, so anything but another layout is refused.
+void check_kept(const at::Tensor &t, const at::Device &device, bool fits, const char *what) {
+    TORCH_CHECK(t.layout() == at::kStrided && t.device() == device && fits, "torchrl_amd: the kept ", what,
+                " came back from its saved-tensor hook with another type, shape or device");
+}
+void check_kept(const at::Tensor &t, const at::Device &device, at::ScalarType type, int64_t numel, const char *what) {
+    check_kept(t, device, t.scalar_type() == type && t.numel() == numel, what);
+}
+
 // What a node keeps of a Processing: the tensors through SavedVariable (writes in place are noticed, hooks are honoured).
 struct KeptProcessing {
     SavedVariable t[6];
@@ -187,6 +197,15 @@ struct KeptProcessing {
         p.a = a;
         p.a.logits = nullptr;
         p.steps = steps;
+        const at::Device dev = options.device();
+        if (p.logits.defined()) check_kept(p.logits, dev, dtype_code(p.logits.scalar_type()) == a.dtype && p.logits.sizes() == sizes, "logits");
+        if (p.tokens.defined())
+            check_kept(p.tokens, dev, p.tokens.scalar_type() == int_type(a.tokens_wide) && p.tokens.dim() == 2 && p.tokens.size(0) == a.B && p.tokens.size(1) == a.L,
+                       "tokens");
+        if (p.lengths.defined()) check_kept(p.lengths, dev, int_type(a.lengths_wide), a.B * a.T, "lengths");
+        if (p.prompt.defined()) check_kept(p.prompt, dev, int_type(a.prompt_wide), a.B, "prompt lengths");
+        if (p.bias.defined()) check_kept(p.bias, dev, 1 + dtype_code(p.bias.scalar_type()) == a.bias_kind, "bias");
+        if (p.mask.defined()) check_kept(p.mask, dev, p.mask.scalar_type() == (a.mask_kind == TRL_MASK_BITS ? at::kInt : at::kBool), "mask");
         // a hook may hand back the values in another layout: the strides are those of the tensors as they are now
         for (at::Tensor *t : {&p.lengths, &p.prompt})
             if (t->defined()) *t = t->contiguous();
@@ -253,6 +272,10 @@ struct TokenLogProbBackward : torch::autograd::Node {
             Processing p = kept.get();
             const at::Tensor act = action.unpack().contiguous(), st = stats.unpack().contiguous(),
                              h = g_h.defined() ? entropy.unpack(shared_from_this()).contiguous() : at::Tensor();
+            const at::Device dev = kept.options.device();
+            check_kept(act, dev, int_type(p.a.action_wide), p.rows(), "action");
+            check_kept(st, dev, at::kFloat, 2 * p.rows(), "statistics");
+            if (h.defined()) check_kept(h, dev, at::kFloat, p.rows(), "entropy");
             g_lp = row_grad(g_lp);
             g_h = row_grad(g_h);
             d = at::empty(kept.sizes, kept.options);
@@ -327,6 +350,7 @@ struct CheckpointedLinearBackward : torch::autograd::Node {
                 shape.back() = features;
                 if (head) {
                     row = weight.unpack().contiguous();
+                    check_kept(row, dy.device(), dy.scalar_type(), features, "weight");
                     dx = at::empty(shape, dy.options());
                 } else {
                     dx = at::_unsafe_view(at::mm(dy, weight.unpack()), shape);
@@ -334,6 +358,9 @@ struct CheckpointedLinearBackward : torch::autograd::Node {
             }
             if (w || b) {
                 const at::Tensor c = w ? codes.unpack().contiguous() : at::Tensor(), e = w ? exponents.unpack().contiguous() : at::Tensor();
+                const int64_t blocks = (features + 31) / 32;
+                if (w) check_kept(c, dy.device(), at::kChar, N * blocks * 32, "codes");
+                if (w) check_kept(e, dy.device(), at::kByte, N * blocks, "exponents");
                 const int code = dtype_code(dy.scalar_type());
                 if (w) dw = at::empty({O, features}, dy.options());
                 if (b) db = at::empty({O}, dy.options());

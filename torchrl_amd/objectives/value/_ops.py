@@ -492,7 +492,8 @@ def token_log_prob_bwd_op(g_lp, g_H, H, stats, logits, action, *args):
     with torch.no_grad():
         K, p = _token_call(logits, *args)
         act = K._int_tensor(action, logits.shape[:-1], "action", logits.device)
-        return K._log_prob_bwd(p, act, H.reshape(-1).contiguous(), stats.contiguous(), g_lp, g_H).view(logits.shape)
+        F._check_kept((H,), ((torch.float32, tuple(action.shape), logits.device),))
+        return K._log_prob_bwd(p, act, H.contiguous(), stats.contiguous(), g_lp, g_H).view(logits.shape)
 
 
 @token_log_prob_bwd_op.register_fake

@@ -260,6 +260,18 @@ def _needs_grad(*xs) -> bool:
     return torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in xs)
 
 
+def _kept_form(x):
+    return None if x is None else (x.dtype, tuple(x.shape), x.device)
+
+
+def _check_kept(kept, forms) -> None:
+    """A saved-tensor hook hands back what it likes in place of a kept tensor; the kernels read what the kept sizes say, so anything but
+    another layout is refused.  ``forms``: :func:`_kept_form` of the tensors as they were kept."""
+    for x, form in zip(kept, forms):
+        if _kept_form(x) != form or (x is not None and x.layout != torch.strided):
+            raise RuntimeError(f"torchrl_amd: a kept tensor {form} came back from its saved-tensor hook with another type, shape or device: {_kept_form(x)}")
+
+
 _GRAD_MSG = (
     "torchrl_amd: differentiating through {} is not implemented yet (GAE, TD(lambda) and V-trace are); "
     "call it under torch.no_grad() / with differentiable=False, or detach the inputs."

@@ -157,11 +157,16 @@ def _weight_grad(dy: Tensor, codes: Optional[Tensor], exponents: Optional[Tensor
     dy = dy if dy.stride(1) == 1 or dy.shape[1] == 1 else dy.contiguous()
     N, O = dy.shape
     dt = _DT[dy.dtype]
+    if D:  # may come from a saved-tensor hook
+        blocks = (D + BLOCK - 1) // BLOCK
+        codes, exponents = codes.reshape(N, blocks * BLOCK).contiguous(), exponents.reshape(N, blocks).contiguous()
+        F._check_kept((codes, exponents), ((torch.int8, (N, blocks * BLOCK), dy.device), (torch.uint8, (N, blocks), dy.device)))
     dw = torch.empty(O, D, dtype=dy.dtype, device=dy.device) if D else None
     db = torch.empty(O, dtype=dy.dtype, device=dy.device) if want_db else None
     need = _extension.get_lib().trl_act_weight_grad_workspace_bytes(dt, N, O, D)
     ws = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
     if weight is not None:
+        F._check_kept((weight,), ((dy.dtype, (1, D), dy.device),))
         w, dx = weight.detach().contiguous(), torch.empty(N, D, dtype=dy.dtype, device=dy.device)
         _call("trl_act_head_bwd", dy.device, dt, dy.data_ptr(), dy.stride(0), _ptr(codes), _ptr(exponents), N, D, w.data_ptr(), _ptr(dw), _ptr(db),
               _ptr(dx), _ptr(ws), need)

@@ -207,12 +207,17 @@ def _save(ctx, p: _Processing, *more, logits: bool = True):
     if not logits:
         saved[0] = None
     ctx.save_for_backward(*saved, *more)
+    ctx.forms = [F._kept_form(t) for t in (*saved, *more)]
     ctx.numbers = p._replace(**dict.fromkeys(_TENSORS))
 
 
 def _saved(ctx):
     kept = ctx.saved_tensors
-    return ctx.numbers._replace(**dict(zip(_TENSORS, kept))), kept[len(_TENSORS):]
+    F._check_kept(kept, ctx.forms)
+    # a hook may hand back another layout: rows of vectors need a last stride of 1, the rest has to be dense
+    rows = ("logits", "tokens", "bias", "mask")
+    tensors = {k: t if t is None or (k in rows and t.stride(-1) == 1) else t.contiguous() for k, t in zip(_TENSORS, kept)}
+    return ctx.numbers._replace(**tensors), [None if t is None else t.contiguous() for t in kept[len(_TENSORS):]]
 
 
 # ---- process_logits ---------------------------------------------------------------------------------------------------------
@@ -340,7 +345,9 @@ def _row_grad(g: Optional[Tensor]) -> Optional[Tensor]:
 
 def _log_prob_bwd(p: _Processing, action: Tensor, H: Optional[Tensor], stats: Tensor, g_lp: Optional[Tensor], g_H: Optional[Tensor]) -> Tensor:
     d = torch.empty(p.B, p.T, p.V, dtype=p.logits.dtype, device=action.device)
-    if p.B * p.T:
+    n = p.B * p.T
+    F._check_kept((stats,), ((torch.float32, (n, 2), p.logits.device),))
+    if n:
         g_lp, g_H = _row_grad(g_lp), _row_grad(g_H)
         _call("trl_token_log_prob_bwd", action.device, _args(p, action=action.data_ptr(), action_wide=_wide(action), entropy=_ptr(H),
                                                              stats=stats.data_ptr(), g_log_prob=_ptr(g_lp), g_entropy=_ptr(g_H), out=d.data_ptr(),
