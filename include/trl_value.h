@@ -526,7 +526,7 @@ typedef struct trl_token_args {
     const float *g_log_prob, *g_entropy;      /* (B, T) incoming gradients, either may be NULL (= zeros) */
 } trl_token_args;
 
-/* out = z' (one rounding to dtype); out may be the logits themselves (same strides), and must not overlap them otherwise.
+/* out = z' (one rounding to dtype); out may be the logits themselves (same strides), and overlaps no input otherwise.
  * bwd: out = d_logits = grad_out * dz'/dz, 0 in masked places; reads the logits only where rep != 1 (their sign). */
 int trl_process_logits_fwd(void *stream, const trl_token_args *args);
 int trl_process_logits_bwd(void *stream, const trl_token_args *args);

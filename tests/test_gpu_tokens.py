@@ -661,3 +661,14 @@ def test_what_a_saved_tensor_hook_hands_back_is_checked(op, route, monkeypatch):
         for change in (lambda t: t.double(), lambda t: t.to(torch.int16), lambda t: t[:-1], lambda t: t.cpu()):
             with pytest.raises(RuntimeError, match="kept|require gradients"):  # (torch itself: integers in place of the logits)
                 gradient(one_changed(k, change)[0])
+
+
+def test_in_place_beside_and_over_other_inputs():
+    buf = torch.randn(5, 600, device="cuda")
+    z, bias = buf[:, :300], buf[:, 300:]
+    want = process_logits(z, bias=bias, temperature=0.5)
+    kept = bias.clone()
+    assert process_logits(z, bias=bias, temperature=0.5, out=z) is z
+    assert torch.equal(z, want) and torch.equal(bias, kept)
+    with pytest.raises(RuntimeError, match="share no memory"):  # row 0 is a bias of every row
+        process_logits(z, bias=z[0], out=z)

@@ -168,3 +168,38 @@ def test_oracle_gradient_is_autograds():
     (want,) = torch.autograd.grad(loss, z)
     got = O.token_policy(z.detach(), temp=0.7, action=action, g_lp=a, g_H=b).d_logits
     assert torch.allclose(got, want, rtol=1e-12, atol=1e-12)
+
+
+def processing(logits, **tensors):
+    from torchrl_amd.objectives.value import tokens as K
+
+    B, V = logits.shape
+    p = K._Processing(B, 1, V, logits.unsqueeze(1), None, None, None, 1.0, 0.0, 0.0, 1.0, *[None] * 6)
+    return p._replace(**tensors)
+
+
+def test_out_shares_no_memory_with_the_inputs_but_the_logits():
+    from torchrl_amd.objectives.value.tokens import _out_rows
+
+    z, refused = torch.zeros(4, 40), "share no memory"
+    shared = z[:1].expand(4, 40).unsqueeze(1)  # a bias read by all rows, and written with the first
+    with pytest.raises(RuntimeError, match=refused):
+        _out_rows(processing(z, bias=shared), z, z)
+    with pytest.raises(RuntimeError, match=refused):
+        _out_rows(processing(z, mask=z.view(torch.bool)[:, :40].unsqueeze(1)), z, z)
+    with pytest.raises(RuntimeError, match=refused):
+        _out_rows(processing(z[:, :20], bias=z[:, 10:30].unsqueeze(1)), z[:, :20], z[:, :20])  # columns that overlap
+    with pytest.raises(RuntimeError, match=refused):
+        _out_rows(processing(z[1:], bias=None), z[1:], z[:3])  # the logits, a row further on
+    with pytest.raises(RuntimeError, match=refused):
+        _out_rows(processing(z, temp_t=z.view(-1)[100:104]), z, z)
+    # beside each other in one buffer
+    assert _out_rows(processing(z, bias=torch.zeros(40).expand(4, 1, 40)), z, z).shape == (4, 1, 40)
+    assert _out_rows(processing(z[:, :20], bias=z[:, 20:].unsqueeze(1)), z[:, :20], z[:, :20]).data_ptr() == z.data_ptr()
+    assert _out_rows(processing(z[:, 20:], bias=z[2, :20].expand(4, 1, 20)), z[:, 20:], z[:, 20:]).shape == (4, 1, 20)
+    assert _out_rows(processing(z[:2], bias=z[2:].unsqueeze(1)), z[:2], z[:2]).shape == (2, 1, 40)
+    assert _out_rows(processing(z[:, :20]), z[:, :20], z[:, 20:]).shape == (4, 1, 20)
+    with pytest.raises(RuntimeError, match="do not overlap"):
+        _out_rows(processing(z), z, torch.zeros(1, 40).expand(4, 40))
+    with pytest.raises(RuntimeError, match="shape, dtype"):
+        _out_rows(processing(z), z, z.half())

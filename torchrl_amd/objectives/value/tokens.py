@@ -263,6 +263,41 @@ class _ProcessLogits(torch.autograd.Function):
         return _process_bwd(p, grad).view(ctx.shape), None
 
 
+def _apart(a: Tensor, b: Tensor) -> bool:
+    """Whether two tensors with dense rows share no byte: they lie one behind the other, or their rows lie beside each other in rows of one buffer."""
+    def span(x):
+        return x.data_ptr(), x.data_ptr() + (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size()
+
+    if a.numel() == 0 or b.numel() == 0:
+        return True
+    (a0, a1), (b0, b1) = span(a), span(b)
+    if a1 <= b0 or b1 <= a0:
+        return True
+    step = math.gcd(*(s * x.element_size() for x in (a, b) for n, s in zip(x.shape[:-1], x.stride()) if n > 1))
+    off = (b0 - a0) % step if step else 0
+    return off >= a.shape[-1] * a.element_size() and off + b.shape[-1] * b.element_size() <= step
+
+
+def _out_rows(p: _Processing, logits: Tensor, out: Tensor) -> Tensor:
+    """``out`` as (B, T, V), after what :func:`process_logits` promises of it has been checked."""
+    _need(isinstance(out, Tensor) and out.shape == logits.shape and out.dtype == logits.dtype and out.device == logits.device, RuntimeError,
+          "out must have the logits' shape, dtype and device")
+    _need(not (torch.is_grad_enabled() and out.requires_grad), RuntimeError, "process_logits(out=...) does not support automatic differentiation")
+    try:
+        o = out.view(p.B, p.T, p.V)
+    except RuntimeError:
+        o = None
+    _need(o is not None and (o.stride(2) == 1 or p.V == 1) and (o.stride(1) >= p.V or p.T == 1) and (o.stride(0) >= p.V or p.B == 1), RuntimeError,
+          "out must have rows that are dense and do not overlap, and batch dims that can be merged")
+    _need(p.B == 1 or p.T == 1 or o.stride(0) >= p.T * o.stride(1) or o.stride(1) >= p.B * o.stride(0), RuntimeError,
+          "out must have rows that do not overlap")
+    # in place every element is read and written by one thread; a bias or a mask is read by all rows
+    same = out.data_ptr() == p.logits.data_ptr() and out.stride() == logits.stride()
+    _need(all(t is None or _apart(o, t) for k, t in ((k, getattr(p, k)) for k in _TENSORS) if not (same and k == "logits")), RuntimeError,
+          "out must be the logits themselves or share no memory with the inputs")
+    return o
+
+
 def process_logits(logits: Tensor, *, tokens: Optional[Tensor] = None, lengths: Optional[Tensor] = None, prompt_lengths: Optional[Tensor] = None,
                    repetition_penalty: Scalar = 1.0, presence_penalty: Scalar = 0.0, frequency_penalty: Scalar = 0.0,
                    bias: Optional[Tensor] = None, mask: Optional[Tensor] = None, temperature: Scalar = 1.0,
@@ -284,7 +319,8 @@ def process_logits(logits: Tensor, *, tokens: Optional[Tensor] = None, lengths: 
     numbers or tensors that broadcast to ``[*B]`` (tensors are not read on the host: repetition penalties and temperatures in them have to be positive).  ``bias`` broadcasts to the logits.  ``mask`` broadcasts to the logits too: truth values, or
     bits of int32 words ``[..., ceil(V / 32)]`` (token j: bit ``j % 32`` of word ``j // 32``); what the logits hold in masked places does not matter.
 
-    Differentiable in ``logits``; masked places get no gradient.  ``out`` (not under autograd) may be ``logits`` itself."""
+    Differentiable in ``logits``; masked places get no gradient.  ``out`` (not under autograd) may be ``logits`` itself, and shares no
+    memory with any other input."""
     if torch.compiler.is_compiling():
         _need(out is None, NotImplementedError, "process_logits(out=...) is not supported under torch.compile")
         from torchrl_amd.objectives.value import _ops
@@ -302,23 +338,7 @@ def process_logits(logits: Tensor, *, tokens: Optional[Tensor] = None, lengths: 
         return _ProcessLogits.apply(logits, p)
     if out is None:
         return _process_new(p, logits.shape)
-    _need(isinstance(out, Tensor) and out.shape == logits.shape and out.dtype == logits.dtype and out.device == logits.device, RuntimeError,
-          "out must have the logits' shape, dtype and device")
-    _need(not (torch.is_grad_enabled() and out.requires_grad), RuntimeError, "process_logits(out=...) does not support automatic differentiation")
-    same = out.data_ptr() == p.logits.data_ptr() and out.stride() == logits.stride()
-    storage = out.untyped_storage().data_ptr()
-    _need(same or all(t is None or t.untyped_storage().data_ptr() != storage for t in (getattr(p, k) for k in _TENSORS)), RuntimeError,
-          "out must be the logits themselves or share no memory with the inputs")
-    try:
-        o = out.view(p.B, p.T, p.V)
-    except RuntimeError:
-        o = None
-    _need(o is not None and (o.stride(2) == 1 or p.V == 1) and (o.stride(1) >= p.V or p.T == 1) and (o.stride(0) >= p.V or p.B == 1)
-          and not (same and o.data_ptr() != p.logits.data_ptr()), RuntimeError,
-          "out must have rows that are dense and do not overlap, and batch dims that can be merged")
-    _need(p.B == 1 or p.T == 1 or o.stride(0) >= p.T * o.stride(1) or o.stride(1) >= p.B * o.stride(0), RuntimeError,
-          "out must have rows that do not overlap")
-    _process_fwd(p, o)
+    _process_fwd(p, _out_rows(p, logits, out))
     torch.autograd.graph.increment_version(out)
     return out
 
