@@ -521,3 +521,37 @@ def test_what_a_saved_tensor_hook_hands_back_is_checked(out, route, monkeypatch)
         for change in (lambda t: t.to(torch.int16), lambda t: t[:, :-1], lambda t: t.cpu()):
             with pytest.raises(RuntimeError):
                 gradients(k, change)
+
+
+def test_more_rows_than_a_launch_takes():
+    """2^26 rows of a value head and 2^35 elements of an activation are several launches: the bits of the same rows alone."""
+    few, N, D = 1 << 10, (1 << 26) + 37, 32
+    x, w, dy = (torch.randn(s, device="cuda").bfloat16() for s in ((few, D), (1, D), (few, 1)))
+    want_y = checkpointed_linear(x, w.requires_grad_())
+    kept = quantize_activation(x)
+    (want_dx,) = torch.autograd.grad(checkpointed_linear(x.requires_grad_(), w), x, dy)
+    leaf = x.detach().repeat(N // few + 1, 1)[:N].requires_grad_()
+    y = checkpointed_linear(leaf, w)
+    dx, dw = torch.autograd.grad(y, (leaf, w), dy.repeat(N // few + 1, 1)[:N])
+    for got, want in ((y.detach(), want_y.detach()), (dx, want_dx)):
+        whole = got[:N // few * few].view(-1, few, got.shape[-1])
+        assert torch.equal(whole.amin(0), whole.amax(0)) and torch.equal(got[:few], want) and torch.equal(got[-(N % few):], want[:N % few])
+    # sums of one wave's every 8th row of 256 splits, 32769 roundings, then 8 waves and 256 splits: under 34000 of the sum of magnitudes
+    parts = dy.double().T @ kept.dequantize().double()
+    size = dy.double().abs().T @ kept.dequantize().double().abs()
+    times = N / few
+    rest = dy.double()[:N % few].T @ kept.dequantize().double()[:N % few]
+    whole_sum = parts * (N // few) + rest
+    O.assert_close(dw, whole_sum.cpu(), (34000 * O.U * size * (times + 1)).cpu(), "dw")
+    del leaf, y, dx, dw, got, whole
+    row = torch.randn(1, 512, device="cuda").bfloat16()
+    q = quantize_activation(row.expand(N, 512))  # 2^35 elements and some
+    one = quantize_activation(row)
+    back = q.dequantize()
+    values = one.dequantize()
+    for i in range(0, N, 1 << 23):
+        assert torch.equal(q.codes[i:i + (1 << 23)], one.codes.expand(min(1 << 23, N - i), -1))
+        assert torch.equal(back[i:i + (1 << 23)], values.expand(min(1 << 23, N - i), -1))
+    assert torch.equal(q.exponents, one.exponents.expand(N, -1))
+    del q, back
+    torch.cuda.empty_cache()

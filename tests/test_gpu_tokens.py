@@ -672,3 +672,42 @@ def test_in_place_beside_and_over_other_inputs():
     assert torch.equal(z, want) and torch.equal(bias, kept)
     with pytest.raises(RuntimeError, match="share no memory"):  # row 0 is a bias of every row
         process_logits(z, bias=z[0], out=z)
+
+
+def test_more_rows_than_a_launch_takes():
+    """2^26 sequences of one row and more are several launches: the bits of the same rows alone, on both sides of every seam."""
+    N, V, few = (1 << 26) + 37, 16, 1 << 10
+    g = torch.Generator("cuda").manual_seed(3)
+    base = {"z": torch.randn(few, V, generator=g, device="cuda").bfloat16(), "tokens": torch.randint(0, V, (few, 2), generator=g, device="cuda", dtype=torch.int32),
+            "lengths": torch.randint(0, 3, (few,), generator=g, device="cuda", dtype=torch.int32),
+            "prompt": torch.randint(0, 3, (few,), generator=g, device="cuda", dtype=torch.int32), "temp": torch.rand(few, generator=g, device="cuda") + 0.5,
+            "mask": torch.randint(1, 1 << V, (few, 1), generator=g, device="cuda", dtype=torch.int32),
+            "bias": torch.randn(few, V, generator=g, device="cuda").bfloat16(), "action": torch.randint(-1, V, (few,), generator=g, device="cuda", dtype=torch.int32),
+            "a": torch.randn(few, generator=g, device="cuda"), "b": torch.randn(few, generator=g, device="cuda"),
+            "g": torch.randn(few, V, generator=g, device="cuda").bfloat16()}
+    many = {k: x.repeat(N // few + 1, *[1] * (x.ndim - 1))[:N] for k, x in base.items()}
+
+    def call(c):
+        kw = dict(tokens=c["tokens"], lengths=c["lengths"], prompt_lengths=c["prompt"], repetition_penalty=1.5, presence_penalty=0.5, frequency_penalty=0.25,
+                  bias=c["bias"], mask=c["mask"], temperature=c["temp"])
+        leaf = c["z"].requires_grad_()
+        out = process_logits(leaf, **kw)
+        (d_out,) = torch.autograd.grad(out, leaf, c["g"])
+        lp, H = token_log_prob(leaf, c["action"], entropy=True, **kw)
+        (d,) = torch.autograd.grad((lp, H), leaf, (c["a"], c["b"]))
+        return out.detach(), d_out, lp.detach(), H.detach(), d
+
+    want = call(base)
+    got = call(many)
+    for x, w in zip(got, want):
+        whole = x[:N // few * few].unflatten(0, (-1, few)).view(torch.int16 if x.dtype == torch.bfloat16 else torch.int32)
+        assert torch.equal(whole.amin(0), whole.amax(0)) and same(x[:few], w) and same(x[-(N % few):], w[:N % few])
+    del many, got, whole, x
+    # nine sub-slices a row, joined by a wave: rows that lie on one another
+    z = torch.randn(1, 16500, generator=g, device="cuda").bfloat16()
+    action = torch.arange(N, device="cuda", dtype=torch.int32) % 16500
+    lp = token_log_prob(z.expand(N, -1), action)
+    want = token_log_prob(z.expand(16500, -1), torch.arange(16500, device="cuda"))
+    assert torch.equal(lp, want.repeat(N // 16500 + 1)[:N])
+    del lp, action
+    torch.cuda.empty_cache()

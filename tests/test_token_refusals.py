@@ -203,3 +203,13 @@ def test_out_shares_no_memory_with_the_inputs_but_the_logits():
         _out_rows(processing(z), z, torch.zeros(1, 40).expand(4, 40))
     with pytest.raises(RuntimeError, match="shape, dtype"):
         _out_rows(processing(z), z, z.half())
+
+
+def test_more_rows_of_a_sequence_than_a_launch_takes():
+    """2^32 threads and more: refused before anything is launched (sequences beyond that go in several launches)."""
+    lib = _extension.get_lib()
+    long = dict(B=1, T=1 << 33, V=4)
+    assert lib.trl_process_logits_fwd(None, token_args(**long)) == 2 and b"more rows" in lib.trl_last_error()
+    assert lib.trl_process_logits_bwd(None, token_args(**long)) == 2 and lib.trl_token_log_prob_bwd(None, token_args(**long)) == 2
+    assert lib.trl_token_log_prob_fwd(None, token_args(**long), 64, 1 << 60) == 2
+    assert lib.trl_token_log_prob_fwd(None, token_args(B=1, T=1 << 27, V=20000), 64, 1 << 60) == 2  # the rows' kernel would fit, joining would not

@@ -456,6 +456,7 @@ __global__ __launch_bounds__(WM *WN *kWave, BM == 256 ? 2 : 1) void act_weight_g
 
 // Adds the parts of a split sum in a fixed order; bound by a launch's latency.  Few parts: a thread a column (3 parts of 515 x 1027: 4.1 us,
 // 7.4 with 8 threads a column).  Many: 8 threads a column, a share of the parts each (256 parts of 256 columns: 5 us and 13).
+constexpr int kFewParts = 16;
 template <typename T, int GROUPS>
 __global__ __launch_bounds__(256) void act_join_kernel(const float *parts, int splits, i64 n_w, i64 n_b, T *dw, T *db) {
     constexpr int kCols = 256 / GROUPS;
@@ -649,27 +650,46 @@ void launch_weight_grad_t(hipStream_t s, const WeightGradArgs &a, const WeightGr
         auto join = [&](auto kernel, int cols) {
             hipLaunchKernelGGL(kernel, dim3((unsigned)((n_w + n_b + cols - 1) / cols)), dim3(256), 0, s, a.parts, a.splits, n_w, n_b, (T *)a.dw, (T *)a.db);
         };
-        if (a.splits > 16) join(act_join_kernel<T, 8>, 32);
+        if (a.splits > kFewParts) join(act_join_kernel<T, 8>, 32);
         else join(act_join_kernel<T, 1>, 256);
     }
 }
 
 }  // namespace
 
+// Calls launch(first row, rows) on runs of rows that one launch can take, `each` being the threads of one.
+template <typename F>
+static void in_launches(i64 N, i64 each, F launch) {
+    const i64 most = kMostThreads / each;
+    for (i64 r = 0; r < N; r += most) launch(r, N - r < most ? N - r : most);
+}
+
 void launch_act_quantize(hipStream_t s, int dtype, const void *x, i64 stride, i64 N, i64 D, int8_t *codes, u8 *exponents) {
     const u32 G = (u32)((D + kActBlock - 1) / kActBlock * kGroups);
-    const dim3 grid((unsigned)((N * G + 255) / 256));
-    if (dtype == TRL_F32) hipLaunchKernelGGL(act_quantize_kernel<float>, grid, dim3(256), 0, s, (const float *)x, stride, N, D, G, codes, exponents);
-    else if (dtype == TRL_BF16) hipLaunchKernelGGL(act_quantize_kernel<__bf16>, grid, dim3(256), 0, s, (const __bf16 *)x, stride, N, D, G, codes, exponents);
-    else hipLaunchKernelGGL(act_quantize_kernel<_Float16>, grid, dim3(256), 0, s, (const _Float16 *)x, stride, N, D, G, codes, exponents);
+    auto launch = [&](auto t) {
+        typedef decltype(t) T;
+        in_launches(N, G, [&](i64 r, i64 n) {
+            hipLaunchKernelGGL(act_quantize_kernel<T>, dim3((unsigned)((n * G + 255) / 256)), dim3(256), 0, s, (const T *)x + r * stride, stride, n, D, G,
+                               codes + r * G * kVec, exponents + r * G / kGroups);
+        });
+    };
+    if (dtype == TRL_F32) launch(0.0f);
+    else if (dtype == TRL_BF16) launch((__bf16)0.0f);
+    else launch((_Float16)0.0f);
 }
 
 void launch_act_dequantize(hipStream_t s, int dtype, const int8_t *codes, const u8 *exponents, i64 N, i64 D, void *out) {
     const u32 G = (u32)((D + kActBlock - 1) / kActBlock * kGroups);
-    const dim3 grid((unsigned)((N * G + 255) / 256));
-    if (dtype == TRL_F32) hipLaunchKernelGGL(act_dequantize_kernel<float>, grid, dim3(256), 0, s, codes, exponents, N, D, G, (float *)out);
-    else if (dtype == TRL_BF16) hipLaunchKernelGGL(act_dequantize_kernel<__bf16>, grid, dim3(256), 0, s, codes, exponents, N, D, G, (__bf16 *)out);
-    else hipLaunchKernelGGL(act_dequantize_kernel<_Float16>, grid, dim3(256), 0, s, codes, exponents, N, D, G, (_Float16 *)out);
+    auto launch = [&](auto t) {
+        typedef decltype(t) T;
+        in_launches(N, G, [&](i64 r, i64 n) {
+            hipLaunchKernelGGL(act_dequantize_kernel<T>, dim3((unsigned)((n * G + 255) / 256)), dim3(256), 0, s, codes + r * G * kVec,
+                               exponents + r * G / kGroups, n, D, G, (T *)out + r * D);
+        });
+    };
+    if (dtype == TRL_F32) launch(0.0f);
+    else if (dtype == TRL_BF16) launch((__bf16)0.0f);
+    else launch((_Float16)0.0f);
 }
 
 size_t act_weight_grad_workspace(int dtype, i64 N, i64 O, i64 D) {
@@ -679,10 +699,12 @@ size_t act_weight_grad_workspace(int dtype, i64 N, i64 O, i64 D) {
 
 void launch_act_head(hipStream_t s, int dtype, const void *x, i64 stride, i64 N, i64 D, const void *w, const void *bias, int8_t *codes, u8 *exponents, void *y) {
     const u32 G = (u32)((D + kActBlock - 1) / kActBlock * kGroups);
-    const dim3 grid((unsigned)((N + 3) / 4));
     auto launch = [&](auto t) {
         typedef decltype(t) T;
-        hipLaunchKernelGGL(act_head_kernel<T>, grid, dim3(256), 0, s, (const T *)x, stride, N, D, G, (const T *)w, (const T *)bias, codes, exponents, (T *)y);
+        in_launches(N, kWave, [&](i64 r, i64 n) {
+            hipLaunchKernelGGL(act_head_kernel<T>, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, s, (const T *)x + r * stride, stride, n, D, G, (const T *)w,
+                               (const T *)bias, codes + r * G * kVec, exponents + r * G / kGroups, (T *)y + r);
+        });
     };
     if (dtype == TRL_F32) launch(0.0f);
     else if (dtype == TRL_BF16) launch((__bf16)0.0f);
@@ -692,7 +714,8 @@ void launch_act_head(hipStream_t s, int dtype, const void *x, i64 stride, i64 N,
 int launch_act_weight_grad(hipStream_t s, int dtype, const void *dy, i64 dy_stride, const int8_t *codes, const u8 *exponents, i64 N, i64 O,
                            i64 D, void *dw, void *db, void *workspace, const void *w, void *dx) {
     const WeightGradPlan p = weight_grad_plan(dtype, N, O, D);
-    if (p.tiles * p.splits > 0x7fffffffLL || (O * (D + 1) + 31) / 32 > 0x7fffffffLL) return 2;
+    // 512 threads a block at most; parts of a split sum are joined by up to 8 a column
+    if (p.tiles * p.splits > kMostThreads / 512 || (p.splits > 1 && O * (D + 1) > kMostThreads / (p.splits > kFewParts ? 8 : 1))) return 2;
     const WeightGradArgs a{dy, dy_stride, codes, exponents, N, O, D, (D + kActBlock - 1) / kActBlock * kActBlock, (int)p.tiles_d, (int)p.tiles, p.part, dw, db,
                            (float *)workspace, p.splits, w, dx};
     if (dtype == TRL_F32) launch_weight_grad_t<float>(s, a, p);

@@ -828,7 +828,7 @@ int trl_process_logits_fwd(void *stream, const trl_token_args *args) {
     if (empty) return TRL_OK;
     if (!args->logits || !args->out) return fail(TRL_ERR_INVALID_ARGUMENT, "trl_process_logits_fwd: null pointer");
     TokenArgs a{*args, nullptr, nullptr, 0, 0, 0, 0};
-    if (launch_process_logits((hipStream_t)stream, a)) return fail(TRL_ERR_UNSUPPORTED, "trl_process_logits_fwd: too many rows for one launch");
+    if (launch_process_logits((hipStream_t)stream, a)) return fail(TRL_ERR_UNSUPPORTED, "trl_process_logits_fwd: more rows in a sequence than one launch takes");
     if (int rc = check_launch("trl_process_logits_fwd")) return rc;
     g_kernel = "process_logits";
     return TRL_OK;
@@ -841,7 +841,7 @@ int trl_process_logits_bwd(void *stream, const trl_token_args *args) {
     const bool needs_z = args->tokens && (args->rep_t || args->rep != 1.0f);
     if (!args->grad_out || !args->out || (needs_z && !args->logits)) return fail(TRL_ERR_INVALID_ARGUMENT, "trl_process_logits_bwd: null pointer");
     TokenArgs a{*args, nullptr, nullptr, 0, 0, 0, 0};
-    if (launch_process_logits_bwd((hipStream_t)stream, a)) return fail(TRL_ERR_UNSUPPORTED, "trl_process_logits_bwd: too many rows for one launch");
+    if (launch_process_logits_bwd((hipStream_t)stream, a)) return fail(TRL_ERR_UNSUPPORTED, "trl_process_logits_bwd: more rows in a sequence than one launch takes");
     if (int rc = check_launch("trl_process_logits_bwd")) return rc;
     g_kernel = "process_logits_bwd";
     return TRL_OK;
@@ -862,7 +862,7 @@ int trl_token_log_prob_fwd(void *stream, const trl_token_args *args, void *works
         return fail(TRL_ERR_WORKSPACE, "trl_token_log_prob_fwd: workspace is %zu bytes, need %zu (16-byte aligned)", workspace_bytes, need);
     float *partials = (float *)workspace;
     TokenArgs a{*args, partials, partials + (size_t)args->B * (size_t)args->T * (size_t)token_subs(args->V) * 4, 0, 0, 0, 0};
-    if (launch_token_log_prob((hipStream_t)stream, a)) return fail(TRL_ERR_UNSUPPORTED, "trl_token_log_prob_fwd: too many rows for one launch");
+    if (launch_token_log_prob((hipStream_t)stream, a)) return fail(TRL_ERR_UNSUPPORTED, "trl_token_log_prob_fwd: more rows in a sequence than one launch takes");
     if (int rc = check_launch("trl_token_log_prob_fwd")) return rc;
     g_kernel = "token_log_prob";
     return TRL_OK;
@@ -876,7 +876,7 @@ int trl_token_log_prob_bwd(void *stream, const trl_token_args *args) {
         (!args->g_entropy && !args->g_log_prob))
         return fail(TRL_ERR_INVALID_ARGUMENT, "trl_token_log_prob_bwd: null pointer");
     TokenArgs a{*args, nullptr, nullptr, 0, 0, 0, 0};
-    if (launch_token_log_prob_bwd((hipStream_t)stream, a)) return fail(TRL_ERR_UNSUPPORTED, "trl_token_log_prob_bwd: too many rows for one launch");
+    if (launch_token_log_prob_bwd((hipStream_t)stream, a)) return fail(TRL_ERR_UNSUPPORTED, "trl_token_log_prob_bwd: more rows in a sequence than one launch takes");
     if (int rc = check_launch("trl_token_log_prob_bwd")) return rc;
     g_kernel = "token_log_prob_bwd";
     return TRL_OK;
@@ -886,7 +886,7 @@ int trl_token_log_prob_bwd(void *stream, const trl_token_args *args) {
 static int check_act_dims(const char *fn, int dtype, int64_t N, int64_t D) {
     if (!low_dtype_ok(dtype)) return fail(TRL_ERR_INVALID_ARGUMENT, "%s: bad dtype", fn);
     if (N < 0 || D <= 0 || N > 0x7fffffffLL || D > 0x7fffffe0LL) return fail(TRL_ERR_INVALID_ARGUMENT, "%s: bad sizes (N %lld, D %lld)", fn, (long long)N, (long long)D);
-    if ((D + kActBlock - 1) / kActBlock * N > 0x7fffffffLL * 64) return fail(TRL_ERR_UNSUPPORTED, "%s: too large for one launch", fn);
+    if ((D + kActBlock - 1) / kActBlock * N > 0x7fffffffLL * 64) return fail(TRL_ERR_UNSUPPORTED, "%s: too large", fn);
     return TRL_OK;
 }
 
@@ -938,7 +938,7 @@ int trl_act_weight_grad(void *stream, int dtype, const void *dy, int64_t dy_stri
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
         return fail(TRL_ERR_WORKSPACE, "trl_act_weight_grad: workspace is %zu bytes, need %zu (16-byte aligned)", workspace_bytes, need);
     if (launch_act_weight_grad((hipStream_t)stream, dtype, dy, dy_stride, codes, exponents, N, O, D, dw, db, workspace))
-        return fail(TRL_ERR_UNSUPPORTED, "trl_act_weight_grad: too large for one launch");
+        return fail(TRL_ERR_UNSUPPORTED, "trl_act_weight_grad: too large");
     if (int rc = check_launch("trl_act_weight_grad")) return rc;
     g_kernel = dw ? "act_weight_grad" : "act_column_sum";
     return TRL_OK;
@@ -953,7 +953,7 @@ int trl_act_head_bwd(void *stream, int dtype, const void *dy, int64_t dy_stride,
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
         return fail(TRL_ERR_WORKSPACE, "trl_act_head_bwd: workspace is %zu bytes, need %zu (16-byte aligned)", workspace_bytes, need);
     if (launch_act_weight_grad((hipStream_t)stream, dtype, dy, dy_stride, codes, exponents, N, 1, D, dw, db, workspace, w, dx))
-        return fail(TRL_ERR_UNSUPPORTED, "trl_act_head_bwd: too large for one launch");
+        return fail(TRL_ERR_UNSUPPORTED, "trl_act_head_bwd: too large");
     if (int rc = check_launch("trl_act_head_bwd")) return rc;
     g_kernel = "act_head_bwd";
     return TRL_OK;

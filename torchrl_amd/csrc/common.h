@@ -174,6 +174,9 @@ struct VtraceBwdArgs {
 
 // Host-side launchers (defined in the .hip files, called from capi.hip).  Each returns the
 // number of per-block partials it wrote (gae only) or a negative value when unsupported.
+// A launch counts its threads a dimension in 32 bits: the most that whole blocks of up to 256 can have.
+constexpr i64 kMostThreads = 0xffffff00LL;
+
 struct LaunchResult { int status; i64 npartials; const char *kernel; };
 
 LaunchResult launch_gae_seq(hipStream_t s, int vdt, int cdt, const GaeArgs &a);

@@ -688,6 +688,45 @@ __global__ __launch_bounds__(256) void token_join_kernel(TokenArgs a) {
     join_row<WAVE>(a, r, y, (const float4 *)a.partials + r * a.nsubs, a.nsubs, y >= 0 && y < a.V ? a.z_action[r] : 0.0f);
 }
 
+template <typename P>
+void advance(P *&p, i64 bytes) { if (p) p = (P *)((uintptr_t)p + (uintptr_t)bytes); }
+
+// The n sequences from b0 on: rows of different sequences share nothing but strides.
+TokenArgs sequences(const TokenArgs &a, i64 b0, i64 n) {
+    TokenArgs p = a;
+    auto width = [](int wide) -> i64 { return wide ? 8 : 4; };
+    const i64 r0 = b0 * a.T, es = a.dtype == TRL_F32 ? 4 : 2;
+    advance(p.logits, b0 * a.logits_sb * es);
+    advance(p.out, b0 * a.out_sb * es);
+    advance(p.grad_out, r0 * a.V * es);
+    advance(p.tokens, b0 * a.tokens_sb * width(a.tokens_wide));
+    advance(p.lengths, r0 * width(a.lengths_wide));
+    advance(p.prompt, b0 * width(a.prompt_wide));
+    advance(p.action, r0 * width(a.action_wide));
+    advance(p.bias, b0 * a.bias_sb);
+    advance(p.mask, b0 * a.mask_sb);
+    for (const float **x : {&p.rep_t, &p.pres_t, &p.freq_t, &p.temp_t}) advance(*x, b0 * 4);
+    for (float **x : {&p.log_prob, &p.entropy, &p.z_action}) advance(*x, r0 * 4);
+    for (const float **x : {&p.g_log_prob, &p.g_entropy}) advance(*x, r0 * 4);
+    advance(p.stats, r0 * 8);
+    advance(p.partials, r0 * a.nsubs * 16);
+    p.B = n;
+    return p;
+}
+
+// Calls launch(args) on runs of sequences that one launch can take, `each` being the threads of one; 2 where a single sequence needs more.
+template <typename F>
+int in_launches(const TokenArgs &a, i64 each, F launch) {
+    const i64 most = kMostThreads / each;
+    if (most == 0) return 2;
+    if (a.B <= most) {
+        launch(a);
+    } else {
+        for (i64 b = 0; b < a.B; b += most) launch(sequences(a, b, a.B - b < most ? a.B - b : most));
+    }
+    return 0;
+}
+
 // Blocks of as many waves as an even split of the vocabulary gives them, up to 8 beside a history: two such blocks share a compute unit,
 // and one streams while the other counts.  Up to 16, one block a unit, where the counting is shared by enough: long histories, or runs of
 // many rows (16 waves and 8: 256 x 131072 bf16 with 4096 tokens 35 us and 37; 8192 x 131072 bf16 with every step on, backward, 800 and 852,
@@ -714,11 +753,11 @@ int launch_waves(hipStream_t s, TokenArgs &a) {
         if (c == 1 || cost < best) { best = cost; a.chunk = c; }
     }
     a.nchunks = (a.T + a.chunk - 1) / a.chunk;
-    const i64 grid = a.nslices * a.nchunks * a.B;
-    if (grid > 0x7fffffffLL) return 2;
+    const i64 threads = waves * kWave, blocks = a.nslices * a.nchunks;  // blocks of a sequence
     const size_t lds = (PEN ? waves * kSub * sizeof(u32) : 0);
-    hipLaunchKernelGGL((token_kernel<T, MODE, PEN, BIAS>), dim3((unsigned)grid), dim3((unsigned)waves * kWave), lds, s, a);
-    return 0;
+    return in_launches(a, blocks * threads, [&](const TokenArgs &p) {
+        hipLaunchKernelGGL((token_kernel<T, MODE, PEN, BIAS>), dim3((unsigned)(blocks * p.B)), dim3((unsigned)threads), lds, s, p);
+    });
 }
 template <typename T, int MODE>
 int launch_mode(hipStream_t s, TokenArgs &a) {
@@ -743,15 +782,16 @@ i64 token_subs(i64 V) { return (V + kSub - 1) / kSub; }
 int launch_process_logits(hipStream_t s, TokenArgs a) { return launch_dtype<kProcess>(s, a); }
 int launch_process_logits_bwd(hipStream_t s, TokenArgs a) { return launch_dtype<kProcessBwd>(s, a); }
 int launch_token_log_prob(hipStream_t s, TokenArgs a) {
-    const int rc = launch_dtype<kLogProb>(s, a);
-    if (rc) return rc;
     a.nsubs = token_subs(a.V);
-    if (a.nsubs == 1) return 0;
     const bool wave = a.nsubs > kSerialSubs;
-    const i64 blocks = wave ? (a.B * a.T + 3) / 4 : (a.B * a.T + 255) / 256;
-    if (blocks > 0x7fffffffLL) return 2;
-    if (wave) hipLaunchKernelGGL(token_join_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(token_join_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, s, a);
-    return 0;
+    const i64 joining = a.T * (wave ? kWave : 1);  // threads of a sequence
+    if (a.nsubs > 1 && joining > kMostThreads) return 2;
+    const int rc = launch_dtype<kLogProb>(s, a);
+    if (rc || a.nsubs == 1) return rc;
+    return in_launches(a, joining, [&](const TokenArgs &p) {
+        const i64 rows = p.B * p.T;
+        if (wave) hipLaunchKernelGGL(token_join_kernel<true>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, p);
+        else hipLaunchKernelGGL(token_join_kernel<false>, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, s, p);
+    });
 }
 int launch_token_log_prob_bwd(hipStream_t s, TokenArgs a) { return launch_dtype<kLogProbBwd>(s, a); }
