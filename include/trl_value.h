@@ -556,7 +556,7 @@ size_t trl_act_weight_grad_workspace_bytes(int dtype, int64_t N, int64_t O, int6
 int trl_act_weight_grad(void *stream, int dtype, const void *dy, int64_t dy_stride, const int8_t *codes, const uint8_t *exponents,
                         int64_t N, int64_t O, int64_t D, void *dw, void *db, void *workspace, size_t workspace_bytes);
 /* A layer of one output (a value head), w (D), in one pass each way.  fwd: y (N) = x w + bias (one element, or NULL), summed in 32 bits,
- * while x is quantized.  bwd: dw (D) and db as trl_act_weight_grad with O == 1 (and its workspace), and dx (N, D) = dy w, dense, unless
+ * while x is quantized (codes and exponents NULL: nothing is kept; y has the same bits).  bwd: dw (D) and db as trl_act_weight_grad with O == 1 (and its workspace), and dx (N, D) = dy w, dense, unless
  * dx is NULL (then w may be, too). */
 int trl_act_head_fwd(void *stream, int dtype, const void *x, int64_t x_stride, int64_t N, int64_t D, const void *w, const void *bias,
                      int8_t *codes, uint8_t *exponents, void *y);

@@ -555,3 +555,39 @@ def test_more_rows_than_a_launch_takes():
     assert torch.equal(q.exponents, one.exponents.expand(N, -1))
     del q, back
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("route", ["host", "python", "compiled"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("out", [1, 3])
+def test_the_same_output_in_training_and_evaluation(out, dtype, route, monkeypatch):
+    if route == "python":
+        monkeypatch.setattr(F, "_HOST", None)
+    torch._dynamo.reset()
+    x = inputs(300, 1100, dtype, seed=5).clamp(-30, 30).cuda().view(3, 100, 1100)
+    layer = CheckpointedLinear(1100, out, device="cuda", dtype=dtype)
+    f = torch.compile(layer, fullgraph=True) if route == "compiled" else layer
+    want = layer(x).detach()  # the weight wants a gradient
+    assert torch.equal(f(x).detach(), want)
+    with torch.no_grad():
+        assert torch.equal(f(x), want)
+    with torch.inference_mode():
+        assert torch.equal(f(x), want)
+    layer.weight.requires_grad_(False)
+    assert torch.equal(f(x.clone().requires_grad_()).detach(), want)
+    layer.bias.requires_grad_(False)
+    y = f(x)
+    assert torch.equal(y, want) and not y.requires_grad
+    if out == 1:
+        assert F.last_kernel() == "act_head"
+
+
+def test_the_python_route_keeps_nothing_without_a_gradient(monkeypatch):
+    monkeypatch.setattr(F, "_HOST", None)
+    x, layer = torch.randn(4096, 1024, device="cuda"), CheckpointedLinear(1024, 1, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        y = layer(x)
+    assert torch.cuda.max_memory_allocated() - before <= y.numel() * 4 + 4096

@@ -213,3 +213,8 @@ def test_more_rows_of_a_sequence_than_a_launch_takes():
     assert lib.trl_process_logits_bwd(None, token_args(**long)) == 2 and lib.trl_token_log_prob_bwd(None, token_args(**long)) == 2
     assert lib.trl_token_log_prob_fwd(None, token_args(**long), 64, 1 << 60) == 2
     assert lib.trl_token_log_prob_fwd(None, token_args(B=1, T=1 << 27, V=20000), 64, 1 << 60) == 2  # the rows' kernel would fit, joining would not
+
+
+def test_a_value_head_without_keeping():
+    lib = _extension.get_lib()
+    assert lib.trl_act_head_fwd(None, 0, 64, 8, 4, 8, 64, None, None, 64, 64) == 1 and lib.trl_act_head_fwd(None, 0, 64, 8, 4, 8, 64, None, 64, None, 64) == 1

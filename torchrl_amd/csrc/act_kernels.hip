@@ -67,7 +67,7 @@ __global__ __launch_bounds__(256) void act_quantize_kernel(const T *x, i64 strid
 // The forward pass of one output (a value head) while its input is quantized: y = x w + b on the way, one read of x.  A wave a row, 512
 // features at a time with the next ones on their way; w comes from the caches (two or four rows a wave read it less often, but hide less of
 // the latency: 8192 x 4096 bf16 18.7 us and 22.4 / 24.4).  Bound by HBM as the quantization alone: 5.4 TB/s, 19.0 us without the product.
-template <typename T>
+template <typename T, bool KEEP>
 __global__ __launch_bounds__(256) void act_head_kernel(const T *__restrict__ x, i64 stride, i64 N, i64 D, u32 G, const T *__restrict__ w, const T *__restrict__ bias,
                                                        int8_t *__restrict__ codes, u8 *__restrict__ exponents, T *__restrict__ y) {
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256) void act_head_kernel(const T *__restrict__ x, 
         unpack8(p.w, vw);
 #pragma unroll
         for (int i = 0; i < kVec; ++i) sum = fmaf(v[i], vw[i], sum);
-        quantize8(v, row * G + group, codes, exponents);
+        if constexpr (KEEP) quantize8(v, row * G + group, codes, exponents);
     };
     now = fetch(lane);
     for (u32 g = 0; g < G; g += 2 * kWave) {
@@ -701,9 +701,10 @@ void launch_act_head(hipStream_t s, int dtype, const void *x, i64 stride, i64 N,
     const u32 G = (u32)((D + kActBlock - 1) / kActBlock * kGroups);
     auto launch = [&](auto t) {
         typedef decltype(t) T;
+        const auto kernel = codes ? act_head_kernel<T, true> : act_head_kernel<T, false>;
         in_launches(N, kWave, [&](i64 r, i64 n) {
-            hipLaunchKernelGGL(act_head_kernel<T>, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, s, (const T *)x + r * stride, stride, n, D, G, (const T *)w,
-                               (const T *)bias, codes + r * G * kVec, exponents + r * G / kGroups, (T *)y + r);
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, s, (const T *)x + r * stride, stride, n, D, G, (const T *)w,
+                               (const T *)bias, codes ? codes + r * G * kVec : nullptr, codes ? exponents + r * G / kGroups : nullptr, (T *)y + r);
         });
     };
     if (dtype == TRL_F32) launch(0.0f);

@@ -904,7 +904,7 @@ int trl_act_head_fwd(void *stream, int dtype, const void *x, int64_t x_stride, i
                      uint8_t *exponents, void *y) {
     if (int rc = check_act_dims("trl_act_head_fwd", dtype, N, D)) return rc;
     if (N == 0) return TRL_OK;
-    if (!x || !w || !y || !codes || !exponents || ((uintptr_t)codes & 15))
+    if (!x || !w || !y || !codes != !exponents || ((uintptr_t)codes & 15))
         return fail(TRL_ERR_INVALID_ARGUMENT, "trl_act_head_fwd: null pointer, or codes not 16-byte aligned");
     launch_act_head((hipStream_t)stream, dtype, x, x_stride, N, D, w, bias, codes, exponents, y);
     if (int rc = check_launch("trl_act_head_fwd")) return rc;

@@ -305,28 +305,36 @@ at::Tensor as_rows(const at::Tensor &x) {
     const at::Tensor r = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
     return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
 }
-// of x; with `y`, the output of the one-output layer (w, b) too
-int quantize(const at::Tensor &x, at::Tensor &codes, at::Tensor &exponents, const at::Tensor &w = {}, const at::Tensor &b = {}, at::Tensor *y = nullptr) {
+void empty_kept(const at::Tensor &x, at::Tensor &codes, at::Tensor &exponents) {
     auto shape = x.sizes().vec();
-    const int64_t D = shape.back(), blocks = (D + 31) / 32;
+    const int64_t blocks = (shape.back() + 31) / 32;
     shape.back() = blocks * 32;
     codes = at::empty(shape, x.options().dtype(at::kChar));
     shape.back() = blocks;
     exponents = at::empty(shape, x.options().dtype(at::kByte));
+}
+int quantize(const at::Tensor &x, at::Tensor &codes, at::Tensor &exponents) {
+    empty_kept(x, codes, exponents);
     const at::Tensor r = as_rows(x);
-    if (y) {
-        shape.back() = 1;
-        *y = at::empty(shape, x.options());
-        const at::Tensor row = w.contiguous();
-        return g_head_fwd(stream_of(x), dtype_code(x.scalar_type()), r.data_ptr(), r.stride(0), r.size(0), D, row.data_ptr(),
-                          b.defined() ? b.data_ptr() : nullptr, (int8_t *)codes.data_ptr(), (uint8_t *)exponents.data_ptr(), y->data_ptr());
-    }
-    return g_quantize(stream_of(x), dtype_code(x.scalar_type()), r.data_ptr(), r.stride(0), r.size(0), D, (int8_t *)codes.data_ptr(),
+    return g_quantize(stream_of(x), dtype_code(x.scalar_type()), r.data_ptr(), r.stride(0), r.size(0), r.size(1), (int8_t *)codes.data_ptr(),
                       (uint8_t *)exponents.data_ptr());
 }
+// the layer of one output (w, b) of x, which is quantized on the way if it is to be kept
+int head(const at::Tensor &x, const at::Tensor &w, const at::Tensor &b, bool keep, at::Tensor &y, at::Tensor &codes, at::Tensor &exponents) {
+    auto shape = x.sizes().vec();
+    shape.back() = 1;
+    y = at::empty(shape, x.options());
+    if (keep) empty_kept(x, codes, exponents);
+    const at::Tensor r = as_rows(x), row = w.contiguous();
+    return g_head_fwd(stream_of(x), dtype_code(x.scalar_type()), r.data_ptr(), r.stride(0), r.size(0), r.size(1), row.data_ptr(),
+                      b.defined() ? b.data_ptr() : nullptr, keep ? (int8_t *)codes.data_ptr() : nullptr, keep ? (uint8_t *)exponents.data_ptr() : nullptr,
+                      y.data_ptr());
+}
 
-// Up to here a layer of one output runs in one pass over x: 8192 x 4096 bf16 19 us, 36 as two calls; 37 x 16384 18 and 23, 300 x 65536 75 and 88,
-// 1000 x 100000 158 and 166.  A wave walks a row: wider ones are the library's and the quantization's.
+// Up to here a layer of one output runs in one pass over x, whether x is kept or not: the same bits in training and evaluation.  Against the library's
+// product and a quantization, us, bf16: 8192 x 4096 19 and 36, 256 x 16384 17 and 20, 300 x 65536 75 and 88; a wave walks a row, so with few rows the
+// width decides: 1 x 16384 14 and 19, 1 x 65536 51 and 49, 64 x 65536 58 and 52, 1000 x 100000 158 and 166 -- wider ones are the library's.  Without
+// keeping: 4096 x 4096 5 and 15, 1 x 65536 26 and 47.  fp32 4 to 10 times ahead of the library's product.
 constexpr int64_t kHeadFeatures = 65536;
 
 struct CheckpointedLinearBackward : torch::autograd::Node {
@@ -487,8 +495,8 @@ PyObject *py_checkpointed_linear(PyObject *, PyObject *const *o, Py_ssize_t narg
     {
         c10::AutoGradMode off(false);
         int rc = 0;
-        if (gw && w.size(0) == 1 && w.size(1) <= kHeadFeatures) {
-            rc = quantize(x, codes, exponents, w, b, &y);
+        if (w.size(0) == 1 && w.size(1) <= kHeadFeatures) {
+            rc = head(x, w, b, gw, y, codes, exponents);
         } else {
             // below the view tracking: the product folds batch dims and comes back as a view, which may not be written in place once it has a history
             at::AutoDispatchBelowADInplaceOrView untracked;

@@ -551,7 +551,7 @@ def checkpointed_linear_op(x: Tensor, weight: Tensor, bias: Optional[Tensor]) ->
     from torchrl_amd.objectives.value import kept_activations as K
     with torch.no_grad():
         K.checkpointed_linear_check(x, weight, bias)
-        return K._linear_and_kept(x, weight, bias)
+        return K._linear_and_kept(x, weight, bias, True)
 
 
 @checkpointed_linear_op.register_fake

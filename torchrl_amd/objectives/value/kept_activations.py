@@ -5,7 +5,8 @@ weights, fill the memory.  :func:`quantize_activation` keeps them at one byte an
 quarter of float32's); :func:`checkpointed_linear` / :class:`CheckpointedLinear` is the layer whose weight gradient is computed from them
 directly, in matrix instructions that read the bytes: the wide activations never come back to memory.  The output and the gradient of the input
 are those of an ordinary linear layer; only the weight gradient sees the rounding (half a step of 2^-6 of the block's largest
-magnitude, less than one at the very top).  The format and the kernels are behind ``trl_act_*`` of include/trl_value.h.
+magnitude, less than one at the very top).  A layer of one output has a kernel of its own, so that its output has the same bits whether a
+gradient is wanted or not.  The format and the kernels are behind ``trl_act_*`` of include/trl_value.h.
 
 The reference has no counterpart.
 """
@@ -138,16 +139,24 @@ def _linear(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> Tensor:
     return torch.ops.aten._unsafe_view(y, y.shape) if y._is_view() else y
 
 
-def _linear_and_kept(x: Tensor, weight: Tensor, bias: Optional[Tensor]):
-    """(x W^T + b, codes, exponents); a layer of one output in one pass over x (host_policy.cpp has the measurements of the rule)."""
-    if weight.shape[0] != 1 or weight.shape[1] > HEAD_FEATURES or x.numel() == 0:
+def _is_head(x: Tensor, weight: Tensor) -> bool:
+    """Whether the layer runs in one pass of its own over x (host_policy.cpp has the measurements of the rule)."""
+    return weight.shape[0] == 1 and weight.shape[1] <= HEAD_FEATURES and x.numel() > 0
+
+
+def _linear_and_kept(x: Tensor, weight: Tensor, bias: Optional[Tensor], keep: bool):
+    """(x W^T + b, codes, exponents), the latter None unless ``keep``: y has the same bits either way."""
+    if not _is_head(x, weight):
+        y = _linear(x, weight, bias)
+        if not keep:
+            return y, None, None
         kept = quantize_activation(x)
-        return _linear(x, weight, bias), kept.codes, kept.exponents
-    codes, exponents = _empty_kept(x)
+        return y, kept.codes, kept.exponents
+    codes, exponents = _empty_kept(x) if keep else (None, None)
     y = torch.empty(*x.shape[:-1], 1, dtype=x.dtype, device=x.device)
     rows, w = _rows(x.detach()), weight.detach().contiguous()
     _call("trl_act_head_fwd", x.device, _DT[x.dtype], rows.data_ptr(), rows.stride(0), rows.shape[0], x.shape[-1], w.data_ptr(), _ptr(bias),
-          codes.data_ptr(), exponents.data_ptr(), y.data_ptr())
+          _ptr(codes), _ptr(exponents), y.data_ptr())
     return y, codes, exponents
 
 
@@ -178,11 +187,7 @@ def _weight_grad(dy: Tensor, codes: Optional[Tensor], exponents: Optional[Tensor
 class _CheckpointedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        codes = exponents = None
-        if ctx.needs_input_grad[1]:
-            y, codes, exponents = _linear_and_kept(x, weight, bias)
-        else:
-            y = _linear(x, weight, bias)
+        y, codes, exponents = _linear_and_kept(x, weight, bias, ctx.needs_input_grad[1])
         ctx.save_for_backward(codes, exponents, weight if ctx.needs_input_grad[0] else None)
         ctx.features = x.shape[-1]
         return y
@@ -225,6 +230,8 @@ def checkpointed_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None
         from torchrl_amd.objectives.value import _ops
         return _ops.checkpointed_linear(x, weight, bias)
     checkpointed_linear_check(x, weight, bias)
+    if not F._needs_grad(x, weight, bias):
+        return _linear_and_kept(x, weight, bias, False)[0]
     return _CheckpointedLinear.apply(x, weight, bias)
 
 
