@@ -70,3 +70,49 @@ def test_a_value_head_compiles_fullgraph():
 
     for a, b in zip(run(head), run(torch.compile(head, fullgraph=True))):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("out", [1, 24])
+@pytest.mark.parametrize("form", ["no_grad", "frozen weight", "bias alone", "all"])
+def test_a_compiled_layer_keeps_what_the_eager_one_keeps(form, out):
+    """No quantization and no weight gradient where the weight wants none; the same results."""
+    torch._dynamo.reset()
+    torch.manual_seed(0)
+    x, dy = torch.randn(5, 64, 512, device="cuda"), torch.randn(5, 64, out, device="cuda")
+    layer = CheckpointedLinear(512, out, device="cuda")
+    layer.weight.requires_grad_(form in ("no_grad", "all"))
+    graphs = []
+
+    def backend(graph, example_inputs):
+        from torch._dynamo.backends.common import aot_autograd
+
+        def seen(g, _):
+            graphs.append([str(n.target) for n in g.graph.nodes])
+            return g
+
+        return aot_autograd(fw_compiler=seen, bw_compiler=seen)(graph, example_inputs)
+
+    def run(f):
+        leaf = x.clone().requires_grad_(form != "bias alone")
+        layer.zero_grad()
+        if form == "no_grad":
+            with torch.no_grad():
+                return (f(leaf),)
+        y = f(leaf)
+        y.backward(dy)
+        return y.detach(), leaf.grad, layer.weight.grad, None if layer.bias.grad is None else layer.bias.grad.clone()
+
+    for a, b in zip(run(layer), run(torch.compile(layer, fullgraph=True, backend=backend))):
+        if a is None:
+            assert b is None
+        else:  # the bias's gradient is a sum of 320 numbers in two orders
+            torch.testing.assert_close(a, b, rtol=0, atol=320 * 2.0 ** -24 * 320 ** 0.5 * 4 if a.shape == (out,) and a.ndim == 1 else 0)
+    ops = [n for g in graphs for n in g]
+    kept = any("checkpointed_linear" in n or "weight_grad" in n or "head_grad" in n for n in ops)
+    assert ops and kept == (form == "all")
+
+
+def test_refused_layers_under_compile():
+    layer = CheckpointedLinear(40, 8)
+    with torch.no_grad(), pytest.raises(Exception, match="HIP"):
+        torch.compile(layer, fullgraph=True)(torch.zeros(3, 40))

@@ -597,12 +597,50 @@ def _checkpointed_linear_backward(ctx, grad, _codes, _exponents):
         dw, db, dx = activation_head_grad_op(dy, codes, exponents, ctx.features, weight)
         return dx.reshape(*grad.shape[:-1], ctx.features), dw, db if need[2] else None
     dx = (dy @ weight).reshape(*grad.shape[:-1], ctx.features) if need[0] else None
-    dw, db = activation_weight_grad_op(dy, codes, exponents, ctx.features) if need[1] or need[2] else (None, None)
-    return dx, dw if need[1] else None, db if need[2] else None
+    dw = db = None
+    if need[1]:
+        dw, db = activation_weight_grad_op(dy, codes, exponents, ctx.features)
+    elif need[2]:
+        db = dy.sum(0)
+    return dx, dw, db if need[2] else None
 
 
 checkpointed_linear_op.register_autograd(_checkpointed_linear_backward, setup_context=_checkpointed_linear_setup)
 
 
+@torch.library.custom_op(f"{_NS}::head_linear", mutates_args=())
+def head_linear_op(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> Tensor:
+    """A layer of one output whose weight wants no gradient: nothing is kept."""
+    from torchrl_amd.objectives.value import kept_activations as K
+    with torch.no_grad():
+        return K._linear_and_kept(x, weight, bias, False)[0]
+
+
+@head_linear_op.register_fake
+def _(x, weight, bias):
+    return torch.empty((*x.shape[:-1], 1), dtype=x.dtype, device=x.device)
+
+
+def _head_linear_setup(ctx, inputs, output):
+    x, weight, _ = inputs
+    ctx.save_for_backward(weight)
+    ctx.features = x.shape[-1]
+
+
+def _head_linear_backward(ctx, grad):
+    (weight,) = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dy = grad.reshape(-1, 1)
+    dx = (dy @ weight).reshape(*grad.shape[:-1], ctx.features) if need[0] else None
+    return dx, None, dy.sum(0) if need[2] else None
+
+
+head_linear_op.register_autograd(_head_linear_backward, setup_context=_head_linear_setup)
+
+
 def checkpointed_linear(x, weight, bias):
-    return checkpointed_linear_op(x, weight, bias)[0]
+    from torchrl_amd.objectives.value import kept_activations as K
+    K.checkpointed_linear_check(x, weight, bias)
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return checkpointed_linear_op(x, weight, bias)[0]
+    return head_linear_op(x, weight.detach(), bias) if K._is_head(x, weight) else torch.nn.functional.linear(x, weight, bias)
