@@ -316,7 +316,7 @@ PyObject *py_set_workspace(PyObject *, PyObject *args) {
 }
 
 #define DECLINE_UNLESS_TENSOR(obj) \
-    if (!THPVariable_Check(obj)) Py_RETURN_NONE
+    if (!THPVariable_Check(obj) || maybe_recorded()) Py_RETURN_NONE
 
 PyObject *py_gae(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     if (!ready(nargs, 10, "gae")) return nullptr;

@@ -58,9 +58,9 @@ void check_status(int rc, const char *what) {
     TORCH_CHECK(rc == 0, "torchrl_amd native call failed (status ", rc, "): ", g_last_error ? g_last_error() : what);
 }
 bool wants_grad(const at::Tensor &t) { return t.defined() && t.requires_grad() && c10::GradMode::is_enabled(); }
-// a tensor with memory of its own kind: no function transform's or subclass's wrapper, no forward-mode tangent
+// a tensor with memory of its own kind: no function transform's or subclass's wrapper, no forward-mode tangent, and nothing that records the call
 bool plain_tensor(PyObject *o, at::Tensor &t) {
-    if (!THPVariable_Check(o)) return false;
+    if (!THPVariable_Check(o) || maybe_recorded()) return false;
     t = THPVariable_Unpack(o);
     using c10::DispatchKey;
     constexpr c10::DispatchKeySet wrapped({DispatchKey::FuncTorchGradWrapper, DispatchKey::FuncTorchBatched, DispatchKey::Functionalize, DispatchKey::Python,
@@ -218,6 +218,12 @@ struct KeptProcessing {
     void release() { for (auto &v : t) v.reset_data(); }
 };
 
+// A gradient of a result that was computed before a recording began has no operator to write down: the recording would lack the kernel.
+void check_not_recorded() {
+    TORCH_CHECK(!c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value() && !torch::jit::tracer::isTracing(),
+                "torchrl_amd: this gradient cannot be recorded: record its forward pass too");
+}
+
 // The gradients of these operators are not differentiable again: where the incoming ones are, the results say so when that is tried.
 bool differentiable(const variable_list &grads) {
     if (!c10::GradMode::is_enabled()) return false;
@@ -238,6 +244,7 @@ struct ProcessLogitsBackward : torch::autograd::Node {
     KeptProcessing kept;
     variable_list apply(variable_list &&grads) override {
         if (!grads[0].defined()) return {at::Tensor()};
+        check_not_recorded();
         const bool again = differentiable(grads);
         at::Tensor d;
         {
@@ -265,6 +272,7 @@ struct TokenLogProbBackward : torch::autograd::Node {
     variable_list apply(variable_list &&grads) override {
         at::Tensor g_lp = grads[0], g_h = grads.size() > 1 ? grads[1] : at::Tensor(), d;
         if (!g_lp.defined() && !g_h.defined()) return {at::Tensor()};
+        check_not_recorded();
         const bool again = differentiable(grads);
         {
             c10::DeviceGuard guard((g_lp.defined() ? g_lp : g_h).device());
@@ -343,6 +351,7 @@ struct CheckpointedLinearBackward : torch::autograd::Node {
     bool need_x = false, need_w = false, need_b = false;
     variable_list apply(variable_list &&grads) override {
         if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
+        check_not_recorded();
         const bool again = differentiable(grads);
         at::Tensor dx, dw, db;
         {

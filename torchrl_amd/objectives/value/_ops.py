@@ -2,7 +2,7 @@
 
 SURVEY.md 8(b): the reference flips its estimators to the Python loop under dynamo (advantages.py:1303-1307); here every
 estimator is ONE opaque op with a fake (meta) implementation, so ``torch.compile(fullgraph=True)`` traces through a
-PPO-style function without graph breaks.  The ops are used ONLY while compiling (``torch.compiler.is_compiling()``):
+PPO-style function without graph breaks.  The ops are used ONLY while compiling or recording (``functional._recording``):
 the eager entry points call the library directly -- the dispatcher's per-call cost is several times the small kernels.
 
 Each op's implementation is the eager entry point itself (ctypes underneath); ``register_autograd`` wires the backward

@@ -239,8 +239,25 @@ def _ptr(t: Optional[torch.Tensor]):
     return t.data_ptr() if t is not None else None
 
 
+def _recorded() -> bool:
+    """Whether torch writes down the operations on plain tensors (``make_fx``, ``torch.jit.trace``): a direct call into the library would be
+    missing from the recording, which would hold its outputs' allocation alone."""
+    if torch._C._len_torch_dispatch_stack():
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+        if get_proxy_mode() is not None:
+            return True
+    return torch._C._get_tracing_state() is not None
+
+
+def _recording() -> bool:
+    """Whether the custom ops of _ops.py take the call."""
+    return torch.compiler.is_compiling() or _recorded()
+
+
 def _stream(device) -> int:
     """The caller's current hipStream_t on ``device`` as an integer handle."""
+    if _recorded():
+        raise RuntimeError("torchrl_amd: this call has no operator that make_fx or torch.jit.trace could record")
     idx = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if idx is None else idx)
 
@@ -986,6 +1003,8 @@ def _gae_fast(gamma, lmbda, state_value, next_state_value, reward, done, termina
         if out.__class__ is int:
             _extension.check(out, _extension.get_lib())
         return out
+    if _recorded():
+        return None
     pre = gamma if (gamma.__class__ is tuple and lmbda is None) else None
     if pre is None and (type(gamma) is not float or type(lmbda) is not float):
         return None
@@ -1089,13 +1108,14 @@ def generalized_advantage_estimate(
     Returns ``(advantage, value_target)``.  All tensors must have shape
     ``[*Batch x TimeSteps x *F]``; ``terminated`` defaults to ``done``.
     """
-    if torch.compiler.is_compiling():
+    compiling = torch.compiler.is_compiling()
+    out = None if compiling else _gae_fast(gamma, lmbda, state_value, next_state_value, reward, done, terminated, None, ALGO_AUTO, time_dim)
+    if out is not None:
+        return out
+    if compiling or _recorded():
         (g, gt), (l, lt) = _ops._split_leaf(gamma, next_state_value.shape, time_dim), _ops._split_leaf(lmbda, next_state_value.shape, time_dim)
         return _ops.gae_op(state_value, next_state_value, reward, done, done if terminated is None else terminated, g, l, gt, lt,
                            time_dim, False)
-    out = _gae_fast(gamma, lmbda, state_value, next_state_value, reward, done, terminated, None, ALGO_AUTO, time_dim)
-    if out is not None:
-        return out
     call = _prepare_gae(gamma, lmbda, state_value, next_state_value, reward, done, terminated, time_dim)
     if _needs_grad(state_value, next_state_value, reward, gamma, lmbda):
         return _GaeFunction.apply(state_value, next_state_value, reward, _coef_leaf(gamma, call.shape, time_dim),
@@ -1117,13 +1137,14 @@ def vec_generalized_advantage_estimate(
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Vectorized GAE (reference: functional.py:272-370).  Same kernels as the loop variant:
     the result is exact rather than filter-truncated."""
-    if torch.compiler.is_compiling():
+    compiling = torch.compiler.is_compiling()
+    out = None if compiling else _gae_fast(gamma, lmbda, state_value, next_state_value, reward, done, terminated, None, ALGO_AUTO, time_dim)
+    if out is not None:
+        return out
+    if compiling or _recorded():
         (g, gt), (l, lt) = _ops._split_leaf(gamma, next_state_value.shape, time_dim), _ops._split_leaf(lmbda, next_state_value.shape, time_dim)
         return _ops.gae_op(state_value, next_state_value, reward, done, done if terminated is None else terminated, g, l, gt, lt,
                            time_dim, True)
-    out = _gae_fast(gamma, lmbda, state_value, next_state_value, reward, done, terminated, None, ALGO_AUTO, time_dim)
-    if out is not None:
-        return out
     call = _prepare_gae(gamma, lmbda, state_value, next_state_value, reward, done, terminated, time_dim)
     call.out_dtype = _vec_gae_out_dtype(state_value.dtype, gamma, lmbda)
     if _needs_grad(state_value, next_state_value, reward, gamma, lmbda):
@@ -1219,16 +1240,17 @@ def gae_normalized(gamma, lmbda, state_value, next_state_value, reward, done, te
     scale pass, so every rank normalises with the global statistics.  ``exchange``
     (:class:`StatsExchange`, intra-node): the moments cross the GPUs inside the launch instead
     (peer-to-peer mailbox stores over xGMI) and the sharded step stays one launch per GPU."""
-    if torch.compiler.is_compiling():
+    compiling = torch.compiler.is_compiling()
+    if not compiling and exchange is None and group is None and not distributed:
+        out = _gae_fast(gamma, lmbda, state_value, next_state_value, reward, done, terminated, float(eps), algo, time_dim)
+        if out is not None:
+            return out
+    if compiling or _recorded():
         if exchange is not None or group is not None or distributed or algo != ALGO_AUTO:
             raise NotImplementedError("gae_normalized under torch.compile: single-GPU call only")
         (g, gt), (l, lt) = _ops._split(gamma), _ops._split(lmbda)
         return _ops.gae_normalized_op(state_value, next_state_value, reward, done, done if terminated is None else terminated, g, l,
                                       gt, lt, float(eps), time_dim)
-    if exchange is None and group is None and not distributed:
-        out = _gae_fast(gamma, lmbda, state_value, next_state_value, reward, done, terminated, float(eps), algo, time_dim)
-        if out is not None:
-            return out
     call = _prepare_gae(gamma, lmbda, state_value, next_state_value, reward, done, terminated, time_dim)
     if _needs_grad(state_value, next_state_value, reward, gamma, lmbda):
         # differentiable path: GAE through the autograd function, normalisation as the reference's torch ops
@@ -1311,7 +1333,7 @@ def standardize(x: torch.Tensor, eps: float, group=None, distributed: bool = Fal
     """Out-of-place ``(x - mean) / std.clamp_min(eps)`` over all elements.  With ``distributed``
     (or an explicit process ``group``) the fp64 moments are all-reduced first -- one 24-byte RCCL
     all-reduce -- so every rank normalises with the global statistics of the sharded batch."""
-    if torch.compiler.is_compiling() and not distributed and group is None:
+    if not distributed and group is None and _recording():
         return _ops.standardize_op(x, float(eps))
     if torch.is_grad_enabled() and x.requires_grad and not distributed and group is None:
         # differentiable input (differentiable=True estimators): the reference's own torch ops keep the graph
@@ -1452,15 +1474,16 @@ def td_lambda_return_estimate(
     ``rolling_gamma=False`` (each return uses the gamma / lmbda of its own first step for the
     whole tail) runs the O(T^2) kernel and needs a gamma or lmbda tensor.
     """
-    if torch.compiler.is_compiling():
-        (g, gt), (l, lt) = _ops._split_leaf(gamma, next_state_value.shape, time_dim), _ops._split_leaf(lmbda, next_state_value.shape, time_dim)
-        return _ops.td_lambda_op(next_state_value, reward, done, done if terminated is None else terminated, g, l, gt, lt,
-                                 -1 if rolling_gamma is None else int(bool(rolling_gamma)), time_dim, False)
-    host = _HOST if _HOST_TRIED else _host_module()
+    compiling = torch.compiler.is_compiling()
+    host = None if compiling else _HOST if _HOST_TRIED else _host_module()
     if host is not None and (rolling_gamma is None or rolling_gamma):
         out = _host_call(host.td_lambda, gamma, lmbda, next_state_value, reward, done, terminated, ALGO_AUTO, time_dim, True)
         if out is not None:
             return out
+    if compiling or _recorded():
+        (g, gt), (l, lt) = _ops._split_leaf(gamma, next_state_value.shape, time_dim), _ops._split_leaf(lmbda, next_state_value.shape, time_dim)
+        return _ops.td_lambda_op(next_state_value, reward, done, done if terminated is None else terminated, g, l, gt, lt,
+                                 -1 if rolling_gamma is None else int(bool(rolling_gamma)), time_dim, False)
     call = _prepare_td_lambda(gamma, lmbda, next_state_value, reward, done, terminated, rolling_gamma, time_dim)
     if _needs_grad(next_state_value, reward, gamma, lmbda):
         return _TdLambdaFunction.apply(next_state_value, reward, _coef_leaf(gamma, call.shape, time_dim),
@@ -1483,16 +1506,17 @@ def vec_td_lambda_return_estimate(
     r"""Vectorized TD(:math:`\lambda`) return estimate (reference: functional.py:1030-1183).
     Same kernels as the loop variant; keeps the reference's ``NotImplementedError`` for
     ``rolling_gamma=False`` with tensor coefficients."""
-    if torch.compiler.is_compiling():
-        (g, gt), (l, lt) = _ops._split_leaf(gamma, next_state_value.shape, time_dim), _ops._split_leaf(lmbda, next_state_value.shape, time_dim)
-        return _ops.td_lambda_op(next_state_value, reward, done, done if terminated is None else terminated, g, l, gt, lt,
-                                 -1 if rolling_gamma is None else int(bool(rolling_gamma)), time_dim, True)
-    host = _HOST if _HOST_TRIED else _host_module()
+    compiling = torch.compiler.is_compiling()
+    host = None if compiling else _HOST if _HOST_TRIED else _host_module()
     if host is not None:   # scalar coefficients: the reference's scalar path ignores rolling_gamma (functional.py:1101-1110)
         out = _host_call(host.td_lambda, gamma, lmbda, next_state_value, reward, done, terminated, ALGO_AUTO, time_dim,
                          rolling_gamma is None or bool(rolling_gamma))
         if out is not None:
             return out
+    if compiling or _recorded():
+        (g, gt), (l, lt) = _ops._split_leaf(gamma, next_state_value.shape, time_dim), _ops._split_leaf(lmbda, next_state_value.shape, time_dim)
+        return _ops.td_lambda_op(next_state_value, reward, done, done if terminated is None else terminated, g, l, gt, lt,
+                                 -1 if rolling_gamma is None else int(bool(rolling_gamma)), time_dim, True)
     if terminated is None:
         terminated = done
     if not (next_state_value.shape == reward.shape == done.shape == terminated.shape):
@@ -1699,16 +1723,17 @@ def vtrace_advantage_estimate(
 
     Returns ``(advantages, vs)``.  ``terminated=None`` makes ``not_terminated = not_done``.
     """
-    if torch.compiler.is_compiling():
-        (g, gt), (rs, rt), (cs, ct) = _ops._split_leaf(gamma, next_state_value.shape, time_dim), _ops._split(rho_thresh), _ops._split(c_thresh)
-        return _ops.vtrace_op(log_pi, log_mu, state_value, next_state_value, reward, done, done if terminated is None else terminated,
-                              g, gt, rs, cs, rt, ct, time_dim)
-    host = _HOST if _HOST_TRIED else _host_module()
+    compiling = torch.compiler.is_compiling()
+    host = None if compiling else _HOST if _HOST_TRIED else _host_module()
     if host is not None:
         out = _host_call(host.vtrace, gamma, log_pi, log_mu, state_value, next_state_value, reward, done, terminated, rho_thresh,
                          c_thresh, ALGO_AUTO, time_dim)
         if out is not None:
             return out
+    if compiling or _recorded():
+        (g, gt), (rs, rt), (cs, ct) = _ops._split_leaf(gamma, next_state_value.shape, time_dim), _ops._split(rho_thresh), _ops._split(c_thresh)
+        return _ops.vtrace_op(log_pi, log_mu, state_value, next_state_value, reward, done, done if terminated is None else terminated,
+                              g, gt, rs, cs, rt, ct, time_dim)
     call = _prepare_vtrace(gamma, log_pi, log_mu, state_value, next_state_value, reward, done, terminated,
                            rho_thresh, c_thresh, time_dim)
     if _needs_grad(log_pi, log_mu, state_value, next_state_value, reward, gamma):
@@ -1833,7 +1858,7 @@ def td1_return_estimate(
     ``g = r + gamma*nt*((1-dnt)*g + dnt*v')`` with ``dnt = done & ~terminated``, starting from the raw
     ``v'_{T-1}``; ``rolling_gamma=False`` (needs a gamma tensor of the inputs' shape) reruns every tail with
     its first step's gamma from ``g = 0``, as the reference's loop does (``trl_td1_fwd``)."""
-    if torch.compiler.is_compiling():
+    if _recording():
         g, gt = _ops._split(gamma)
         return _ops.td1_op(next_state_value, reward, done, done if terminated is None else terminated, g, gt,
                            -1 if rolling_gamma is None else int(bool(rolling_gamma)), time_dim)
@@ -1886,7 +1911,7 @@ def reward2go(reward, done, gamma, *, time_dim: int = -2):
     ``R_t = r_t + gamma * (1-done_t) * R_{t+1}`` restarting after every ``done`` and at the end
     of every row: GAE with ``v = v' = 0`` and ``lmbda*gamma -> gamma``.  Like the reference, a
     tensor with more than two dims is flattened so that trailing dims are independent rows."""
-    if torch.compiler.is_compiling() and not isinstance(gamma, torch.Tensor):
+    if not isinstance(gamma, torch.Tensor) and _recording():
         return _ops.reward2go_op(reward, done, float(gamma), time_dim)
     if reward.shape != done.shape:
         raise ValueError(f"reward and done must share the same shape, got {reward.shape} and {done.shape}")

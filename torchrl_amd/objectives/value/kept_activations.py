@@ -88,14 +88,15 @@ class QuantizedActivation:
                 exponents.dtype != torch.uint8 or codes.device != exponents.device:
             raise RuntimeError(f"QuantizedActivation: codes {tuple(codes.shape)} {codes.dtype} and exponents {tuple(exponents.shape)} {exponents.dtype} "
                                f"do not hold a tensor of shape {tuple(self.shape)}")
-        if torch.compiler.is_compiling():
-            from torchrl_amd.objectives.value import _ops
-            return _ops.dequantize_activation_op(codes, exponents, D, dtype)
-        host = F._HOST if F._HOST_TRIED else F._host_module()
+        compiling = torch.compiler.is_compiling()
+        host = None if compiling else F._HOST if F._HOST_TRIED else F._host_module()
         if host is not None:
             out = host.dequantize(codes, exponents, D, _DT[dtype])
             if out is not None:
                 return _done(out)
+        if compiling or F._recorded():
+            from torchrl_amd.objectives.value import _ops
+            return _ops.dequantize_activation_op(codes, exponents, D, dtype)
         _check_device(codes)
         out = torch.empty(self.shape, dtype=dtype, device=codes.device)
         if out.numel():
@@ -107,14 +108,15 @@ class QuantizedActivation:
 def quantize_activation(x: Tensor) -> QuantizedActivation:
     """Keeps ``x`` ``[*B, D]`` (float32, bfloat16 or float16) in 8 bits: blocks of 32 features share a power of two, 2^-6 of the one at or below
     the block's largest magnitude; codes are rounded to nearest even and held to 127.  Blocks with a NaN or an infinity stand for NaN."""
-    if torch.compiler.is_compiling():
-        from torchrl_amd.objectives.value import _ops
-        return QuantizedActivation(*_ops.quantize_activation_op(x), x.shape, x.dtype)
-    host = F._HOST if F._HOST_TRIED else F._host_module()
+    compiling = torch.compiler.is_compiling()
+    host = None if compiling else F._HOST if F._HOST_TRIED else F._host_module()
     if host is not None:
         got = host.quantize(x)
         if got is not None:
             return QuantizedActivation(*_done(got), x.shape, x.dtype)
+    if compiling or F._recorded():
+        from torchrl_amd.objectives.value import _ops
+        return QuantizedActivation(*_ops.quantize_activation_op(x), x.shape, x.dtype)
     _check(x, "x")
     if x.ndim < 1 or x.shape[-1] == 0:
         raise RuntimeError(f"quantize_activation needs a feature dim, got shape {tuple(x.shape)}")
@@ -216,8 +218,8 @@ def checkpointed_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None
 
     ``x`` ``[*B, D]``, ``weight`` ``[O, D]`` and ``bias`` ``[O]`` share one dtype (float32, bfloat16 or float16) and device; under autocast they
     are cast to its dtype.  Without a gradient to ``weight`` nothing is kept."""
-    autocast = torch.is_autocast_enabled("cuda")
-    if not autocast and not torch.compiler.is_compiling():
+    autocast, compiling = torch.is_autocast_enabled("cuda"), torch.compiler.is_compiling()
+    if not autocast and not compiling:
         host = F._HOST if F._HOST_TRIED else F._host_module()
         if host is not None:  # checks, launches and the autograd node in one C++ hop (csrc/host_policy.cpp)
             got = host.checkpointed_linear(x, weight, bias)
@@ -226,7 +228,7 @@ def checkpointed_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None
     if autocast and all(isinstance(t, Tensor) for t in (x, weight)):
         dt = torch.get_autocast_dtype("cuda")
         x, weight, bias = x.to(dt), weight.to(dt), None if bias is None else bias.to(dt)
-    if torch.compiler.is_compiling():
+    if compiling or F._recorded():
         from torchrl_amd.objectives.value import _ops
         return _ops.checkpointed_linear(x, weight, bias)
     checkpointed_linear_check(x, weight, bias)

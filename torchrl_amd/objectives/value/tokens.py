@@ -321,17 +321,18 @@ def process_logits(logits: Tensor, *, tokens: Optional[Tensor] = None, lengths: 
 
     Differentiable in ``logits``; masked places get no gradient.  ``out`` (not under autograd) may be ``logits`` itself, and shares no
     memory with any other input."""
-    if torch.compiler.is_compiling():
-        _need(out is None, NotImplementedError, "process_logits(out=...) is not supported under torch.compile")
-        from torchrl_amd.objectives.value import _ops
-        return _ops.process_logits(logits, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty, bias, mask,
-                                   temperature)
-    host = F._HOST if F._HOST_TRIED else F._host_module()
+    compiling = torch.compiler.is_compiling()
+    host = None if compiling else F._HOST if F._HOST_TRIED else F._host_module()
     if host is not None and out is None:  # the plain layouts in one C++ hop (csrc/host_policy.cpp)
         got = host.process_logits(logits, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty, bias, mask,
                                   temperature)
         if got is not None:
             return _done(got)
+    if compiling or F._recorded():
+        _need(out is None, NotImplementedError, "process_logits(out=...) is not supported under torch.compile, make_fx and torch.jit.trace")
+        from torchrl_amd.objectives.value import _ops
+        return _ops.process_logits(logits, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty, bias, mask,
+                                   temperature)
     p = _processing(logits, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty, bias, mask, temperature)
     if F._needs_grad(logits):
         _need(out is None, RuntimeError, "process_logits(out=...) does not support automatic differentiation")
@@ -405,16 +406,17 @@ def token_log_prob(logits: Tensor, action: Tensor, *, entropy: bool = False, tok
     action that the mask does not allow has ``-inf`` too; an id of ``V`` or more gives NaN.
 
     Differentiable in ``logits`` (whose gradient has their dtype); neither a softmax nor the processed logits are kept for that."""
-    if torch.compiler.is_compiling():
-        from torchrl_amd.objectives.value import _ops
-        return _ops.token_log_prob(logits, action, entropy, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty,
-                                   bias, mask, temperature)
-    host = F._HOST if F._HOST_TRIED else F._host_module()
+    compiling = torch.compiler.is_compiling()
+    host = None if compiling else F._HOST if F._HOST_TRIED else F._host_module()
     if host is not None:  # the plain layouts in one C++ hop (csrc/host_policy.cpp)
         got = host.token_log_prob(logits, action, bool(entropy), tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty,
                                   frequency_penalty, bias, mask, temperature)
         if got is not None:
             return _done(got)
+    if compiling or F._recorded():
+        from torchrl_amd.objectives.value import _ops
+        return _ops.token_log_prob(logits, action, entropy, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty,
+                                   bias, mask, temperature)
     _need(isinstance(logits, Tensor), TypeError, "logits must be a tensor")
     lead = logits.shape[:-1]
     act = _int_tensor(action, lead, "action", logits.device)
