@@ -497,7 +497,7 @@ int trl_normalize_cpu(int dtype, const void *x, int64_t n, const double *stats, 
  * Ids outside [0, V) in `tokens` are no tokens; lengths are clamped to [0, L].
  */
 enum { TRL_BF16 = 2, TRL_F16 = 3 }; /* element types of these entry points, besides TRL_F32 */
-enum { TRL_MASK_NONE = 0, TRL_MASK_BOOL = 1, TRL_MASK_BITS = 2 }; /* a byte (0 / 1) a token; bit j % 32 of 32-bit word j / 32 */
+enum { TRL_MASK_NONE = 0, TRL_MASK_BOOL = 1, TRL_MASK_BITS = 2 }; /* a byte a token, any but 0 allows it; bit j % 32 of 32-bit word j / 32 */
 
 typedef struct trl_token_args {
     int32_t dtype;                            /* of logits, out, grad_out: TRL_F32, TRL_BF16, TRL_F16 */

@@ -711,3 +711,17 @@ def test_more_rows_than_a_launch_takes():
     assert torch.equal(lp, want.repeat(N // 16500 + 1)[:N])
     del lp, action
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("V", [5, 40, 2049, 4100])
+def test_truth_values_of_any_byte(V):
+    """A byte tensor viewed as truth values: whatever is not 0 allows, in whole vectors and in the last one."""
+    g = torch.Generator().manual_seed(V)
+    z = torch.randn(4, V, generator=g).cuda()
+    bytes_ = torch.randint(0, 256, (4, V), generator=g, dtype=torch.uint8)
+    bytes_ = torch.where(torch.rand(4, V, generator=g) < 0.5, bytes_, torch.tensor([0, 2, 128, 254], dtype=torch.uint8)[torch.randint(0, 4, (4, V), generator=g)]).cuda()
+    action = torch.randint(0, V, (4,), generator=g).cuda()
+    odd, plain = bytes_.view(torch.bool), bytes_ != 0
+    assert torch.equal(process_logits(z, mask=odd), z.masked_fill(~plain, -math.inf))
+    for a, b in zip(token_log_prob(z, action, entropy=True, mask=odd), token_log_prob(z, action, entropy=True, mask=plain)):
+        assert torch.equal(a, b)

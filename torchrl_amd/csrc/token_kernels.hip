@@ -76,8 +76,10 @@ __device__ __forceinline__ u32 mask_bits(int kind, const u8 *mask_lo, int off, i
         typedef u32 u32x2 __attribute__((ext_vector_type(2)));
         typedef u32x2 u32x2_any __attribute__((aligned(1)));
         const u32x2 w = *(const u32x2_any *)(mask_lo + off);  // 8 truth values of one byte
-        // byte i's lowest bit to bit 24 + i: no carries, the partial products do not meet
-        bits = (((w[0] & 0x01010101u) * 0x01020408u) >> 24 & 0xfu) | (((w[1] & 0x01010101u) * 0x01020408u) >> 20 & 0xf0u);
+        // Any byte but 0 allows (a byte tensor may be viewed as truth values): bit 7 of a byte is set where the rest or itself is not 0; the product
+        // takes byte i's to bit 28 + i.  No carries in either.
+        auto four = [](u32 x) { return (((((x & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x) & 0x80808080u) * 0x00204081u) >> 28; };
+        bits = four(w[0]) | four(w[1]) << 4;
     } else {
 #pragma unroll
         for (int i = 0; i < kVec; ++i)
