@@ -218,3 +218,14 @@ def test_more_rows_of_a_sequence_than_a_launch_takes():
 def test_a_value_head_without_keeping():
     lib = _extension.get_lib()
     assert lib.trl_act_head_fwd(None, 0, 64, 8, 4, 8, 64, None, None, 64, 64) == 1 and lib.trl_act_head_fwd(None, 0, 64, 8, 4, 8, 64, None, 64, None, 64) == 1
+
+
+def test_an_actors_tensors_move_with_it():
+    temperature = torch.tensor([0.7, 0.9])
+    actor = TokenActor(torch.nn.Linear(3, 4), temperature=temperature, presence_penalty=0.5, bias=torch.zeros(4))
+    keys = set(actor.state_dict())
+    assert actor.to("meta") is actor
+    assert actor.settings["temperature"].device.type == "meta" and actor.bias.device.type == "meta" and actor.settings["presence_penalty"] == 0.5
+    actor = TokenActor(torch.nn.Linear(3, 4), temperature=temperature, bias=torch.zeros(4)).to(torch.bfloat16)
+    assert torch.equal(actor.settings["temperature"], temperature) and actor.settings["temperature"].dtype == torch.float32
+    assert set(actor.state_dict()) == keys == {"bias", "network.weight", "network.bias"}

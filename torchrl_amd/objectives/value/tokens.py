@@ -434,7 +434,7 @@ class TokenActor(nn.Module):
 
     ``network``: any callable ``data -> logits [*B, T, V]`` (or a collection that holds them under ``logits_key``).  The keys name where the
     data keeps the picked ids, the sequences (``tokens`` / ``lengths`` / ``prompt_lengths`` of :func:`process_logits`) and a mask a row;
-    ``bias``, ``temperature`` and the penalties are :func:`process_logits`'s."""
+    ``bias``, ``temperature`` and the penalties are :func:`process_logits`'s; tensors among them move with the module."""
 
     def __init__(self, network, *, action_key="action", logits_key="logits", tokens_key=None, lengths_key=None, prompt_lengths_key=None, mask_key=None,
                  bias: Optional[Tensor] = None, temperature: Scalar = 1.0, repetition_penalty: Scalar = 1.0, presence_penalty: Scalar = 0.0,
@@ -446,6 +446,13 @@ class TokenActor(nn.Module):
         self.register_buffer("bias", bias)
         self.settings = {"temperature": temperature, "repetition_penalty": repetition_penalty, "presence_penalty": presence_penalty,
                          "frequency_penalty": frequency_penalty}
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        for k, v in self.settings.items():  # tensors follow to the module's device; what they hold is float32 arithmetic's and keeps its type
+            if isinstance(v, Tensor):
+                self.settings[k] = v.to(fn(v).device)
+        return self
 
     def _inputs(self, data):
         logits = self.network(data)
