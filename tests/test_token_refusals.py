@@ -229,3 +229,13 @@ def test_an_actors_tensors_move_with_it():
     actor = TokenActor(torch.nn.Linear(3, 4), temperature=temperature, bias=torch.zeros(4)).to(torch.bfloat16)
     assert torch.equal(actor.settings["temperature"], temperature) and actor.settings["temperature"].dtype == torch.float32
     assert set(actor.state_dict()) == keys == {"bias", "network.weight", "network.bias"}
+
+
+@pytest.mark.parametrize("name", ["temperature", "presence_penalty"])
+def test_numbers_that_round_to_infinity_are_refused(name):
+    largest = torch.finfo(torch.float32).max
+    kw = {} if name == "temperature" else dict(tokens=TOK, lengths=LEN)
+    with pytest.raises(RuntimeError, match="HIP"):
+        process_logits(Z, **{name: largest}, **kw)
+    with pytest.raises(ValueError, match="finite"):
+        process_logits(Z, **{name: math.nextafter(2.0 ** 128, 0.0)}, **kw)

@@ -26,6 +26,7 @@ __all__ = ["process_logits", "token_log_prob", "TokenActor"]
 _DT = {torch.float32: 0, torch.bfloat16: 2, torch.float16: 3}
 _INT = (torch.int32, torch.int64)
 _NONE, _BOOL, _BITS = 0, 1, 2
+_LARGEST = torch.finfo(torch.float32).max
 
 Scalar = Union[float, Tensor]
 
@@ -77,7 +78,7 @@ def _rows_view(x: Tensor, batch, T: int, name: str) -> Tensor:
 def _per_sequence(x: Scalar, batch, name: str, device, positive: bool) -> Tuple[float, Optional[Tensor]]:
     if not isinstance(x, Tensor):
         x = float(x)
-        _need(math.isfinite(x) and abs(x) < 2.0 ** 128 and (x >= 2.0 ** -126 or not positive), ValueError,
+        _need(math.isfinite(x) and abs(x) <= _LARGEST and (x >= 2.0 ** -126 or not positive), ValueError,
               f"{name} must be {'positive and ' if positive else ''}finite in float32, got {x}")
         return x, None
     _need(not (torch.is_grad_enabled() and x.requires_grad), NotImplementedError, f"gradients with respect to {name} are not implemented: detach it")
