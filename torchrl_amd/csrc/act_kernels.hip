@@ -7,14 +7,6 @@ namespace {
 
 constexpr int kGroups = kActBlock / kVec;  // 4 lanes hold a block
 
-__device__ __forceinline__ float wave_sum(float x) {
-    x += dpp_mov<0xB1>(x);
-    x += dpp_mov<0x4E>(x);
-    x += dpp_mov<0x141>(x);
-    x += dpp_mov<0x140>(x);
-    return (read_lane(x, 0) + read_lane(x, 16)) + (read_lane(x, 32) + read_lane(x, 48));
-}
-
 // Thread -> (row, group of 8 features) over N rows of G groups; one 64-bit division a block of threads.
 __device__ __forceinline__ bool row_and_group(i64 N, u32 G, i64 &row, u32 &group) {
     const i64 first = (i64)blockIdx.x * blockDim.x;
@@ -192,9 +184,6 @@ __device__ __forceinline__ void convert16(u32x4 codes, int e, u32x4 *w) {
         w[i / 2][2 * (i % 2) + 1] = pack_exact<T>(v[2], v[3]);
     }
 }
-
-template <bool B>
-struct Flag { static constexpr bool value = B; };
 
 // orders LDS alone: loads from memory stay in flight
 __device__ __forceinline__ void lds_barrier() {
@@ -389,8 +378,8 @@ __global__ __launch_bounds__(WM *WN *kWave, BM == 256 ? 2 : 1) void act_weight_g
             }
         };
         if (n + 3 * BK <= n_whole) {
-            if (want_db) middle(Flag<true>());
-            else middle(Flag<false>());
+            if (want_db) middle(Bool<true>());
+            else middle(Bool<false>());
             __syncthreads();
         }
     }

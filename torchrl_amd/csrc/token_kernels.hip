@@ -37,8 +37,6 @@ constexpr float kFloor = -1.0e4f;            // 2^kFloor is 0: keeps 0 * (-inf) 
 constexpr u32 kSeenInPrompt = 0x80000000u;
 typedef unsigned long long u64;
 
-template <bool B>
-struct Bool { static constexpr bool value = B; };
 enum Mode { kProcess, kProcessBwd, kLogProb, kLogProbBwd };
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
@@ -169,21 +167,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
 }
-__device__ __forceinline__ float wave_max_f(float x) {
-    x = fmaxf(x, dpp_mov<0xB1>(x));
-    x = fmaxf(x, dpp_mov<0x4E>(x));
-    x = fmaxf(x, dpp_mov<0x141>(x));
-    x = fmaxf(x, dpp_mov<0x140>(x));
-    return fmaxf(fmaxf(read_lane(x, 0), read_lane(x, 16)), fmaxf(read_lane(x, 32), read_lane(x, 48)));
-}
-__device__ __forceinline__ float wave_sum_f(float x) {
-    x += dpp_mov<0xB1>(x);
-    x += dpp_mov<0x4E>(x);
-    x += dpp_mov<0x141>(x);
-    x += dpp_mov<0x140>(x);
-    return (read_lane(x, 0) + read_lane(x, 16)) + (read_lane(x, 32) + read_lane(x, 48));
-}
-
 // the shift of d = z * c - shift for a row's (or a wave's) largest value m; *steep: d = (z - m) * c, see the head of the file
 __device__ __forceinline__ float softmax_shift(float m, float c, bool *steep) {
     const float m2 = m * c;
@@ -254,7 +237,7 @@ __device__ __forceinline__ void join_row(const TokenArgs &a, i64 r, i64 y, const
     float m = neg_inf(), s = 0.0f, u = 0.0f, scale = 0.0f;
     if (y >= 0) {
         for (i64 i = lane; i < nsubs; i += kStep) m = fmaxf(m, part[i].x);
-        if (WAVE) m = wave_max_f(m);
+        if (WAVE) m = wave_max(m);
         scale = kLog2e * (1.0f / (a.temp_t ? a.temp_t[r / a.T] : a.temp));  // the row kernel's own bits
         bool steep;
         const float shift = softmax_shift(m, scale, &steep);
@@ -273,8 +256,8 @@ __device__ __forceinline__ void join_row(const TokenArgs &a, i64 r, i64 y, const
             u = fmaf(w, fmaf(q.y, fmaxf(d, kFloor), q.z), u);
         }
         if (WAVE) {
-            s = wave_sum_f(s);
-            u = wave_sum_f(u);
+            s = wave_sum(s);
+            u = wave_sum(u);
         }
     }
     if (lane == 0) finish_row(a, r, y, m, s, u, scale, z_action);
@@ -552,7 +535,7 @@ __global__ __launch_bounds__((kMostWaves<T, MODE, PEN, BIAS>) * kWave, (kSimdWav
                         z_y = read_lane(mine_z, ((int)at & (kBlk - 1)) / kVec);
                     }
                 }
-                m = wave_max_f(m);
+                m = wave_max(m);
                 float s = 0.0f, u = 0.0f;
                 bool steep;
                 float shift = softmax_shift(m, scale, &steep);
@@ -568,8 +551,8 @@ __global__ __launch_bounds__((kMostWaves<T, MODE, PEN, BIAS>) * kWave, (kSimdWav
                             u = fmaf(e, d, u);
                         }
                     }
-                    s = wave_sum_f(s);
-                    u = wave_sum_f(u);
+                    s = wave_sum(s);
+                    u = wave_sum(u);
                     careful = __builtin_isnan(u) && !__builtin_isnan(s);
                 }
                 if (careful) {
@@ -584,7 +567,7 @@ __global__ __launch_bounds__((kMostWaves<T, MODE, PEN, BIAS>) * kWave, (kSimdWav
                             m = fmaxf(m, z[k][i]);
                         }
                     }
-                    m = wave_max_f(m);
+                    m = wave_max(m);
                     shift = softmax_shift(m, scale, &steep);
 #pragma unroll
                     for (int k = 0; k < kRowVecs; ++k) {
@@ -596,8 +579,8 @@ __global__ __launch_bounds__((kMostWaves<T, MODE, PEN, BIAS>) * kWave, (kSimdWav
                             u = fmaf(e, fmaxf(d, kFloor), u);
                         }
                     }
-                    s = wave_sum_f(s);
-                    u = wave_sum_f(u);
+                    s = wave_sum(s);
+                    u = wave_sum(u);
                 }
                 if (alone) {
                     const bool its = lane == i_row;

@@ -273,6 +273,15 @@ def _on(device):
     return torch.cuda.device(device)
 
 
+def _native(name: str, device, *args) -> None:
+    """One C-ABI call on the caller's current stream of ``device``."""
+    lib = _extension.get_lib()
+    with _on(device):
+        rc = getattr(lib, name)(_stream(device), *args)
+    if rc:
+        _extension.check(rc, lib)
+
+
 def _needs_grad(*xs) -> bool:
     return torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in xs)
 
@@ -970,12 +979,16 @@ def host_fast_path() -> bool:
     return _host_module() is not None
 
 
-def _host_call(fn, *args):
-    """One call into the host module: its outputs, or None when the call is not a fast-path one."""
-    out = fn(*args)
+def _host_done(out):
+    """What the host module returned: the outputs, None, or the status of a native call that failed, which raises."""
     if out.__class__ is int:
         _extension.check(out, _extension.get_lib())
     return out
+
+
+def _host_call(fn, *args):
+    """One call into the host module: its outputs, or None when the call is not a fast-path one."""
+    return _host_done(fn(*args))
 
 
 def _step_mask(m: torch.Tensor, shape, td: int) -> bool:

@@ -22,6 +22,7 @@ from torch.autograd.function import once_differentiable
 
 from torchrl_amd import _extension
 from torchrl_amd.objectives.value import functional as F
+from torchrl_amd.objectives.value.functional import _host_done, _native, _ptr
 
 __all__ = ["QuantizedActivation", "quantize_activation", "checkpointed_linear", "CheckpointedLinear"]
 
@@ -46,25 +47,6 @@ def _rows(x: Tensor) -> Tensor:
     """``x`` as (N, D) with last stride 1."""
     x = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
-
-
-def _ptr(x: Optional[Tensor]):
-    return None if x is None else x.data_ptr()
-
-
-def _call(name, device, *args):
-    lib = _extension.get_lib()
-    with F._on(device):
-        rc = getattr(lib, name)(F._stream(device), *args)
-    if rc:
-        _extension.check(rc, lib)
-
-
-def _done(got):
-    """What the host module returns: the result, or the status of a native call that failed."""
-    if got.__class__ is int:
-        _extension.check(got, _extension.get_lib())
-    return got
 
 
 @dataclass
@@ -93,7 +75,7 @@ class QuantizedActivation:
         if host is not None:
             out = host.dequantize(codes, exponents, D, _DT[dtype])
             if out is not None:
-                return _done(out)
+                return _host_done(out)
         if compiling or F._recorded():
             from torchrl_amd.objectives.value import _ops
             return _ops.dequantize_activation_op(codes, exponents, D, dtype)
@@ -101,7 +83,7 @@ class QuantizedActivation:
         out = torch.empty(self.shape, dtype=dtype, device=codes.device)
         if out.numel():
             codes, exponents = codes.contiguous(), exponents.contiguous()
-            _call("trl_act_dequantize", out.device, _DT[dtype], codes.data_ptr(), exponents.data_ptr(), out.numel() // D, D, out.data_ptr())
+            _native("trl_act_dequantize", out.device, _DT[dtype], codes.data_ptr(), exponents.data_ptr(), out.numel() // D, D, out.data_ptr())
         return out
 
 
@@ -113,7 +95,7 @@ def quantize_activation(x: Tensor) -> QuantizedActivation:
     if host is not None:
         got = host.quantize(x)
         if got is not None:
-            return QuantizedActivation(*_done(got), x.shape, x.dtype)
+            return QuantizedActivation(*_host_done(got), x.shape, x.dtype)
     if compiling or F._recorded():
         from torchrl_amd.objectives.value import _ops
         return QuantizedActivation(*_ops.quantize_activation_op(x), x.shape, x.dtype)
@@ -124,7 +106,7 @@ def quantize_activation(x: Tensor) -> QuantizedActivation:
     codes, exponents = _empty_kept(x)
     if x.numel():
         rows = _rows(x.detach())
-        _call("trl_act_quantize", x.device, _DT[x.dtype], rows.data_ptr(), rows.stride(0), rows.shape[0], x.shape[-1], codes.data_ptr(),
+        _native("trl_act_quantize", x.device, _DT[x.dtype], rows.data_ptr(), rows.stride(0), rows.shape[0], x.shape[-1], codes.data_ptr(),
               exponents.data_ptr())
     return QuantizedActivation(codes, exponents, x.shape, x.dtype)
 
@@ -157,7 +139,7 @@ def _linear_and_kept(x: Tensor, weight: Tensor, bias: Optional[Tensor], keep: bo
     codes, exponents = _empty_kept(x) if keep else (None, None)
     y = torch.empty(*x.shape[:-1], 1, dtype=x.dtype, device=x.device)
     rows, w = _rows(x.detach()), weight.detach().contiguous()
-    _call("trl_act_head_fwd", x.device, _DT[x.dtype], rows.data_ptr(), rows.stride(0), rows.shape[0], x.shape[-1], w.data_ptr(), _ptr(bias),
+    _native("trl_act_head_fwd", x.device, _DT[x.dtype], rows.data_ptr(), rows.stride(0), rows.shape[0], x.shape[-1], w.data_ptr(), _ptr(bias),
           _ptr(codes), _ptr(exponents), y.data_ptr())
     return y, codes, exponents
 
@@ -179,10 +161,10 @@ def _weight_grad(dy: Tensor, codes: Optional[Tensor], exponents: Optional[Tensor
     if weight is not None:
         F._check_kept((weight,), ((dy.dtype, (1, D), dy.device),))
         w, dx = weight.detach().contiguous(), torch.empty(N, D, dtype=dy.dtype, device=dy.device)
-        _call("trl_act_head_bwd", dy.device, dt, dy.data_ptr(), dy.stride(0), _ptr(codes), _ptr(exponents), N, D, w.data_ptr(), _ptr(dw), _ptr(db),
+        _native("trl_act_head_bwd", dy.device, dt, dy.data_ptr(), dy.stride(0), _ptr(codes), _ptr(exponents), N, D, w.data_ptr(), _ptr(dw), _ptr(db),
               _ptr(dx), _ptr(ws), need)
         return dw, db, dx
-    _call("trl_act_weight_grad", dy.device, dt, dy.data_ptr(), dy.stride(0), _ptr(codes), _ptr(exponents), N, O, D, _ptr(dw), _ptr(db), _ptr(ws), need)
+    _native("trl_act_weight_grad", dy.device, dt, dy.data_ptr(), dy.stride(0), _ptr(codes), _ptr(exponents), N, O, D, _ptr(dw), _ptr(db), _ptr(ws), need)
     return dw, db
 
 
@@ -224,7 +206,7 @@ def checkpointed_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None
         if host is not None:  # checks, launches and the autograd node in one C++ hop (csrc/host_policy.cpp)
             got = host.checkpointed_linear(x, weight, bias)
             if got is not None:
-                return _done(got)
+                return _host_done(got)
     if autocast and all(isinstance(t, Tensor) for t in (x, weight)):
         dt = torch.get_autocast_dtype("cuda")
         x, weight, bias = x.to(dt), weight.to(dt), None if bias is None else bias.to(dt)

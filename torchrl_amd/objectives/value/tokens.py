@@ -20,6 +20,7 @@ from torch.autograd.function import once_differentiable
 
 from torchrl_amd import _extension
 from torchrl_amd.objectives.value import functional as F
+from torchrl_amd.objectives.value.functional import _host_done, _native, _ptr
 
 __all__ = ["process_logits", "token_log_prob", "TokenActor"]
 
@@ -161,10 +162,6 @@ def _processing(logits, tokens, lengths, prompt_lengths, repetition_penalty, pre
                        rep_t, pres_t, freq_t, temp_t, bias, mask)
 
 
-def _ptr(x):
-    return None if x is None else x.data_ptr()
-
-
 def _wide(x):
     return 0 if x is None or x.dtype == torch.int32 else 1
 
@@ -185,21 +182,6 @@ def _args(p: _Processing, **more) -> "_extension.TokenArgs":
     for k, v in more.items():
         setattr(a, k, v)
     return a
-
-
-def _call(name, device, args, *more):
-    lib = _extension.get_lib()
-    with F._on(device):
-        rc = getattr(lib, name)(F._stream(device), args, *more)
-    if rc:
-        _extension.check(rc, lib)
-
-
-def _done(got):
-    """What the host module returns: the result, or the status of a native call that failed."""
-    if got.__class__ is int:
-        _extension.check(got, _extension.get_lib())
-    return got
 
 
 def _save(ctx, p: _Processing, *more, logits: bool = True):
@@ -224,7 +206,7 @@ def _saved(ctx):
 # ---- process_logits ---------------------------------------------------------------------------------------------------------
 def _process_fwd(p: _Processing, out: Tensor) -> None:
     if p.B * p.T:
-        _call("trl_process_logits_fwd", out.device, _args(p, out=out.data_ptr(), out_sb=out.stride(0), out_st=out.stride(1)))
+        _native("trl_process_logits_fwd", out.device, _args(p, out=out.data_ptr(), out_sb=out.stride(0), out_st=out.stride(1)))
 
 
 def _process_new(p: _Processing, shape) -> Tensor:
@@ -239,7 +221,7 @@ def _process_bwd(p: _Processing, grad: Tensor) -> Tensor:
     grad = grad.reshape(p.B, p.T, p.V).contiguous()
     d = torch.empty_like(grad)
     if p.B * p.T:
-        _call("trl_process_logits_bwd", grad.device, _args(p, grad_out=grad.data_ptr(), out=d.data_ptr(), out_sb=d.stride(0), out_st=d.stride(1)))
+        _native("trl_process_logits_bwd", grad.device, _args(p, grad_out=grad.data_ptr(), out=d.data_ptr(), out_sb=d.stride(0), out_st=d.stride(1)))
     return d
 
 
@@ -328,7 +310,7 @@ def process_logits(logits: Tensor, *, tokens: Optional[Tensor] = None, lengths: 
         got = host.process_logits(logits, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty, bias, mask,
                                   temperature)
         if got is not None:
-            return _done(got)
+            return _host_done(got)
     if compiling or F._recorded():
         _need(out is None, NotImplementedError, "process_logits(out=...) is not supported under torch.compile, make_fx and torch.jit.trace")
         from torchrl_amd.objectives.value import _ops
@@ -356,7 +338,7 @@ def _log_prob_fwd(p: _Processing, action: Tensor, shape, entropy: bool, stats: b
     if n:
         need = _extension.get_lib().trl_token_workspace_bytes(p.B, p.T, p.V)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _call("trl_token_log_prob_fwd", dev, _args(p, action=action.data_ptr(), action_wide=_wide(action), log_prob=log_prob.data_ptr(),
+        _native("trl_token_log_prob_fwd", dev, _args(p, action=action.data_ptr(), action_wide=_wide(action), log_prob=log_prob.data_ptr(),
                                                    entropy=_ptr(H), stats=_ptr(st)), ws.data_ptr(), need)
     return log_prob, H, st
 
@@ -371,7 +353,7 @@ def _log_prob_bwd(p: _Processing, action: Tensor, H: Optional[Tensor], stats: Te
     F._check_kept((stats,), ((torch.float32, (n, 2), p.logits.device),))
     if n:
         g_lp, g_H = _row_grad(g_lp), _row_grad(g_H)
-        _call("trl_token_log_prob_bwd", action.device, _args(p, action=action.data_ptr(), action_wide=_wide(action), entropy=_ptr(H),
+        _native("trl_token_log_prob_bwd", action.device, _args(p, action=action.data_ptr(), action_wide=_wide(action), entropy=_ptr(H),
                                                              stats=stats.data_ptr(), g_log_prob=_ptr(g_lp), g_entropy=_ptr(g_H), out=d.data_ptr(),
                                                              out_sb=d.stride(0), out_st=d.stride(1)))
     return d
@@ -413,7 +395,7 @@ def token_log_prob(logits: Tensor, action: Tensor, *, entropy: bool = False, tok
         got = host.token_log_prob(logits, action, bool(entropy), tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty,
                                   frequency_penalty, bias, mask, temperature)
         if got is not None:
-            return _done(got)
+            return _host_done(got)
     if compiling or F._recorded():
         from torchrl_amd.objectives.value import _ops
         return _ops.token_log_prob(logits, action, entropy, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty,
