@@ -7,7 +7,6 @@
  *   torchrl/objectives/value/functional.py   (the ATen op soup of the loop / vec variants)
  * and are loaded the way the reference loads its only native module
  *   torchrl/_extension.py:17-31, setup.py:121-169  (`torchrl._torchrl` discovery convention).
- * INTEGRATION.md shows the reference-side ctypes stub a maintainer would add.
  *
  * Conventions
  *  - Plain pointers and sizes only; no torch types.  PyTorch (or any caller) owns every
@@ -141,7 +140,7 @@ int trl_gae_fwd(void *stream, int val_dtype, int coef_dtype,
                 double *stats, void *workspace, size_t workspace_bytes, int algo);
 
 /*
- * GAE followed by advantage normalisation over ALL elements -- the north-star step.
+ * GAE followed by advantage normalisation over ALL elements -- the flagship step.
  * Replaces: GAE.forward with average_gae=True (torchrl/objectives/value/advantages.py:1436-1463):
  *   adv, value_target = gae(...);  adv = (adv - adv.mean()) / adv.std().clamp_min(eps)
  * Arguments as trl_gae_fwd; `advantage` receives the NORMALISED advantage.  `stats` (optional,
@@ -425,7 +424,7 @@ int trl_gae_normalize_xchg_fwd(void *stream, int val_dtype, int coef_dtype,
 /*
  * Host entry points (ABI 7): the same estimators for tensors in HOST memory -- every pointer below is a host pointer,
  * `stats` included; the call returns when the outputs are written.  The reference runs its estimators on whatever device
- * the tensors live on (functional.py:163-170 allocates on state_value.device; the CartPole-shaped BASELINE config is a CPU
+ * the tensors live on (functional.py:163-170 allocates on state_value.device; a CartPole-sized rollout is a CPU
  * call), so the drop-in takes CPU tensors too.  Arguments as in the device entry points of the same name, minus stream,
  * workspace and `algo`: there is one family, the row-sequential walk in the reference's operation order -- the very row
  * functions of the SEQ kernels (csrc/seq_rows.h) -- so results are bit-identical to TRL_ALGO_SEQ on the GPU (V-trace: up to

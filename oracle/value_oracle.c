@@ -55,7 +55,7 @@
  * :1828-1832 (VTrace average_adv):  (x - x.mean()) / x.std().clamp_min(eps)
  * with the unbiased (N-1) standard deviation over ALL elements.  Statistics are
  * accumulated in double (two-pass), rounded to the storage dtype, and the scale
- * pass runs in the storage dtype (SURVEY.md A11: bit-identical to torch at
+ * pass runs in the storage dtype (bit-identical to torch at
  * [65536x32]; torch's own reduction order is internal, so parity is to ~1e-6).
  * stats_out (optional) receives {N, sum, sum of squares} in double.
  * ------------------------------------------------------------------------- */

@@ -8,7 +8,7 @@ the reference's sequential loops, reference: torchrl/objectives/value/functional
 783-889, 1270-1350).  This file only (i) reshapes ``[*B, T, *F]`` inputs to the canonical
 contiguous ``(O, T, I)`` view (the effect of the reference's ``_transpose_time`` decorator,
 functional.py:49-113), and (ii) reproduces the dtype the reference's coefficient tensors get
-(``gamma * int_mask`` rounds python floats to the default dtype, SURVEY.md fact 3) by running
+(``gamma * int_mask`` rounds python floats to the default dtype) by running
 the same torch expression on a one-element int32 tensor.
 
 Parity pin: tests/test_oracle_golden.py checks every function against the golden fixtures in
@@ -203,7 +203,7 @@ def td1(gamma, next_state_value, reward, done, terminated=None, rolling_gamma=No
 
 def td0(gamma, next_state_value, reward, terminated):
     """functional.py:418-456 -- reward + gamma * not_terminated * next_state_value, op for op in numpy
-    (``gamma * int_mask`` first: a python-float gamma is rounded to the default dtype, SURVEY.md fact 3)."""
+    (``gamma * int_mask`` first: a python-float gamma is rounded to the default dtype)."""
     nt = (~terminated).to(torch.int32)
     coef = gamma * nt
     if not coef.dtype.is_floating_point:

@@ -11,7 +11,7 @@
  *   TS      storage dtype of reward / state_value / next_state_value / outputs
  *   TG      dtype the reference's coefficient tensors have (gamma * int_mask);
  *           float when gamma is a python float under default dtype float32,
- *           whatever dtype a full gamma tensor has otherwise (SURVEY.md fact 3)
+ *           whatever dtype a full gamma tensor has otherwise
  *   TC      compute dtype = promote(TS, TG)
  *   SFX     symbol suffix
  *

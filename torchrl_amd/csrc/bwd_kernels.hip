@@ -368,7 +368,7 @@ LaunchResult dispatch_bwd_scan(int vdt, int cdt, i64 T, F &&f) {
             if (cdt == 1) return f(OpT<float, double, 2>{});
         }
         // fp64: ONE element per lane (8-byte accesses).  V = 2 needs 164 VGPRs (3 waves per SIMD); V = 1 about half of that.
-        // Measured (round 3, tools/dev/bench_vtrace_bwd.py): C4 55.2 -> 36.2 us, C5 261.5 -> 225.0 us (4.15 -> 4.82 TB/s, the
+        // Measured (tools/dev/bench_vtrace_bwd.py): C4 55.2 -> 36.2 us, C5 261.5 -> 225.0 us (4.15 -> 4.82 TB/s, the
         // DRAM-bound rate of this box for a 1 GB footprint).  fp32 long rows with V = 2: 179 us (123 with the prefetch) against
         // 115 with V = 4 -- there the per-chunk latency chain, not occupancy, is what counts.
         if (vdt == 1 && cdt == 1) return f(OpT<double, double, 1>{});

@@ -155,7 +155,7 @@ static bool prefer_lockstep(int val_dtype, int coef_dtype, int64_t T, int64_t I)
     return R * T * I * 100 < chunk * 95;
 }
 
-// GAE only (round 3): GAE has its own transposing kernel (gae_interleaved.h: 2 arrays instead of 5 cross LDS; rows of 64 < T <= 256
+// GAE only: GAE has its own transposing kernel (gae_interleaved.h: 2 arrays instead of 5 cross LDS; rows of 64 < T <= 256
 // steps as 16- / 32-lane groups in the row phase) and the rule above, measured on the generic kernel, no longer describes it.
 // Transposing / lock-step us at every chunk fill (profiles/r03_gae_rows_as_dpp_rows.txt): [4096x80x5] 7.9 / 12.8, [4096x96x4]
 // 7.6 / 9.9, [8192x64x4] 8.1 / 10.1, [8192x40x3] 6.7 / 8.0, [8192x60x6] 15.4 / 22.3, [4096x136x7] 16.9 / 31.7, [4096x160x3]
@@ -200,7 +200,7 @@ static bool vtrace_prefers_transposing(int val_dtype, int64_t T, int64_t I) {
 // over i, but every (o, i) row is a lane).  Measured fp32 (SEQ / LOCKSTEP us): [64x1000x16] 381 / 20, [1024x300x16]
 // 145 / 62, [4096x300x16] 281 / 218, [1024x100x31] 68 / 65, [8192x100x16] 117 / 146, [16384x64x31] 360 / 817:
 // SEQ once there are enough rows to hide its per-step latency -- unless I factors as G * NI (G = 2 / 4 / 8 groups of a step
-// in neighbouring lanes, lockstep_impl.h, round 3): then a wave reads whole cache lines and LOCKSTEP wins everywhere
+// in neighbouring lanes, lockstep_impl.h): then a wave reads whole cache lines and LOCKSTEP wins everywhere
 // measured ([8192x100x16] 129 / 55, [16384x64x20] 207 / 149, [8192x100x24] 193 / 163, [4096x300x16] 281 / 82).
 static bool lockstep_over_seq(int64_t O, int64_t I) {
     const bool lanes = I == 10 || I == 12 || I == 14 || I == 16 || I == 20 || I == 24 || I == 28;

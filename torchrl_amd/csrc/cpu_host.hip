@@ -1,7 +1,7 @@
 // Host entry points (trl_*_cpu, include/trl_value.h ABI 7): the estimators for tensors that live in HOST memory.
 //
 // The reference runs on whatever device its tensors are on (torchrl/objectives/value/functional.py:163-170 allocates on
-// state_value.device; BASELINE config 1 is a CPU call), so a drop-in must take CPU tensors too.  This is the product's own
+// state_value.device; a CartPole-sized rollout is a CPU call), so a drop-in must take CPU tensors too.  This is the product's own
 // host path, not the test oracle: it runs the very row functions of the SEQ kernel family (seq_rows.h, __host__ __device__)
 // -- the reference's per-step expressions in the reference's order, compiled with -ffp-contract=off -- over the (o, i) rows,
 // split across a few worker threads.  Results are bit-identical to the SEQ kernels (up to libm's exp in V-trace) and to the

@@ -1,6 +1,6 @@
 // Single-launch GAE + advantage normalisation ("FUSED" family).
 //
-// The north-star step -- GAE followed by `(adv - adv.mean()) / adv.std().clamp_min(eps)`
+// The flagship step -- GAE followed by `(adv - adv.mean()) / adv.std().clamp_min(eps)`
 // (reference: torchrl/objectives/value/advantages.py:1436-1463) -- needs the moments of ALL
 // advantages before the first normalised value can be written.  Instead of three launches
 // (scan + moments, final reduce, scale pass re-reading the advantage from HBM) this kernel keeps
@@ -17,7 +17,7 @@
 //     (16 bytes per block, 8 replicas); wave 0 of every block sweeps its replica -- 4 KB for 256 blocks, four
 //     coalesced 16-byte sc1 loads per lane and round -- until every tag matches (no fences, no atomics, no
 //     counters), sums them in a fixed order (bitwise reproducible) and broadcasts mean / std through LDS
-//     (round 3: last publish -> last gathered 2.1 -> 1.6 us at C4 against one 128-byte line per block polled with
+//     (last publish -> last gathered 2.1 -> 1.6 us at C4 against one 128-byte line per block polled with
 //     8-byte loads, 7.95 -> 7.45 us per launch; tools/kbench/kfused3.hip, kxchg.hip);
 //   * the normalised advantages are written: 22 B of HBM traffic per transition in total, the
 //     algorithmic minimum.

@@ -1,14 +1,14 @@
 // GAE for rollouts with feature dims after time (I > 1, whole outer rows inside one chunk: T*I <= 256*V) -- the VMAS /
-// MAPPO shape [E, T, A, 1] (BASELINE config 3).  Element (o, t, i) sits at (o*T + t)*I + i: the I scans of an outer row are
+// MAPPO shape [E, T, A, 1].  Element (o, t, i) sits at (o*T + t)*I + i: the I scans of an outer row are
 // interleaved in memory.  As in the generic kernel of scan_impl.h a team loads a chunk of whole outer rows with coalesced
 // 16-byte loads and turns it through LDS so that every lane ends up with V consecutive time steps of ONE (o, i) row; the
 // difference is WHAT crosses LDS.  Everything elementwise is done in memory order, before and after the turn:
 //   in : delta = (r + gamma*nt*v') - v   and   disc = lmbda*gamma*nd     (2 values per element instead of 5 tensors)
 //   out: the advantage; value_target = advantage + v is formed in memory order from the v the lane still holds
 // -- 16 B of LDS traffic per element and direction instead of 44, a third of the LDS footprint (12.7 KB per block) and far
-// fewer live registers, so twice as many blocks are resident.  C3 [4096 x 100 x 5]: 13.1 -> 9.8 us (DESIGN.md section 5).
+// fewer live registers, so twice as many blocks are resident.  C3 [4096 x 100 x 5]: 13.1 -> 9.8 us.
 // Same arithmetic as every other family: the lane replays its steps with delta + x*disc from its carry-in.
-// Round 3: the estimator-specific parts are policies (GaeTurn, TdLambdaTurn, Td1Turn): TD(lambda) / TD(1) returns with rolling
+// The estimator-specific parts are policies (GaeTurn, TdLambdaTurn, Td1Turn): TD(lambda) / TD(1) returns with rolling
 // gamma take the same route -- C3-shaped TD(lambda) 11.1 -> 8.8 us, [4096x136x7] 18.3 -> 13.3, fp64 C3 17.6 -> 12.7 against the
 // generic transposing kernel that scan_impl.h held until then; V-trace followed (VtraceTurn: its outputs need the next step's x and
 // value, read in memory order I elements further) and that kernel is gone.
@@ -276,8 +276,8 @@ constexpr int kGilBlocksPerCu = 4;  // resident blocks per CU = the grid's block
 // steps, no cross-wave stage and no barrier of its own -- at the price of idle lanes in that phase (C3: 10 rows = 160 of 256
 // lanes, 100 of 112 steps).  The memory-order phases (V elements per lane, 16-byte accesses) are the same.  Measured: C3 9.55 ->
 // 8.49 us back-to-back, 10.45 -> 9.28 us rocprofv3 average; [4096x112x3] 9.16 -> 8.08; fp64 C3 17.65 -> 16.6; LG = 32 (128 < T <=
-// 256): [4096x200x5] 19.4 -> 17.8, [4096x160x3] 9.55 -> 8.2, [4096x136x7] 18.7 -> 16.9, fp64 [4096x160x3] 16.5 -> 15.4 (DESIGN.md section 5).
-// NT: threads per block.  256 (a team, 4 blocks per CU), or 1024 with a chunk of 1024 * V elements (round 3, row mapping only):
+// 256): [4096x200x5] 19.4 -> 17.8, [4096x160x3] 9.55 -> 8.2, [4096x136x7] 18.7 -> 16.9, fp64 [4096x160x3] 16.5 -> 15.4.
+// NT: threads per block.  256 (a team, 4 blocks per CU), or 1024 with a chunk of 1024 * V elements (row mapping only):
 // whole outer rows of up to 4096 fp32 elements -- MAPPO-shaped rollouts with 11 - 40 agents, which the lock-step kernels served
 // at 1.1 - 3.6 TB/s ([4096x100x30] 238 us, [4096x100x11] 59.5 us, [4096x100x20] 57.0 us).
 template <class P, int V, int VR, int LG, bool VEC, bool WAVE_INDEP, bool PAD, int NT = kTeam>

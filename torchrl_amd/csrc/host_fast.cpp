@@ -1,7 +1,7 @@
 // Host-side fast path of the python entry points (CPython module torchrl_amd/lib/_trl_host.so): the eligibility checks, the
 // output allocations and the C-ABI call in one C++ function, so that generalized_advantage_estimate /
 // vec_generalized_advantage_estimate / gae_normalized / (vec_)td_lambda_return_estimate / vtrace_advantage_estimate cost
-// about the kernel launch itself (drop-in API overhead; measured numbers in DESIGN.md section 5).  Plumbing
+// about the kernel launch itself (what a drop-in API may cost; tools/bench_entry.py measures it).  Plumbing
 // only: no arithmetic on the data happens here, the kernels are reached through the same entry points of
 // include/trl_value.h, whose addresses python hands over at init -- the library this module drives is whichever one ctypes
 // loaded.

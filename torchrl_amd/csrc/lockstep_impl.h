@@ -323,7 +323,7 @@ template <template <typename, typename, int> class OpT, class Args>
 LaunchResult dispatch_ls(hipStream_t s, int vdt, int cdt, const Args &a, bool aligned, double *partials, const char *name) {
     if (a.I < 2 || a.I > 31 || a.T >= (1LL << 31) - 4096) return LaunchResult{2, 0, nullptr};
     // 9 <= I <= 31 = G * NI with G a power of two and NI <= 8: the G groups of a step in neighbouring lanes (whole cache lines
-    // per wave).  Measured fp32 GAE (round 3), groups on blockIdx.y -> in lanes: [4096x300x16] 218 -> 82 us (5.3 TB/s),
+    // per wave).  Measured fp32 GAE, groups on blockIdx.y -> in lanes: [4096x300x16] 218 -> 82 us (5.3 TB/s),
     // [8192x100x16] 146 -> 55 (SEQ 129), [1024x300x16] 62 -> 22, [256x300x24] 49 -> 22; few small groups beat fewer large
     // ones (registers): I = 12 as 4 x 3 107 us vs 2 x 6 124 at [4096x300x12], I = 24 as 8 x 3 183 vs 4 x 6 225 at
     // [4096x300x24].  A handful of long rows keeps the old mapping (more blocks: [64x1000x16] 20 vs 29 us).

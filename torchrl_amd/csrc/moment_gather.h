@@ -9,7 +9,7 @@
 //   * every spin is bounded (1 s wall clock); a wave that gives up re-tags what it published with the PREVIOUS tag so
 //     that nothing of it can match the next launch's tag, and reports failure to its caller.
 // Measured at C4 (tools/kbench/kfused3.hip, kxchg.hip): 1 / 4 / 8 / 16 / 32 replicas 7.81 / 7.48 / 7.45 / 7.49 / 7.58 us per
-// launch; one 128-byte line per block polled with 8-byte loads (round 2) 7.95; line strides of 256 B - 16 KB no better;
+// launch; one 128-byte line per block polled with 8-byte loads 7.95; line strides of 256 B - 16 KB no better;
 // two-level gathers (16 x 16, 8 x 32 groups) 7.5 - 7.7; two poll rounds in flight: slower.
 // Rule for the callers: EVERY slot of the workspace is rewritten by EVERY launch (by the block that owns it, or -- grids
 // smaller than the layout's stride -- by refresh_absent_slots): a stale tag is then at most one launch old and never matches.

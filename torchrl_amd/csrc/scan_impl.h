@@ -130,7 +130,7 @@ __global__ __launch_bounds__(kShortThreads) void scan_short_kernel(typename Op::
 
 // ---- SHORT rows with feature dims (I > 1, T*I <= chunk): gae_interleaved.h ---------------------------------
 // (the generic transposing kernel that lived here -- every input array staged through LDS, the Op's own scan_chunk on the
-// gathered rows -- served TD(lambda) / TD(1) / V-trace until round 3; all four estimators now run on the map-forming kernel of
+// gathered rows -- served TD(lambda) / TD(1) / V-trace before; all four estimators now run on the map-forming kernel of
 // gae_interleaved.h, which moves 2 arrays instead of 5 - 7 across LDS.  make_plan below still lays the chunks out for it.)
 
 // ---- LONG rows: one team per block walks (row, chunk) pairs from each row's end -----------------

@@ -1,5 +1,5 @@
 // Cross-GPU exchange of the advantage moments {N, sum, sumsq}: the one collective of the path
-// (SURVEY.md 8e; reference semantics: adv.mean() / adv.std() over ALL elements,
+// (reference semantics: adv.mean() / adv.std() over ALL elements,
 // torchrl/objectives/value/advantages.py:1459-1463, when the env dimension is sharded over GPUs).
 //
 // 24 bytes per rank is far below the size where a ring or tree pays: every rank WRITES its three

@@ -1,13 +1,13 @@
 """``torch.library`` custom ops over the C-ABI entry points, so that the estimators are ``torch.compile``-friendly.
 
-SURVEY.md 8(b): the reference flips its estimators to the Python loop under dynamo (advantages.py:1303-1307); here every
+The reference flips its estimators to the Python loop under dynamo (advantages.py:1303-1307); here every
 estimator is ONE opaque op with a fake (meta) implementation, so ``torch.compile(fullgraph=True)`` traces through a
 PPO-style function without graph breaks.  The ops are used ONLY while compiling or recording (``functional._recording``):
 the eager entry points call the library directly -- the dispatcher's per-call cost is several times the small kernels.
 
 Each op's implementation is the eager entry point itself (ctypes underneath); ``register_autograd`` wires the backward
 kernels (``trl_gae_bwd`` / ``trl_td_lambda_bwd`` / ``trl_td1_bwd`` / ``trl_vtrace_bwd``) for the value / reward /
-log-probability inputs.  Gradients w.r.t. gamma / lmbda TENSORS (round 3): GAE, TD(lambda) with rolling gamma and V-trace's
+log-probability inputs.  Gradients w.r.t. gamma / lmbda TENSORS: GAE, TD(lambda) with rolling gamma and V-trace's
 gamma -- the tensor enters the op as a differentiable view of the inputs' shape (``_split_leaf``) and the backward forms its
 per-element gradient with torch ops on the kernel's adjoint, as the eager Functions do; TD(1) and the
 ``rolling_gamma=False`` forms keep coefficient gradients eager-only.
@@ -219,7 +219,7 @@ def _(g_ret, next_state_value, reward, done, terminated, gamma, lmbda, gamma_t, 
 
 def _td_setup(ctx, inputs, output):
     next_state_value, reward, done, terminated, gamma, lmbda, gamma_t, lmbda_t, rolling, time_dim, vec = inputs
-    ctx.fixed = rolling == 0 and (gamma_t is not None or lmbda_t is not None)  # rolling_gamma=False: trl_td_fixed_bwd (ADVICE r2)
+    ctx.fixed = rolling == 0 and (gamma_t is not None or lmbda_t is not None)  # rolling_gamma=False: trl_td_fixed_bwd
     need = ctx.needs_input_grad
     ctx.coef_grads = (gamma_t is not None and need[6], lmbda_t is not None and need[7])
     if any(ctx.coef_grads) and ctx.fixed:

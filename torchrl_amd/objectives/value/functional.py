@@ -100,7 +100,7 @@ def _expand_coef(x: torch.Tensor, shape, time_dim: int) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------------------------------------
-# coefficient rounding (SURVEY.md fact 3 / appendix A1-A3)
+# coefficient rounding
 # ---------------------------------------------------------------------------------------------
 _F32 = struct.Struct("f")
 
@@ -620,7 +620,7 @@ def _keep_call(ctx, call):
     """Keep the prepared call for backward together with the version counters of its tensors.  The call holds detached
     aliases of the caller's tensors (same storage, same version counter when no conversion was needed) and the backward
     kernels re-read them: an in-place update of a rollout buffer between forward and backward must raise, as torch's own
-    autograd does for saved tensors, instead of giving silently wrong gradients (ADVICE r2)."""
+    autograd does for saved tensors, instead of giving silently wrong gradients."""
     ctx.call = call
     ctx.versions = tuple((name, t, t._version) for name, t in vars(call).items() if isinstance(t, torch.Tensor))
 
@@ -901,7 +901,7 @@ class _VtraceFunction(torch.autograd.Function):
 # ---------------------------------------------------------------------------------------------
 # GAE fast path: the common call (python-float gamma / lmbda, contiguous same-dtype tensors on the current
 # device, time at dim -2, no autograd) goes from the public signature to ONE ctypes call without building the
-# general call description -- the general path costs 2 - 4x the kernel at the small BASELINE shapes.  Anything
+# general call description -- the general path costs 2 - 4x the kernel at small shapes.  Anything
 # else (and every error) falls through to the general path, which validates and raises as the reference does.
 # ---------------------------------------------------------------------------------------------
 _FAST_COEF = {}   # (gamma, lmbda, default dtype) -> (gamma rounded, lmbda*gamma rounded, coefficient dtype code)
@@ -1758,7 +1758,7 @@ def vtrace_advantage_estimate(
 
 
 # ---------------------------------------------------------------------------------------------
-# TD(0), TD(1), reward-to-go -- "next" rows of SURVEY.md 8(f).  TD(1) has its own kernels (trl_td1_fwd: the
+# TD(0), TD(1), reward-to-go.  TD(1) has its own kernels (trl_td1_fwd: the
 # reference's TD(1) loops differ from TD(lambda) at lmbda = 1 in the start value and in how masks enter);
 # vec TD(1) is vec TD(lambda) with lmbda = 1, exactly as functional.py:691-700 does.
 # ---------------------------------------------------------------------------------------------
