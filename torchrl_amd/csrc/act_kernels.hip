@@ -577,7 +577,8 @@ __global__ __launch_bounds__(256) void act_column_sum_kernel(WeightGradArgs a) {
 
 // Tile and splits: the cheapest of a few by a count of clocks.  A block costs `clocks` a token (measured with the chip full, `slots`
 // blocks at a time; the head and tail of a block as two steps more), the parts of a split sum are written and read at 1900 bytes a clock,
-// and joining them is a launch of its own.
+// and joining them is a launch of its own.  By the count and measured, us at 2.4 GHz without the join: 8192 x 2048 x 8192 bf16 267 and 260-282,
+// 8192 x 2048 x 2048 fp32 277 and 257-275, 65536 x 257 x 13 bf16 25 and 22, fp32 38 and 29.
 struct WeightGradPlan { int bm, bn, bk; i64 tiles_d, tiles, part; int splits; };
 WeightGradPlan weight_grad_plan(int dtype, i64 N, i64 O, i64 D) {
     WeightGradPlan p{};
