@@ -853,6 +853,8 @@ def _vtrace_bwd(c, g_adv, g_vs, vs, need, need_gamma: bool):
     outs = [new(n) for n in need]
     d_gamma_t = new(need_gamma, odt)
     vs = vs.detach()
+    if vs.numel() != c.O * c.T * c.I or vs.device != dev:
+        raise RuntimeError(f"torchrl_amd: V-trace's kept values came back from their saved-tensor hook as {tuple(vs.shape)} on {vs.device}")
     if vs.dtype != odt:
         vs = vs.to(odt)
     vs = vs.contiguous()
